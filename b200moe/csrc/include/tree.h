@@ -1,0 +1,70 @@
+// Host interface of the draft-tree operators: attention of a tree's nodes over the
+// paged pool (kernels/tree_attn.cu) and the commit of its accepted path
+// (kernels/tree_commit.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+
+#include "attention.h"
+
+namespace b200 {
+
+constexpr int kTreeMaxNodes = 256;   // nodes of one tree
+
+struct TreeAttnArgs {
+  const void* q;             // [rows, q_heads, D] bf16
+  const void* k_cache;       // layer base of the pool, [blocks, kv_heads, block_size, D]
+  const void* v_cache;
+  const float* k_scale;      // kv_int8 == 1: [blocks, kv_heads, block_size] (strided over blocks)
+  const float* v_scale;
+  int kv_int8;               // 0 bf16, 1 int8 per-token scales, 2 int8 channel mode (ch)
+  KvChannel ch;
+  const int* cu_seqlens_q;   // [batch + 1] first node of each sequence
+  const int* seq_lens;       // [batch] keys: committed prefix + nodes
+  const int* block_tables;   // [batch, max_blocks]
+  const int* parents;        // [rows] place of a node's parent in its tree, -1: none
+  int batch;
+  int rows;
+  int max_blocks;
+  int num_blocks;
+  int block_size;
+  int64_t block_stride;      // elements between consecutive blocks of one layer
+  int64_t scale_block_stride;
+  int num_kv_heads;
+  int group;                 // q heads per kv head
+  int head_dim;
+  float scale;
+  void* out;                 // [rows, q_heads, D] bf16
+  int* status;               // device status word
+};
+void tree_attn(const TreeAttnArgs& a, cudaStream_t s);
+
+// One kind of rows the commit moves: [blocks, planes, block_size, row_bytes], contiguous.
+struct TreeRows {
+  uint8_t* base;
+  int row_bytes;
+};
+struct TreeCommitArgs {
+  TreeRows rows[3];          // payload, int8 scales, channel-mode side values
+  int kinds;
+  int planes;                // layers * 2 * kv_heads
+  int block_size;
+  int num_blocks;
+  const int* cu_seqlens_q;   // [batch + 1]
+  const int* seq_lens;       // [batch] committed prefix + nodes
+  const int* block_tables;   // [batch, max_blocks]
+  const int* parents;        // [nodes]
+  const int* draft;          // [nodes] drafted token of each node
+  const int* target;         // [nodes] token the model picks behind each node
+  int batch;
+  int nodes;                 // entries of parents / draft / target
+  int max_blocks;
+  int max_q_len;             // row length of path / tokens
+  int* accepted;             // [batch]
+  int* path;                 // [batch, max_q_len], -1 behind the path
+  int* tokens;               // [batch, max_q_len], -1 behind the path
+  int* status;
+};
+void tree_commit(const TreeCommitArgs& a, cudaStream_t s);
+
+}  // namespace b200

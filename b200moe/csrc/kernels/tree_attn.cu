@@ -1,0 +1,154 @@
+// Attention of the nodes of drafted trees over the paged pool.
+//
+//   o_i = sum_j p_ij v_j,   p_ij = softmax_j(scale * q_i . k_j)
+//
+// where j runs over the committed prefix [0, P) of node i's sequence and over node i
+// and its ancestors, whose keys sit at positions P + node.
+//
+// One warp per (node, query head): a lane scores one key of 32, the warp keeps the
+// running maximum and sum in fp32, and each lane accumulates D / 32 columns of o.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+
+#include "pdl.cuh"
+#include "sm100.cuh"
+#include "tree.h"
+
+namespace b200 {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+constexpr int kWarps = 4;
+
+// Element d of a stored row as the float it stands for.
+template <int MODE>
+__device__ __forceinline__ float kv_value(const TreeAttnArgs& a, const void* pool, const void* side, int kv, int64_t blk,
+                                          int h, int y, int d, float row_scale) {
+  const int64_t at = blk * a.block_stride + ((int64_t)h * a.block_size + y) * a.head_dim + d;
+  if (MODE == 0) return __bfloat162float(static_cast<const bf16*>(pool)[at]);
+  const float q = (float)static_cast<const int8_t*>(pool)[at];
+  if (MODE == 1) return q * row_scale;
+  const int n_out = a.ch.n_out[h];
+  for (int o = 0; o < n_out; ++o)
+    if (a.ch.out_idx[h * kKvNoutMax + o] == d)
+      return __bfloat162float(static_cast<const bf16*>(side)[blk * a.ch.side_block_stride +
+                                                             ((int64_t)h * a.block_size + y) * kKvNoutMax + o]);
+  // the channel mode's values are bf16 by definition, as its other readers round them
+  return __bfloat162float(__float2bfloat16(q * a.ch.dscale[((int64_t)kv * a.num_kv_heads + h) * a.head_dim + d]));
+}
+
+template <int D, int MODE>
+__global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnArgs a) {
+  pdl_enter();
+  __shared__ int s_par[kTreeMaxNodes];
+  __shared__ float s_q[kWarps][D];
+  const int row = blockIdx.x, h = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the sequence that holds this row: last b with cu[b] <= row
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid;
+  }
+  const int b = lo, q0 = a.cu_seqlens_q[b], n = a.cu_seqlens_q[b + 1] - q0, node = row - q0;
+  if (node < 0 || node >= n) return;  // rows behind the last sequence
+  const int len = a.seq_lens[b], prefix = len - n;
+  if (n > kTreeMaxNodes || prefix < 0 || q0 < 0 || q0 + n > a.rows) {
+    if (threadIdx.x == 0) record_status(a.status, kStatusBadShape);
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += kWarps * 32) s_par[i] = a.parents[q0 + i];
+  __syncthreads();
+  const int* tab = a.block_tables + (int64_t)b * a.max_blocks;
+  const float sl2 = a.scale * 1.4426950408889634f;
+  bool bad = false;
+  for (int g = warp; g < a.group; g += kWarps) {
+    const int64_t qrow = ((int64_t)row * a.num_kv_heads * a.group + h * a.group + g) * D;
+    for (int d = lane; d < D; d += 32) s_q[warp][d] = __bfloat162float(static_cast<const bf16*>(a.q)[qrow + d]);
+    __syncwarp();
+    float m = -INFINITY, l = 0.f, o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+    for (int k0 = 0; k0 < len; k0 += 32) {
+      const int key = k0 + lane;
+      bool see = key < prefix;
+      if (!see && key < len) {
+        for (int at = node; at >= 0;) {  // this node's ancestors; a parent behind its child ends the walk
+          if (at == key - prefix) { see = true; break; }
+          const int up = s_par[at];
+          at = up < at ? up : -1;
+        }
+      }
+      int64_t blk = 0;
+      const int bi = key / a.block_size, y = key % a.block_size;
+      if (see) {
+        blk = bi < a.max_blocks ? tab[bi] : -1;
+        if (blk < 0 || blk >= a.num_blocks) { bad = true; see = false; blk = 0; }
+      }
+      float ks = 1.f, vs = 1.f;
+      if (MODE == 1 && see) {
+        const int64_t at = blk * a.scale_block_stride + (int64_t)h * a.block_size + y;
+        ks = a.k_scale[at];
+        vs = a.v_scale[at];
+      }
+      float s = -INFINITY;
+      if (see) {
+        s = 0.f;
+        for (int d = 0; d < D; ++d)
+          s = fmaf(s_q[warp][d], kv_value<MODE>(a, a.k_cache, a.ch.side_k, 0, blk, h, y, d, ks), s);
+        s *= sl2;
+      }
+      const float mn = fmaxf(m, warp_max(s));
+      if (mn == -INFINITY) continue;
+      const float alpha = exp2f(m - mn);  // m = -inf: 0
+      const float p = see ? exp2f(s - mn) : 0.f;
+      m = mn;
+      l = l * alpha + warp_sum(p);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+      for (int j = 0; j < 32; ++j) {
+        const float pj = __shfl_sync(0xffffffffu, p, j);
+        const bool sj = __shfl_sync(0xffffffffu, see, j);
+        const int64_t bj = __shfl_sync(0xffffffffu, blk, j);
+        const float vj = __shfl_sync(0xffffffffu, vs, j);
+        if (!sj) continue;
+        const int yj = (k0 + j) % a.block_size;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          o[i] = fmaf(pj, kv_value<MODE>(a, a.v_cache, a.ch.side_v, 1, bj, h, yj, i * 32 + lane, vj), o[i]);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      static_cast<bf16*>(a.out)[qrow + i * 32 + lane] = __float2bfloat16(o[i] * inv);
+    __syncwarp();
+  }
+  if (bad) record_status(a.status, kStatusBadShape);
+  pdl_trigger();
+}
+
+template <int D>
+void launch(const TreeAttnArgs& a, cudaStream_t s) {
+  const dim3 grid(a.rows, a.num_kv_heads);
+  if (a.kv_int8 == 0) pdl_launch(tree_attn_kernel<D, 0>, grid, kWarps * 32, 0, s, a);
+  else if (a.kv_int8 == 1) pdl_launch(tree_attn_kernel<D, 1>, grid, kWarps * 32, 0, s, a);
+  else pdl_launch(tree_attn_kernel<D, 2>, grid, kWarps * 32, 0, s, a);
+}
+
+}  // namespace
+
+void tree_attn(const TreeAttnArgs& a, cudaStream_t s) {
+  if (a.rows == 0 || a.batch == 0) return;
+  if (a.head_dim == 128) launch<128>(a, s);
+  else launch<64>(a, s);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("tree_attn: ") + cudaGetErrorString(e));
+}
+
+}  // namespace b200

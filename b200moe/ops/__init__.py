@@ -485,6 +485,73 @@ def moe_permute(x, ids, counts, cursor, x_perm, slot_of_row, offsets_out=None):
     count_launches()
 
 
+MOE_FEW_MAX_TOKENS = 64
+
+
+def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True, out=None, ids=None, weights=None,
+                   tiled: bool = False):
+    """A whole MoE layer for a few tokens in one launch: out [T, H] = sum_k w_k FFN_{e_k}(x), T <=
+    ``MOE_FEW_MAX_TOKENS``, with the router's rounding points (bf16 logits and weights, the lowest
+    expert id wins a tie).  w13 [E, 2I, H] and w2 [E, H, I] are e4m3 with 128 x 128 block scales
+    (``tiled``: stored by ``tile_fp8``) or bf16 (s13 = s2 = None); every expert is on this GPU.
+    ``ids`` [T, topk] int32 / ``weights`` [T, topk] fp32 receive the routing.  An e4m3 weight enters as
+    q * scale in fp32, where the grouped GEMMs round that product to bf16 first."""
+    if x.dim() != 2 or not x.is_contiguous():
+        raise ValueError("x must be contiguous [tokens, hidden]")
+    T, H = x.shape
+    if T > MOE_FEW_MAX_TOKENS:
+        raise ValueError(f"moe_few_tokens takes at most {MOE_FEW_MAX_TOKENS} tokens, got {T}")
+    if w13.dim() != 3 or w2.dim() != 3 or w13.shape != (num_experts, 2 * w2.shape[2], H) or w2.shape[:2] != (
+            num_experts, H):
+        raise ValueError("w13 must be [E, 2I, H] and w2 [E, H, I]")
+    if not 1 <= topk <= min(8, num_experts) or num_experts > 256:
+        raise ValueError("topk must be in [1, min(8, num_experts)] and num_experts at most 256")
+    if (s13 is None) != (s2 is None) or (s13 is None) == (w13.dtype == torch.float8_e4m3fn) or w2.dtype != w13.dtype:
+        raise ValueError("expert weights are both e4m3 with scales or both unquantised without")
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+        raise ValueError("out must be like x")
+    if not x.is_cuda:
+        return _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled)
+    if H % 128 or w2.shape[2] % 128:
+        raise ValueError("hidden and intermediate sizes must be multiples of 128")
+    if T:
+        native().moe_few(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled,
+                         status_word(x.device))
+        count_launches()
+    return out
+
+
+def _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled):
+    T = x.shape[0]
+    logits = (x.double() @ router_w[:num_experts].double().t()).to(torch.bfloat16).float()
+    p = torch.softmax(logits, dim=-1)
+    e = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :topk]
+    w = p.gather(1, e)
+    if renorm:
+        w = w / w.sum(dim=-1, keepdim=True)
+    w = w.to(torch.bfloat16).float()
+    if ids is not None:
+        ids.copy_(e.to(ids.dtype))
+    if weights is not None:
+        weights.copy_(w)
+    I = w2.shape[2]
+    y = torch.zeros(T, topk, x.shape[1])
+
+    def natural(wt, sc, g):
+        if sc is None:
+            return wt[g].float()
+        return dequant_block_fp8(untile_fp8(wt[g]) if tiled else wt[g], sc[g])
+
+    for g in torch.unique(e).tolist():
+        t_idx, k_idx = (e == g).nonzero(as_tuple=True)
+        gu = x[t_idx].float() @ natural(w13, s13, g).t()
+        h = torch.nn.functional.silu(gu[:, :I]) * gu[:, I:]
+        y[t_idx, k_idx] = (h @ natural(w2, s2, g).t()) * w[t_idx, k_idx, None]
+    return out.copy_(y.sum(dim=1))
+
+
 def _chan_read(kv_layer) -> list[int]:
     """Device pointers of the int8 channel mode's read side (attention kernels), or []."""
     c = kv_layer.chan
@@ -595,6 +662,142 @@ def _attention_ref(q, kv_layer, block_tables, seq_lens, cu_seqlens_q, scale, out
         o = torch.einsum("hgqk,khd->qhgd", p, v.float()).reshape(qlen, nq, D)
         out[q0:q1] = o.to(out.dtype)
     return out
+
+
+# ------------------------------------------------------------- drafted trees
+TREE_MAX_NODES = 256   # nodes of one drafted tree
+
+
+def _check_tree(rows, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, device):
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens), ("block_tables", block_tables),
+                    ("parents", parents)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+    if cu_seqlens_q.dim() != 1 or seq_lens.dim() != 1 or cu_seqlens_q.shape[0] != seq_lens.shape[0] + 1:
+        raise ValueError("cu_seqlens_q must hold one entry more than seq_lens")
+    if block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0] or block_tables.shape[1] < 1:
+        raise ValueError("block_tables must be [batch, max_blocks]")
+    if parents.dim() != 1 or (rows is not None and parents.shape[0] != rows):
+        raise ValueError("parents must hold one entry per row")
+    if not 1 <= max_q_len <= TREE_MAX_NODES:
+        raise ValueError(f"max_q_len must be in [1, {TREE_MAX_NODES}], got {max_q_len}")
+
+
+def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, scale, out=None):
+    """Attention of drafted trees over the paged pool: each node sees its sequence's
+    committed prefix, its ancestors and itself.
+
+    q [rows, nq, D]: the nodes of sequence b are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] and node
+    i's key sits at position seq_lens[b] - n_b + i (seq_lens counts prefix and nodes; the keys are
+    stored before the call, as for ``prefill_attention``).  parents [rows]: place of a node's parent in
+    its tree, below the node's own; -1 for a node that follows the prefix directly.  max_q_len: no tree
+    has more nodes (at most ``TREE_MAX_NODES``).  Chains (parents i - 1) give causal attention.  Rows
+    behind the last sequence are left as they are.  bf16 and int8 pools, head_dim 64 or 128.  A tree
+    that does not fit (offsets outside q, more nodes than keys or than max_q_len) is left out and a
+    block id outside the pool is not read; both set the status word (``check_status``)."""
+    if q.dim() != 3 or not q.is_contiguous():
+        raise ValueError("q must be contiguous [rows, q_heads, head_dim]")
+    _check_tree(q.shape[0], cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, q.device)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
+        raise ValueError("out must be like q")
+    if q.shape[1] % kv_layer.num_kv_heads:
+        raise ValueError("q heads must be a multiple of kv heads")
+    if not q.is_cuda:
+        return _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out)
+    if q.shape[0] and seq_lens.shape[0]:
+        native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q, seq_lens,
+                           block_tables, parents, out, max_q_len, kv_layer.block_size, kv_layer.block_stride,
+                           kv_layer.scale_block_stride, scale, status_word(q.device), _chan_read(kv_layer))
+        count_launches()
+    return out
+
+
+def _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out):
+    """fp32 tree attention over the paged pool, one sequence at a time."""
+    nq, D = q.shape[1], q.shape[2]
+    nkv = kv_layer.num_kv_heads
+    cu, lens, par = cu_seqlens_q.tolist(), seq_lens.tolist(), parents.tolist()
+    for b, L in enumerate(lens):
+        q0, n = cu[b], cu[b + 1] - cu[b]
+        if n <= 0:
+            continue
+        if L < n or q0 < 0 or q0 + n > q.shape[0]:
+            raise ValueError(f"sequence {b}: {n} nodes at row {q0} do not fit its {L} keys or the {q.shape[0]} rows")
+        k, v = (t.float() for t in kv_layer.gather(block_tables[b], L))
+        for i in range(n):   # one node's keys at a time: what it does not see is not touched, NaN or not
+            seen, at = [], i
+            while at >= 0:
+                seen.append(L - n + at)
+                up = par[q0 + at]
+                at = up if up < at else -1
+            idx = torch.tensor(list(range(L - n)) + seen[::-1], device=q.device)
+            qf = q[q0 + i].float().view(nkv, nq // nkv, D)
+            p = torch.softmax(torch.einsum("hgd,khd->hgk", qf, k[idx]) * scale, dim=-1)
+            out[q0 + i] = torch.einsum("hgk,khd->hgd", p, v[idx]).reshape(nq, D).to(out.dtype)
+    return out
+
+
+def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids, max_q_len,
+                kv_scales=None, kv_side=None):
+    """Accept one path of every drafted tree and keep its cache rows.
+
+    draft_ids [rows]: drafted token of each node (node 0: the sequence's last emitted token);
+    target_ids [rows]: the token the model picks behind each node (``argmax`` or ``sample`` of its
+    logits).  The path starts at node 0 and goes on to the lowest child whose drafted token is the
+    picked one.  The rows of the path, at positions P + node behind the committed prefix P =
+    seq_lens - nodes, move to P, P + 1, ... in every layer of ``kv_data`` (``KVPool.data``, with its
+    ``scales`` and ``side`` where it has them), in place.  Blocks that hold nodes belong to one
+    sequence.  Returns int32 (accepted [B], path [B, max_q_len], tokens [B, max_q_len]): nodes on the
+    path, their places and the tokens to emit behind them, -1 behind the path; the committed length is
+    P + accepted.  A malformed row accepts nothing, a move through a block id outside the pool is left
+    out; both set the status word."""
+    _check_tree(None, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, kv_data.device)
+    for name, t in (("draft_ids", draft_ids), ("target_ids", target_ids)):
+        if t.dtype != torch.int32 or t.shape != parents.shape or t.device != kv_data.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be int32 like parents")
+    if kv_data.dim() != 6 or kv_data.shape[2] != 2 or not kv_data.is_contiguous():
+        raise ValueError("kv_data must be contiguous [blocks, layers, 2, kv_heads, block_size, head_dim]")
+    for name, t in (("kv_scales", kv_scales), ("kv_side", kv_side)):
+        if t is not None and (t.shape[:5] != kv_data.shape[:5] or not t.is_contiguous() or t.device != kv_data.device):
+            raise ValueError(f"{name} must be contiguous rows [blocks, layers, 2, kv_heads, block_size] like kv_data")
+    if not kv_data.is_cuda:
+        return _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids,
+                                max_q_len, kv_scales, kv_side)
+    res = native().tree_commit(kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids,
+                               target_ids, max_q_len, status_word(kv_data.device))
+    count_launches(1 if seq_lens.shape[0] else 0)
+    return res
+
+
+def _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids, max_q_len,
+                     kv_scales, kv_side):
+    B, bs = seq_lens.shape[0], kv_data.shape[4]
+    accepted = torch.zeros(B, dtype=torch.int32)
+    path = torch.full((B, max_q_len), -1, dtype=torch.int32)
+    tokens = torch.full((B, max_q_len), -1, dtype=torch.int32)
+    cu, lens = cu_seqlens_q.tolist(), seq_lens.tolist()
+    for b in range(B):
+        q0, n = cu[b], cu[b + 1] - cu[b]
+        if n == 0:
+            continue
+        if n < 0 or n > max_q_len or q0 < 0 or q0 + n > parents.shape[0] or lens[b] < n:
+            raise ValueError(f"sequence {b}: {n} nodes at row {q0} do not fit")
+        par, dr, ta = (t[q0:q0 + n].tolist() for t in (parents, draft_ids, target_ids))
+        at, j = 0, 0
+        while at is not None:
+            path[b, j], tokens[b, j] = at, ta[at]
+            j += 1
+            at = next((c for c in range(at + 1, n) if par[c] == at and dr[c] == ta[at]), None)
+        accepted[b] = j
+        for i, node in enumerate(path[b, :j].tolist()):
+            src, dst = lens[b] - n + node, lens[b] - n + i
+            sb, db = int(block_tables[b, src // bs]), int(block_tables[b, dst // bs])
+            for t in (kv_data, kv_scales, kv_side):
+                if t is not None and src != dst:
+                    t[db, :, :, :, dst % bs] = t[sb, :, :, :, src % bs]
+    return accepted, path, tokens
 
 
 # ---------------------------------------------------------------- sampler

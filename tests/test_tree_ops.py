@@ -1,0 +1,429 @@
+"""Draft-tree operators: tree attention over the paged pool, the commit of the accepted path and the
+few-token MoE layer, against plain 64-bit implementations written here."""
+import math
+
+import pytest
+import torch
+
+from b200moe import ops
+from b200moe.engine.kv_cache import KVPool
+from b200moe.utils.weights import quantize_block_fp8
+
+HALF = torch.finfo(torch.bfloat16).eps / 2   # a bf16 rounding is off by at most this, relative to the value
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _tree(n, kind, gen):
+    """Parents of a tree of n nodes."""
+    if kind == "chain":
+        return list(range(-1, n - 1))
+    if kind == "star":
+        return [-1] + [0] * (n - 1)
+    if kind == "forest":   # several nodes follow the prefix directly
+        return [-1 if i % 3 == 0 else i - 1 for i in range(n)]
+    r = torch.rand(n, generator=gen).tolist()
+    return ([-1] + [int(r[i] * i) for i in range(1, n)])[:n]
+
+
+def _sees(par):
+    n = len(par)
+    m = torch.zeros(n, n, dtype=torch.bool)
+    for i in range(n):
+        j = i
+        while j >= 0:
+            m[i, j] = True
+            j = par[j]
+    return m
+
+
+class Batch:
+    """Pool, tables and trees of a ragged batch; ``pad`` rows of q behind the last sequence."""
+
+    def __init__(self, dev, nodes, ctx, nq, nkv, D, bs, kind="random", int8=False, mode="token", pad=0, seed=0,
+                 dtype=torch.bfloat16, layers=2, layer=1):
+        g = torch.Generator().manual_seed(seed)
+        need = [max(1, -(-(n + c) // bs)) for n, c in zip(nodes, ctx)]
+        self.pool = KVPool(sum(need) + 1, layers, nkv, bs, D, dtype, dev, int8=int8, int8_mode=mode)
+        ids = torch.randperm(sum(need), generator=g).tolist()
+        tab = torch.zeros(len(nodes), max(need) + 1, dtype=torch.int32)
+        at = 0
+        for b, k in enumerate(need):
+            tab[b, :k] = torch.tensor(ids[at:at + k])
+            at += k
+        self.tables = tab.to(dev)
+        if int8:
+            self.pool.data.copy_(torch.randint(-127, 128, self.pool.data.shape, generator=g, dtype=torch.int8))
+            if self.pool.scales is not None:
+                self.pool.scales.copy_(torch.rand(self.pool.scales.shape, generator=g) * 0.02 + 0.002)
+            else:
+                self.pool.side.copy_(torch.randn(self.pool.side.shape, generator=g))
+                self.pool.ch_scale.copy_(torch.rand(self.pool.ch_scale.shape, generator=g) * 0.02 + 0.002)
+                self.pool.ch_dscale.copy_(self.pool.ch_scale)
+                self.pool.n_out.fill_(2)
+                self.pool.out_idx[..., 0] = 3
+                self.pool.out_idx[..., 1] = D - 1
+                for d in (3, D - 1):
+                    self.pool.ch_dscale[..., d] = 0.0
+        else:
+            self.pool.data.copy_(torch.randn(self.pool.data.shape, generator=g))
+        self.nodes, self.ctx, self.D, self.nq, self.nkv = nodes, ctx, D, nq, nkv
+        cu = [0]
+        for n in nodes:
+            cu.append(cu[-1] + n)
+        self.cu_list = cu
+        self.trees = [_tree(n, kind, g) for n in nodes]
+        par = [p for t in self.trees for p in t] + [-1] * pad
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.cu = torch.tensor(cu, **i32)
+        self.lens = torch.tensor([n + c for n, c in zip(nodes, ctx)], **i32)
+        self.parents = torch.tensor(par, **i32)
+        self.q = (torch.randn(cu[-1] + pad, nq, D, generator=g) * 2).to(dtype).to(dev)
+        self.layer = self.pool.layer(layer)
+        self.scale = D ** -0.5
+        self.max_nodes = max(max(nodes), 1)
+
+    def args(self):
+        return (self.q, self.layer, self.cu, self.lens, self.tables, self.parents, self.max_nodes, self.scale)
+
+    def exact(self):
+        """(o, sum_j p_ij |v_j|) in 64 bits."""
+        q = self.q.double().cpu()
+        out, mass = torch.zeros_like(q), torch.zeros_like(q)
+        for b, (n, c) in enumerate(zip(self.nodes, self.ctx)):
+            if n == 0:
+                continue
+            k, v = (t.double().cpu() for t in self.layer.gather(self.tables[b], n + c))
+            see = torch.cat([torch.ones(n, c, dtype=torch.bool), _sees(self.trees[b])], dim=1)
+            s0 = self.cu_list[b]
+            for h in range(self.nq):
+                kv = h // (self.nq // self.nkv)
+                z = q[s0:s0 + n, h] @ k[:, kv].t() * self.scale
+                p = torch.softmax(z.masked_fill(~see, -math.inf), dim=1)
+                out[s0:s0 + n, h] = p @ v[:, kv]
+                mass[s0:s0 + n, h] = p @ v[:, kv].abs()
+        return out, mass
+
+    def check(self, got):
+        """The output is rounded to bf16 once (HALF of its value), and a kernel may round each p_ij to
+        bf16 in front of the product and in the sum that divides it (HALF of the mass, twice).  fp32
+        scores of at most a few hundred add less than 2^-13 of the mass."""
+        o, mass = self.exact()
+        n = self.cu_list[-1]
+        err = (got[:n].double().cpu() - o[:n]).abs()
+        lim = HALF * o[:n].abs() + (2 * HALF + 2 ** -13) * mass[:n] + 1e-30
+        assert bool((err <= lim).all()), float((err / lim).max())
+
+
+ATTN = [
+    # nodes, ctx, nq, nkv, D, block
+    ([1], [0], 4, 2, 64, 16),
+    ([8], [500], 32, 4, 128, 256),
+    ([5, 1, 17, 0, 3], [0, 1, 130, 40, 255], 8, 4, 128, 64),
+    ([16, 9], [128, 127], 16, 1, 128, 128),          # 16 query heads on one KV head
+    ([7, 33], [100, 300], 6, 2, 64, 32),             # a group of three
+    ([4, 3, 2], [1023, 1025, 64], 8, 8, 128, 128),   # one query head per KV head
+    ([40, 64], [700, 65], 32, 4, 128, 16),           # several row tiles, pages that end inside a key tile
+    ([3, 20], [50, 77], 4, 2, 64, 24),               # a block size that no tile divides into
+]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nodes,ctx,nq,nkv,D,bs", ATTN)
+@pytest.mark.parametrize("kind", ["random", "chain", "forest"])
+def test_tree_attention(dev, nodes, ctx, nq, nkv, D, bs, kind):
+    b = Batch(dev, nodes, ctx, nq, nkv, D, bs, kind)
+    got = ops.tree_attention(*b.args())
+    b.check(got)
+    if dev == "cuda":
+        ops.check_status(got.device)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("mode", ["token", "channel"])
+@pytest.mark.parametrize("D,bs", [(128, 64), (64, 16)])
+def test_tree_attention_int8(dev, mode, D, bs):
+    b = Batch(dev, [9, 1, 24], [40, 300, 0], 8, 2, D, bs, int8=True, mode=mode)
+    b.check(ops.tree_attention(*b.args()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_chain_is_prefill(dev):
+    """A chain sees what causal prefill sees."""
+    b = Batch(dev, [6, 13], [33, 190], 8, 2, 128, 32, "chain")
+    got = ops.tree_attention(*b.args())
+    ref = ops.prefill_attention(b.q, b.layer, b.cu, b.lens, b.tables, 13, b.scale, torch.empty_like(b.q))
+    _, mass = b.exact()
+    lim = 2 * (HALF + 2 * HALF + 2 ** -13) * mass    # both are within check()'s bound of the exact value
+    assert bool(((got.double() - ref.double()).abs().cpu() <= lim).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_leaves_padding_rows(dev):
+    b = Batch(dev, [3, 5], [20, 70], 8, 2, 128, 16, pad=4)
+    out = torch.full_like(b.q, 7.0)
+    assert ops.tree_attention(*b.args(), out=out) is out
+    assert bool((out[8:] == 7.0).all())
+    b.check(out)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_ignores_what_it_does_not_see(dev):
+    """NaN and infinite keys and values behind the sequence and in other branches change nothing."""
+    b = Batch(dev, [6], [25], 8, 2, 128, 16, "star")
+    want = ops.tree_attention(*b.args()).clone()
+    last = b.tables[0, 30 // 16].item()
+    b.layer.k[last, :, 15:] = math.nan      # slot 31: behind the last node (30 keys + 1)
+    b.layer.v[last, :, 15:] = math.inf
+    node = 25 + 4                            # node 4: a leaf that only itself sees
+    blk = b.tables[0, node // 16].item()
+    b.layer.k[blk, :, node % 16] = math.nan
+    b.layer.v[blk, :, node % 16] = math.nan
+    got = ops.tree_attention(*b.args())
+    keep = [i for i in range(6) if i != 4]
+    assert torch.equal(got[keep], want[keep])
+    assert bool(torch.isnan(got[4].float()).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_large_scores(dev):
+    """Scores of many hundreds: the running maximum keeps the exponentials in range."""
+    b = Batch(dev, [10], [300], 4, 2, 64, 16)
+    b.q *= 50
+    got = ops.tree_attention(*b.args())
+    assert bool(torch.isfinite(got.float()).all())
+    o, mass = b.exact()
+    # fp32 products of 64 terms are off by at most 64 * 2^-24 of their absolute sum (below 12,000 here
+    # in units of log 2), which moves p by that factor
+    z = (b.q.double().abs().amax() * b.layer.k.double().abs().amax() * 64 * b.scale).item()
+    lim = HALF * o.abs() + (2 * HALF + 2 * 64 * 2 ** -24 * z) * mass
+    assert bool(((got.double().cpu() - o).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_empty(dev):
+    b = Batch(dev, [0, 0], [5, 0], 4, 2, 64, 16)
+    assert ops.tree_attention(*b.args()).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_refusals(dev):
+    b = Batch(dev, [4], [20], 8, 2, 128, 16)
+    q, kv, cu, lens, tab, par, n, sc = b.args()
+    bad = [
+        (q, kv, cu, lens, tab, par[:3], n, sc), (q, kv, cu[:1], lens, tab, par, n, sc),
+        (q, kv, cu.long(), lens, tab, par, n, sc), (q, kv, cu, lens, tab[0], par, n, sc),
+        (q, kv, cu, lens, tab, par, 0, sc), (q, kv, cu, lens, tab, par, ops.TREE_MAX_NODES + 1, sc),
+        (q.transpose(0, 1), kv, cu, lens, tab, par, n, sc), (q[:, :3].contiguous(), kv, cu, lens, tab, par, n, sc),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError):
+            ops.tree_attention(*args)
+    with pytest.raises(ValueError):
+        ops.tree_attention(*b.args(), out=torch.empty(3, 8, 128, dtype=q.dtype, device=dev))
+    d = torch.zeros_like(par)
+    for args in [(b.pool.data[0], cu, lens, tab, par, d, d, n), (b.pool.data, cu, lens, tab, par, d[:2], d, n),
+                 (b.pool.data, cu, lens, tab, par, d, d.long(), n), (b.pool.data, cu, lens, tab, par, d, d, 0)]:
+        with pytest.raises(ValueError):
+            ops.tree_commit(*args)
+    with pytest.raises(ValueError):
+        ops.tree_commit(b.pool.data, cu, lens, tab, par, d, d, n, kv_scales=torch.ones(3, device=dev))
+
+
+@pytest.mark.gpu
+def test_tree_bad_metadata_sets_status():
+    """Block ids outside the pool, tables that are too short and trees that do not fit are left out."""
+    for what in ("block", "short", "cu", "prefix"):
+        b = Batch("cuda", [4, 3], [40, 20], 8, 2, 128, 16)
+        q, kv, cu, lens, tab, par, n, sc = b.args()
+        if what == "block":
+            tab[0, 0], tab[0, 1] = 1 << 20, -5
+        elif what == "short":
+            tab = tab[:, :1].contiguous()
+        elif what == "cu":
+            cu[2] = 1 << 20
+        else:
+            lens[0] = 2
+        d = torch.zeros_like(par)
+        before = b.pool.data.clone()
+        ops.tree_attention(q, kv, cu, lens, tab, par, n, sc)
+        with pytest.raises(RuntimeError):
+            ops.check_status(q.device)
+        if what != "block":   # the commit touches the nodes' own blocks only
+            t = torch.full_like(par, 1)
+            d[2] = 1          # accepts a node that has to move
+            par[:4] = torch.tensor([-1, 0, 0, 0], dtype=torch.int32)
+            ops.tree_commit(b.pool.data, cu, lens, tab, par, d, t, n)
+            with pytest.raises(RuntimeError):
+                ops.check_status(q.device)
+            assert what == "cu" or torch.equal(before, b.pool.data)
+
+
+def _commit_case(dev, seed, nodes, ctx, int8=False, mode="token", bs=16, layers=3, nkv=2, D=64):
+    b = Batch(dev, nodes, ctx, 2 * nkv, nkv, D, bs, int8=int8, mode=mode, seed=seed, layers=layers, pad=2)
+    g = torch.Generator().manual_seed(seed + 100)
+    rows = b.parents.shape[0]
+    # few tokens, so that siblings often draft the same one and paths are long
+    draft = torch.randint(0, 3, (rows,), generator=g, dtype=torch.int32)
+    target = torch.randint(0, 3, (rows,), generator=g, dtype=torch.int32)
+    return b, draft.to(dev), target.to(dev)
+
+
+def _commit_expect(b, draft, target):
+    """Paths by walking lists; moved rows by copying through a snapshot."""
+    paths, toks = [], []
+    dr, ta = draft.tolist(), target.tolist()
+    for q0, par in zip(b.cu_list, b.trees):
+        path = [0] if par else []
+        while path:
+            kids = [c for c in range(len(par)) if par[c] == path[-1] and dr[q0 + c] == ta[q0 + path[-1]]]
+            if not kids:
+                break
+            path.append(min(kids))
+        paths.append(path)
+        toks.append([ta[q0 + i] for i in path])
+    return paths, toks
+
+
+def _commit_moved(b, paths, t):
+    want = t.clone()
+    bs = b.pool.block_size
+    for i, (n, c, path) in enumerate(zip(b.nodes, b.ctx, paths)):
+        for j, node in enumerate(path):
+            s, d = c + node, c + j
+            want[b.tables[i, d // bs].item(), :, :, :, d % bs] = t[b.tables[i, s // bs].item(), :, :, :, s % bs]
+    return want
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("int8,mode", [(False, "token"), (True, "token"), (True, "channel")])
+@pytest.mark.parametrize("nodes,ctx", [([1], [0]), ([12, 0, 7, 31], [3, 9, 16, 44]), ([64], [15]), ([2, 2, 200], [0, 31, 5])])
+def test_tree_commit(dev, int8, mode, nodes, ctx):
+    for seed in range(3):
+        b, draft, target = _commit_case(dev, seed, nodes, ctx, int8, mode)
+        paths, toks = _commit_expect(b, draft, target)
+        tensors = [t for t in (b.pool.data, b.pool.scales, b.pool.side) if t is not None]
+        want = [_commit_moved(b, paths, t) for t in tensors]
+        acc, path, tokens = ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, draft, target,
+                                            b.max_nodes, kv_scales=b.pool.scales, kv_side=b.pool.side)
+        assert acc.tolist() == [len(p) for p in paths]
+        for i, (p, t) in enumerate(zip(paths, toks)):
+            pad = [-1] * (b.max_nodes - len(p))
+            assert path[i].tolist() == p + pad and tokens[i].tolist() == t + pad
+        for t, w in zip(tensors, want):
+            assert torch.equal(t, w)
+
+
+# ------------------------------------------------------------------ few-token MoE
+def _moe_weights(dev, E, H, I, fp8, seed):
+    g = torch.Generator().manual_seed(seed)
+    router = torch.zeros(-(-E // 128) * 128, H)
+    router[:E] = torch.randn(E, H, generator=g) * 2 / math.sqrt(H)
+    w13, w2 = (torch.randn(E, n, k, generator=g) * 0.05 for n, k in ((2 * I, H), (H, I)))
+    if fp8:
+        (w13, s13), (w2, s2) = quantize_block_fp8(w13.to(dev)), quantize_block_fp8(w2.to(dev))
+        return router.to(dev, torch.bfloat16), w13, s13, w2, s2
+    return router.to(dev, torch.bfloat16), w13.to(dev, torch.bfloat16), None, w2.to(dev, torch.bfloat16), None
+
+
+def _moe_check(x, router, w13, s13, w2, s2, E, k, renorm, out, ids, wts):
+    """Routing exactly, then the outputs for that routing within the bound of its roundings."""
+    T, H = x.shape
+    I = w2.shape[2]
+    xd = x.double()
+    logits = (xd @ router[:E].double().t())
+    m, e = torch.frexp(logits)
+    logits = torch.ldexp(torch.round(m * 256), e - 8)     # bf16, rounded once
+    want = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(ids.long(), want)
+    p = torch.softmax(logits, dim=1).gather(1, want)
+    if renorm:
+        p = p / p.sum(dim=1, keepdim=True)
+    assert bool(((wts.double() - p).abs() <= (HALF + 2 ** -18) * p).all())
+    deq = (lambda w, s, g: w[g].double()) if s13 is None else \
+        (lambda w, s, g: w[g].double() * s[g].double().repeat_interleave(128, 0).repeat_interleave(128, 1))
+    y, lim = torch.zeros_like(xd), torch.zeros_like(xd)
+    u32 = 2.0 ** -24
+    for g in torch.unique(want).tolist():
+        t, j = (want == g).nonzero(as_tuple=True)
+        a13, a2 = deq(w13, s13, g), deq(w2, s2, g)
+        z, az = xd[t] @ a13.t(), xd[t].abs() @ a13.abs().t()
+        gt, up, ag, au = z[:, :I], z[:, I:], az[:, :I], az[:, I:]
+        s = gt * torch.sigmoid(gt)
+        h = s * up
+        # fp32 sums of H terms (H u32 of their absolute sum; the scale adds two roundings), |silu'| < 1.1;
+        # silu and the product: a few roundings; the hidden value may be rounded to bf16
+        dh = (H + 4) * u32 * (1.1 * ag * up.abs() + s.abs() * au) + (HALF + 2 ** -20) * h.abs()
+        w = wts.double()[t, j, None]
+        y.index_add_(0, t, w * (h @ a2.t()))
+        lim.index_add_(0, t, w * (dh @ a2.abs().t() + (I + 8) * u32 * (h.abs() @ a2.abs().t())))
+    lim += HALF * y.abs()
+    err = (out.double() - y).abs()
+    assert bool((err <= lim).all()), float((err / lim).max())
+
+
+MOE = [  # T, H, I, E, topk, fp8, tiled, renorm
+    (1, 256, 128, 8, 2, True, True, True), (5, 256, 128, 8, 2, False, False, True),
+    (3, 128, 128, 1, 1, True, False, False), (64, 256, 256, 8, 8, True, True, True),
+    (17, 1280, 640, 24, 6, True, True, False), (33, 384, 128, 40, 4, True, False, True),
+    (64, 512, 128, 4, 1, False, False, True), (9, 2048, 768, 128, 8, True, True, True),
+    (2, 640, 1152, 200, 3, False, False, True),
+]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,H,I,E,k,fp8,tiled,renorm", MOE)
+def test_moe_few_tokens(dev, T, H, I, E, k, fp8, tiled, renorm):
+    router, w13, s13, w2, s2 = _moe_weights(dev, E, H, I, fp8, seed=T + E)
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(dev, torch.bfloat16)
+    ids = torch.empty(T, k, dtype=torch.int32, device=dev)
+    wts = torch.empty(T, k, dtype=torch.float32, device=dev)
+    a13, a2 = (ops.tile_fp8(w13), ops.tile_fp8(w2)) if tiled else (w13, w2)
+    out = ops.moe_few_tokens(x, router, a13, s13, a2, s2, E, k, renorm, ids=ids, weights=wts, tiled=tiled)
+    _moe_check(x, router, w13, s13, w2, s2, E, k, renorm, out, ids, wts)
+    if dev == "cuda":
+        ops.check_status(out.device)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_moe_few_tokens_all_to_one_expert(dev):
+    """Every token picks the same experts, and experts that tie: the lowest id wins."""
+    E, H, I, k, T = 8, 256, 128, 2, 50
+    router, w13, s13, w2, s2 = _moe_weights(dev, E, H, I, True, seed=3)
+    router[:E] = router[0]                       # all experts tie
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(9)).to(dev, torch.bfloat16)
+    ids = torch.empty(T, k, dtype=torch.int32, device=dev)
+    wts = torch.empty(T, k, dtype=torch.float32, device=dev)
+    out = ops.moe_few_tokens(x, router, w13, s13, w2, s2, E, k, ids=ids, weights=wts)
+    assert bool((ids == torch.tensor([0, 1], dtype=torch.int32, device=dev)).all())
+    _moe_check(x, router, w13, s13, w2, s2, E, k, True, out, ids, wts)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_moe_few_tokens_one_bad_token(dev):
+    """A token with a NaN gives a NaN row; the other rows do not change."""
+    E, H, I, k = 8, 256, 128, 2
+    router, w13, s13, w2, s2 = _moe_weights(dev, E, H, I, True, seed=4)
+    x = torch.randn(6, H, generator=torch.Generator().manual_seed(2)).to(dev, torch.bfloat16)
+    want = ops.moe_few_tokens(x, router, w13, s13, w2, s2, E, k)
+    x[2, 5] = math.nan
+    got = ops.moe_few_tokens(x, router, w13, s13, w2, s2, E, k)
+    keep = [0, 1, 3, 4, 5]
+    assert bool(torch.isnan(got[2].float()).all())
+    # (the CPU path multiplies an expert's rows together: another row may change its last bits)
+    assert torch.equal(got[keep], want[keep]) if dev == "cuda" else bool(torch.isfinite(got[keep].float()).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_moe_few_refusals(dev):
+    E, H, I, k = 8, 256, 128, 2
+    router, w13, s13, w2, s2 = _moe_weights(dev, E, H, I, True, seed=4)
+    x = torch.zeros(ops.MOE_FEW_MAX_TOKENS + 1, H, dtype=torch.bfloat16, device=dev)
+    ok = (router, w13, s13, w2, s2, E, k)
+    for xx, args in [(x, ok), (x[:4, ::2], ok), (x[:4], (router, w13, None, w2, None, E, k)),
+                     (x[:4], (router, w13, s13, w2, s2, E, 9)), (x[:4], (router, w13[:4], s13, w2, s2, E, k)),
+                     (x[:4], (router, w13, s13, w2.transpose(1, 2), s2, E, k))]:
+        with pytest.raises(ValueError):
+            ops.moe_few_tokens(xx, *args)
+    with pytest.raises(ValueError):
+        ops.moe_few_tokens(x[:4], *ok, out=x[:3])
+    assert ops.moe_few_tokens(x[:0], *ok).shape == (0, H)
