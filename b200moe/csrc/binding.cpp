@@ -6,6 +6,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cmath>
 #include <cstring>
 #include <tuple>
 #include <vector>
@@ -793,6 +794,7 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   check_tree(cu, lens, tables, parents, q.device(), max_q_len);
   check_aligned(q, "q"); check_aligned(out, "out"); check_aligned(k_cache, "k"); check_aligned(v_cache, "v");
   TORCH_CHECK(block_stride * k_cache.element_size() % 16 == 0, "cache blocks must be multiples of 16 bytes");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   TORCH_CHECK(parents.numel() == q.size(0), "parents must hold one entry per row of q");
   b200::TreeAttnArgs a{};
   a.q = q.data_ptr();
@@ -816,6 +818,7 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   a.parents = parents.data_ptr<int>();
   a.batch = (int)lens.numel();
   a.rows = (int)q.size(0);
+  a.max_q_len = (int)max_q_len;
   a.max_blocks = (int)tables.size(1);
   a.num_blocks = (int)k_cache.size(0);
   a.block_size = (int)block_size;
@@ -828,7 +831,14 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   a.out = out.data_ptr();
   a.status = status.data_ptr<int>();
   c10::cuda::CUDAGuard guard(q.device());
-  b200::tree_attn(a, stream());
+  b200::TreeAttnTcPlan plan{};
+  if (b200::tree_attn_tc_plan(a, (int)max_q_len, &plan)) {
+    Tensor ws = torch::empty({plan.workspace_bytes}, q.options().dtype(torch::kUInt8));
+    plan.workspace = ws.data_ptr();
+    b200::tree_attn_tc(a, plan, stream());
+  } else {
+    b200::tree_attn(a, stream());
+  }
 }
 
 // Accepted paths of a batch of trees; the rows of kv_data (and scales / side) move in place.

@@ -25,6 +25,7 @@ struct TreeAttnArgs {
   const int* parents;        // [rows] place of a node's parent in its tree, -1: none
   int batch;
   int rows;
+  int max_q_len;             // no tree has more nodes (<= kTreeMaxNodes)
   int max_blocks;
   int num_blocks;
   int block_size;
@@ -38,6 +39,20 @@ struct TreeAttnArgs {
   int* status;               // device status word
 };
 void tree_attn(const TreeAttnArgs& a, cudaStream_t s);
+
+// Tensor-core form (kernels/tree_attn_tc.cu): bf16 pool, head_dim 64 or 128, blocks that
+// hold whole tiles of 128 keys or divide one in multiples of 8 rows.
+constexpr int kTreeTcBatch = 1024;   // sequences of one launch
+struct TreeAttnTcPlan {
+  int sub_rows;              // key rows of one TMA box
+  int part_rows;             // rows of one partial result
+  int grid;
+  int64_t workspace_bytes;
+  void* workspace;           // 16-byte aligned
+};
+// False where the shape is not the tensor-core kernel's.
+bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p);
+void tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s);
 
 // One kind of rows the commit moves: [blocks, planes, block_size, row_bytes], contiguous.
 struct TreeRows {

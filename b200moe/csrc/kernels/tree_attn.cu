@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
   const int b = lo, q0 = a.cu_seqlens_q[b], n = a.cu_seqlens_q[b + 1] - q0, node = row - q0;
   if (node < 0 || node >= n) return;  // rows behind the last sequence
   const int len = a.seq_lens[b], prefix = len - n;
-  if (n > kTreeMaxNodes || prefix < 0 || q0 < 0 || q0 + n > a.rows) {
+  if (n > a.max_q_len || prefix < 0 || q0 < 0 || q0 + n > a.rows || len > (int64_t)a.max_blocks * a.block_size) {
     if (threadIdx.x == 0) record_status(a.status, kStatusBadShape);
     return;
   }
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
       int64_t blk = 0;
       const int bi = key / a.block_size, y = key % a.block_size;
       if (see) {
-        blk = bi < a.max_blocks ? tab[bi] : -1;
+        blk = tab[bi];
         if (blk < 0 || blk >= a.num_blocks) { bad = true; see = false; blk = 0; }
       }
       float ks = 1.f, vs = 1.f;

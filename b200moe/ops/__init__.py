@@ -693,11 +693,14 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     its tree, below the node's own; -1 for a node that follows the prefix directly.  max_q_len: no tree
     has more nodes (at most ``TREE_MAX_NODES``).  Chains (parents i - 1) give causal attention.  Rows
     behind the last sequence are left as they are.  bf16 and int8 pools, head_dim 64 or 128.  A tree
-    that does not fit (offsets outside q, more nodes than keys or than max_q_len) is left out and a
-    block id outside the pool is not read; both set the status word (``check_status``)."""
+    that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
+    table row has) is left out and a block id outside the pool is not read; both set the status word
+    (``check_status``)."""
     if q.dim() != 3 or not q.is_contiguous():
         raise ValueError("q must be contiguous [rows, q_heads, head_dim]")
     _check_tree(q.shape[0], cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, q.device)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, got {scale}")
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
