@@ -60,25 +60,26 @@ constexpr int kRows = 128, kKeys = 128;
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
-constexpr int kDirtyBufs = 4;
+constexpr int kCutTiles = 4;
+constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
 template <int D>
 struct Lay {
   static constexpr int TILE = kKeys * D * 2;       // a K, V or Q tile: D / 64 halves of [128][64]
   static constexpr int HALF = kKeys * 64 * 2;
   static constexpr int SLOTS = D == 128 ? 2 : 4;   // K tiles, and V tiles, in flight
-  static constexpr int Q = 0;                      // two row tiles
+  static constexpr int Q = 0;                      // two row tiles; the second also carries the join
   static constexpr int K = Q + 2 * TILE;
   static constexpr int V = K + SLOTS * TILE;
-  static constexpr int STAGE = V + SLOTS * TILE;   // join of the two groups: 2 x [4][128] float4
-  static constexpr int ANC = STAGE + 2 * 8192;     // [nodes][kAncWords] ancestor bits
+  static constexpr int ANC = V + SLOTS * TILE;     // [nodes][kAncWords] ancestor bits
   static constexpr int PAR = ANC + kTreeMaxNodes * kAncWords * 4;
   static constexpr int ML = PAR + kTreeMaxNodes * 4;          // [2][128] (max, sum)
   static constexpr int DIRTY = ML + 2 * kRows * 8;
-  static constexpr int BARS = DIRTY + kDirtyBufs * kAncWords * 4;
-  static constexpr int NBARS = 5 * SLOTS + 2 + 6 + 3;
-  static constexpr int PU = BARS + NBARS * 8 + 16;            // [batch + 1] units before a sequence
-  static int smem(int batch) { return PU + (batch + 1) * 4 + 1024; }
+  static constexpr int SEG = DIRTY + kRing * kAncWords * 4;   // [kRing] segments
+  static constexpr int BARS = SEG + kRing * 64;
+  static constexpr int NBARS = 5 * SLOTS + 2 + 6 + 3 + 2 * kRing;
+  static constexpr int TAB = BARS + NBARS * 8 + 32;           // per sequence: Row, then one more
+  static int smem(int batch) { return TAB + (batch + 1) * 16 + 1024; }
 };
 
 struct TcArgs {
@@ -142,6 +143,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+// two fp32 operations in one instruction, each rounded to nearest
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -155,62 +172,91 @@ struct Chunks {
   __device__ __forceinline__ int start(int i) const { return (int)((int64_t)i * nt / n); }
   __device__ __forceinline__ int of(int tile) const { return (int)(((int64_t)(tile + 1) * n - 1) / nt); }
 };
-__device__ __forceinline__ Chunks chunks_of(int nt, int pairs, int share) {
-  return {pairs == 1 || nt <= share ? 1 : nt / share, nt};
-}
 
-// What a sequence adds to the order of units.
-struct Seq {
-  int q0, n, len;      // first row, nodes, keys
-  int nt, pairs;       // key tiles, pairs of row tiles
+// Per sequence, in shared memory.
+struct Row {
+  int q0, len;         // first row, keys
+  int unit, item;      // units and items in front of it
 };
-__device__ __forceinline__ Seq seq_of(const TreeAttnArgs& a, int b) {
-  Seq s;
-  s.q0 = a.cu_seqlens_q[b];
-  s.n = a.cu_seqlens_q[b + 1] - s.q0;
-  s.len = a.seq_lens[b];
-  s.nt = (s.len + kKeys - 1) / kKeys;
-  const int per = kRows / a.group;  // nodes per row tile
-  s.pairs = ((s.n + per - 1) / per + 1) / 2;
-  return s;
-}
+
+// The grid's work: equal shares of the units, or whole items where that costs hardly more.
+struct Plan {
+  const Row* rows;     // [batch + 1]
+  int batch, kvh, per; // sequences, KV heads, nodes per row tile
+  int W, items;        // units and items in all
+  int grid, share;     // CTAs with work, units of the largest share
+  int whole;           // shares end at items: nothing is cut
+  int base, rem;       // quotient and remainder of W (items) by the CTAs
+
+  __device__ __forceinline__ int nodes(int b) const { return rows[b + 1].q0 - rows[b].q0; }
+  __device__ __forceinline__ int tiles(int b) const { return (rows[b].len + kKeys - 1) / kKeys; }
+  __device__ __forceinline__ int pairs(int b) const { return ((nodes(b) + per - 1) / per + 1) >> 1; }
+  __device__ __forceinline__ Chunks chunks(int nt, int pr) const {
+    return {whole || pr == 1 || nt <= share ? 1 : nt / share, nt};
+  }
+  // last sequence with at most x units (items) in front of it
+  __device__ __forceinline__ int at(int x, bool by_item) const {
+    int lo = 0, up = batch;
+    while (up - lo > 1) {
+      const int mid = (lo + up) >> 1;
+      if ((by_item ? rows[mid].item : rows[mid].unit) <= x) lo = mid; else up = mid;
+    }
+    return lo;
+  }
+  // first unit of CTA c
+  __device__ __forceinline__ int lo(int c) const {
+    if (c >= grid) return W;
+    const int x = c * base + min(c, rem);
+    if (!whole || x >= items) return whole ? W : x;
+    const int b = at(x, true);
+    return rows[b].unit + (x - rows[b].item) * tiles(b);
+  }
+  // the CTA whose share holds unit u (shares of units)
+  __device__ __forceinline__ int cta(int u) const {
+    const int edge = rem * (base + 1);
+    return u < edge ? u / (base + 1) : rem + (u - edge) / base;
+  }
+};
 
 // A run of key tiles [t0, t1) of one item (sequence, KV head, row pair) inside a CTA's share.
 struct Seg {
-  Seq s;
-  int b, h, pair, t0, t1;
+  int b, h, pair, q0, n, len;
+  int t0, t1;          // t1 = 0: no more segments
   int two;             // two row tiles
   int whole;           // covers all of the item's keys
-  int next;            // first unit behind it
+  int slot;            // partial result of the CTA
+  int pad[5];
 };
-__device__ __forceinline__ Seg seg_at(const TreeAttnArgs& a, const int* pu, int share, int u, int hi) {
+static_assert(sizeof(Seg) == 64, "segment ring");
+
+__device__ __forceinline__ Seg seg_at(const Plan& p, int u, int lo, int hi) {
   Seg g;
-  int lo = 0, up = a.batch;
-  while (up - lo > 1) {
-    const int mid = (lo + up) >> 1;
-    if (pu[mid] <= u) lo = mid; else up = mid;
-  }
-  g.b = lo;
-  g.s = seq_of(a, lo);
-  int r = u - pu[lo];
-  const int per_head = g.s.nt * g.s.pairs;
+  g.b = p.at(u, false);
+  const Row row = p.rows[g.b];
+  g.q0 = row.q0;
+  g.len = row.len;
+  g.n = p.nodes(g.b);
+  const int nt = p.tiles(g.b), pr = p.pairs(g.b);
+  int r = u - row.unit;
+  const int per_head = nt * pr;
   g.h = r / per_head;
   r -= g.h * per_head;
-  const Chunks c = chunks_of(g.s.nt, g.s.pairs, share);
-  const int ci = c.of(r / g.s.pairs), start = c.start(ci), end = c.start(ci + 1), clen = end - start;
-  r -= start * g.s.pairs;
-  g.pair = r / clen;
-  g.t0 = start + r % clen;
+  const Chunks c = p.chunks(nt, pr);
+  int start = 0, end = nt;
+  if (c.n > 1) {
+    const int ci = c.of(r / pr);
+    start = c.start(ci);
+    end = c.start(ci + 1);
+  }
+  r -= start * pr;
+  g.pair = pr == 1 ? 0 : r / (end - start);
+  g.t0 = start + r - g.pair * (end - start);
   g.t1 = min(end, g.t0 + (hi - u));
-  g.next = u + (g.t1 - g.t0);
-  g.whole = g.t0 == 0 && g.t1 == g.s.nt;
-  const int per = kRows / a.group;
-  g.two = g.s.n > (2 * g.pair + 1) * per;
+  g.whole = g.t0 == 0 && g.t1 == nt;
+  g.two = g.n > (2 * g.pair + 1) * p.per;
+  g.slot = u == lo ? 0 : 1;
   return g;
 }
-
-// CTA c's share of W units.
-__device__ __forceinline__ int share_lo(int c, int W, int grid) { return (int)((int64_t)c * W / grid); }
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -232,11 +278,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   uint64_t* p_full = s_full + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* fin = pv_done + 2;            // [2] an issuer's last products
-  uint64_t* both = fin + 2;               // the eight softmax warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(both + 1);
+  uint64_t* both = fin + 2;               // the eight softmax warps meet
+  uint64_t* joined = both + 1;            // [kRing] the softmax warps are done with the segment's join
+  uint64_t* seg_full = joined + kRing;    // [kRing]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_full + kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_max_nt = reinterpret_cast<int*>(tmem_slot + 2);
-  int* pu = reinterpret_cast<int*>(smem + L::PU);
+  Row* rows = reinterpret_cast<Row*>(smem + L::TAB);
+  volatile Seg* segs = reinterpret_cast<volatile Seg*>(smem + L::SEG);
   uint32_t* anc = reinterpret_cast<uint32_t*>(smem + L::ANC);
   int* s_par = reinterpret_cast<int*>(smem + L::PAR);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::ML);
@@ -246,17 +295,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   const int G = a.group, per = kRows / G;   // nodes per row tile
   int* status = a.status;
 
-  // ---- units before each sequence; a tree that does not fit counts none
+  // ---- the work of every sequence; a tree that does not fit has none
   if (threadIdx.x == 0) *s_max_nt = 0;
   __syncthreads();
   for (int b = threadIdx.x; b < a.batch; b += kThreads) {
-    const Seq s = seq_of(a, b);
-    const bool bad = s.n < 0 || s.n > a.max_q_len || s.q0 < 0 || s.q0 + s.n > a.rows ||
-                     (s.n > 0 && (s.len < s.n || s.len > (int64_t)a.max_blocks * a.block_size));
+    const int q0 = a.cu_seqlens_q[b], n = a.cu_seqlens_q[b + 1] - q0, len = a.seq_lens[b];
+    const bool bad = n < 0 || n > a.max_q_len || q0 < 0 || q0 + n > a.rows ||
+                     (n > 0 && (len < n || len > (int64_t)a.max_blocks * a.block_size));
     if (bad && blockIdx.x == 0) record_status(status, kStatusBadShape);
-    const bool none = bad || s.n == 0;
-    pu[b + 1] = none ? 0 : s.nt * s.pairs * a.num_kv_heads;
-    if (!none) atomicMax(s_max_nt, s.nt);
+    Row r{q0, len, 0, 0};
+    if (!bad && n > 0) {
+      const int nt = (len + kKeys - 1) / kKeys;
+      r.item = ((n + per - 1) / per + 1) / 2 * a.num_kv_heads;
+      r.unit = r.item * nt;
+      atomicMax(s_max_nt, nt);
+    }
+    rows[b] = r;
+    if (b == a.batch - 1) rows[b + 1].q0 = q0 + n;
   }
   if (threadIdx.x == 32) {
     for (int i = 0; i < kSlots; ++i) {
@@ -275,23 +330,35 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       mbar_init(&fin[i], 1);
     }
     mbar_init(both, 8);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&joined[i], 8);
+      mbar_init(&seg_full[i], 1);
+    }
     fence_barrier_init();
     *abort_flag = 0;
   }
   __syncthreads();
   if (warp == 0) {
-    int at = 0;
-    if (lane == 0) pu[0] = 0;
+    int units = 0, items = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
       const int b = b0 + lane;
-      int v = b < a.batch ? pu[b + 1] : 0;
+      const int mu = b < a.batch ? rows[b].unit : 0, mi = b < a.batch ? rows[b].item : 0;
+      int u = mu, i = mi;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += up;
+        const int pu = __shfl_up_sync(0xffffffffu, u, o), pi = __shfl_up_sync(0xffffffffu, i, o);
+        if (lane >= o) { u += pu; i += pi; }
       }
-      if (b < a.batch) pu[b + 1] = at + v;
-      at += __shfl_sync(0xffffffffu, v, 31);
+      if (b < a.batch) {
+        rows[b].unit = units + u - mu;
+        rows[b].item = items + i - mi;
+      }
+      units += __shfl_sync(0xffffffffu, u, 31);
+      items += __shfl_sync(0xffffffffu, i, 31);
+    }
+    if (lane == 0) {
+      rows[a.batch].unit = units;
+      rows[a.batch].item = items;
     }
   }
   if (warp == 1) {
@@ -302,10 +369,30 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;   // S0 | S1 | O0 | O1, 128 columns each
-  const int W = pu[a.batch];
-  const int grid = gridDim.x;
-  const int share = (W + grid - 1) / grid;
-  const int u_lo = share_lo(blockIdx.x, W, grid), u_hi = share_lo(blockIdx.x + 1, W, grid);
+  Plan plan{rows, a.batch, a.num_kv_heads, per, rows[a.batch].unit, rows[a.batch].item};
+  const int max_nt = *s_max_nt;
+  plan.share = (plan.W + (int)gridDim.x - 1) / (int)gridDim.x;
+  // Cutting items costs their partial results, a grid barrier and the join, worth about kCutTiles
+  // key tiles; whole items cost the rounding up of their number.
+  plan.whole = (plan.items + (int)gridDim.x - 1) / (int)gridDim.x * max_nt <= plan.share + kCutTiles;
+  const int spread = plan.whole ? plan.items : plan.W;
+  plan.grid = min((int)gridDim.x, spread);
+  plan.base = plan.grid ? spread / plan.grid : 0;
+  plan.rem = plan.grid ? spread % plan.grid : 0;
+  const int u_lo = plan.lo(blockIdx.x), u_hi = plan.lo(blockIdx.x + 1);
+  // No role is kRing segments ahead of another, so a ring of barriers tells segments apart.
+  auto join_over = [&](int sg) {
+    return mbar_wait(&joined[sg % kRing], (sg / kRing) & 1, status, kStatusTimeoutEmpty, abort_flag);
+  };
+  // segment sg of this CTA, written by the producer; none behind the last
+  auto segment = [&](int sg, Seg& g) {
+    if (!mbar_wait(&seg_full[sg % kRing], (sg / kRing) & 1, status, kStatusTimeoutFull, abort_flag)) return false;
+    const volatile int* src = reinterpret_cast<const volatile int*>(&segs[sg % kRing]);
+    int* dst = reinterpret_cast<int*>(&g);
+#pragma unroll
+    for (int i = 0; i < 11; ++i) dst[i] = src[i];
+    return g.t1 > 0;
+  };
 
   if (warp == 0) {
     // ================================================================ TMA producer
@@ -316,17 +403,27 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const int nsub = kKeys / t.sub_rows;
       int gt = 0, sg = 0;   // tiles, segments
       bool ok = true, bad = false;
-      for (int u = u_lo; u < u_hi && ok; ++sg) {
-        const Seg g = seg_at(a, pu, share, u, u_hi);
-        u = g.next;
+      for (int u = u_lo; ok; ++sg) {
+        Seg g{};
+        if (u < u_hi) g = seg_at(plan, u, u_lo, u_hi);
+        u += g.t1 - g.t0;
+        {
+          volatile int* dst = reinterpret_cast<volatile int*>(&segs[sg % kRing]);
+          const int* src = reinterpret_cast<const int*>(&g);
+#pragma unroll
+          for (int i = 0; i < 11; ++i) dst[i] = src[i];
+          mbar_arrive(&seg_full[sg % kRing]);
+        }
+        if (g.t1 == 0) break;
         if (!mbar_wait(q_empty, (sg & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag)) break;
         const int tiles = g.two ? 2 : 1;
+        if (g.two && sg > 0 && !join_over(sg - 1)) break;   // its second Q tile may still carry a join
         mbar_arrive_expect_tx(q_full, tiles * kHalves * per * G * 128);
         for (int i = 0; i < tiles; ++i)
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf)
             tma_3d(smem_u32(smem + L::Q + i * L::TILE + hf * L::HALF), &q_map, q_full, hf * 64, g.h * G,
-                   g.s.q0 + (2 * g.pair + i) * per);
+                   g.q0 + (2 * g.pair + i) * per);
         const int* tab = a.block_tables + (int64_t)g.b * a.max_blocks;
         for (int j = g.t0; j < g.t1 && ok; ++j, ++gt) {
           const int slot = gt % kSlots;
@@ -343,7 +440,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             for (int sub = 0; sub < nsub; ++sub) {
               const int key = j * kKeys + sub * t.sub_rows;
               int blk = a.num_blocks;      // out of range: zero fill
-              if (key < g.s.len) {
+              if (key < g.len) {
                 const int bi = key / a.block_size;
                 const int id = bi < a.max_blocks ? tab[bi] : -1;
                 if (id >= 0 && id < a.num_blocks) blk = id;
@@ -374,9 +471,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
       int gt = 0, sg = 0, mine = 0;   // tiles of the CTA, segments, tiles of this group
       bool ok = true;
-      for (int u = u_lo; u < u_hi && ok; ++sg) {
-        const Seg g = seg_at(a, pu, share, u, u_hi);
-        u = g.next;
+      Seg g;
+      for (; ok && segment(sg, g); ++sg) {
         if (!mbar_wait(q_full, sg & 1, status, kStatusTimeoutFull, abort_flag)) { ok = false; break; }
         const uint32_t qa = smem_u32(smem + L::Q + (g.two ? w : 0) * L::TILE);
         bool first = true;
@@ -423,13 +519,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // ================================================================ V cleaner
     int gt = 0, sg = 0;
     bool ok = true;
-    for (int u = u_lo; u < u_hi && ok; ++sg) {
-      const Seg g = seg_at(a, pu, share, u, u_hi);
-      u = g.next;
-      uint32_t* dirt = dirty + (sg % kDirtyBufs) * kAncWords;
+    Seg g;
+    for (; ok && __all_sync(0xffffffffu, segment(sg, g)); ++sg) {
+      uint32_t* dirt = dirty + (sg % kRing) * kAncWords;
       if (lane < kAncWords) dirt[lane] = 0;
       __syncwarp();
-      const int prefix = g.s.len - g.s.n;
+      const int prefix = g.len - g.n;
       for (int j = g.t0; j < g.t1; ++j, ++gt) {
         const int slot = gt % kSlots;
         ok = mbar_wait(&v_full[slot], (gt / kSlots) & 1, status, kStatusTimeoutFull, abort_flag);
@@ -439,7 +534,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           for (int r = lane; r < kKeys; r += 32) {
             const int node = j * kKeys + r - prefix;
             if (node < 0) continue;
-            const bool behind = node >= g.s.n;
+            const bool behind = node >= g.n;
             bool bad = false;
 #pragma unroll 1
             for (int c = 0; c < D / 8; ++c) {
@@ -485,31 +580,46 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const bool here = mbar_wait(both, syncs++ & 1, status, kStatusTimeoutFlag, abort_flag);
       return __all_sync(0xffffffffu, here) != 0;
     };
-    for (int u = u_lo; u < u_hi && ok; ++sg) {
-      const Seg g = seg_at(a, pu, share, u, u_hi);
-      const int slot_id = u == u_lo ? 0 : 1;
-      u = g.next;
-      const int prefix = g.s.len - g.s.n;
-      if (g.b != seen_b) {
+    Seg g;
+    while (ok && __all_sync(0xffffffffu, segment(sg, g))) {
+      const int prefix = g.len - g.n;
+      if (g.t1 * kKeys > prefix && g.b != seen_b) {
         // ancestor bits of the sequence's nodes, by walking the parents in shared memory
         if (!meet()) break;
-        for (int i = tid; i < g.s.n; i += 256) s_par[i] = a.parents[g.s.q0 + i];
-        for (int i = tid; i < g.s.n * kAncWords; i += 256) anc[i] = 0;
+        if (tid < g.n) s_par[tid] = a.parents[g.q0 + tid];
         if (!meet()) break;
-        for (int i = tid; i < g.s.n; i += 256) {
-          for (int at = i; at >= 0;) {          // a parent that is not in front of its child ends the walk
-            anc[i * kAncWords + (at >> 5)] |= 1u << (at & 31);
+        if (tid < g.n) {
+          uint32_t bits[kAncWords] = {};
+          for (int at = tid; at >= 0;) {        // a parent that is not in front of its child ends the walk
+#pragma unroll
+            for (int i = 0; i < kAncWords; ++i) bits[i] |= (at >> 5) == i ? 1u << (at & 31) : 0u;
             const int up = s_par[at];
             at = up < at ? up : -1;
           }
+          uint4* dst = reinterpret_cast<uint4*>(anc + tid * kAncWords);
+          dst[0] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+          dst[1] = make_uint4(bits[4], bits[5], bits[6], bits[7]);
         }
         if (!meet()) break;
         seen_b = g.b;
       }
       const int tile = 2 * g.pair + (g.two ? w : 0);
       const int node = tile * per + r / G, head = g.h * G + r % G;
-      const bool valid = r < per * G && node < g.s.n;
+      const bool valid = r < per * G && node < g.n;
       const bool any = __any_sync(0xffffffffu, valid);
+      // columns [c, c + 32) of key tile j that this row sees
+      auto sees = [&](int kb, int c) -> uint32_t {
+        const int t0 = kb + c - prefix;                 // node of the first column
+        uint32_t see = t0 >= 0 ? 0u : t0 <= -32 ? 0xffffffffu : (1u << -t0) - 1u;
+        if (t0 > -32 && valid) {
+          const int i = t0 >> 5;
+          const uint32_t* row = anc + node * kAncWords;
+          const uint32_t lo = i >= 0 && i < kAncWords ? row[i] : 0u;
+          const uint32_t up = i + 1 < kAncWords ? row[i + 1] : 0u;
+          see |= __funnelshift_r(lo, up, t0 & 31);
+        }
+        return see;
+      };
       float m = -INFINITY, l = 0.f;
       int done = 0;                              // tiles of this group in the segment
       for (int j = g.t0; j < g.t1; ++j, ++gt) {
@@ -518,31 +628,34 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (any) {
-          float s[kKeys];
-#pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) tmem_ld<32>(tS + c * 32, s + c * 32);
-          tmem_ld_wait();
           const int kb = j * kKeys;
-          if (kb + kKeys > prefix) {
+          const bool tail = kb + kKeys > prefix;
+          // The row goes through registers twice, 64 columns at a time: a loop of two keeps the
+          // code small (a cold instruction cache costs more than the second read of TMEM).
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < kKeys; c += 64) {
+            float s[64];
+            tmem_ld<32>(tS + c, s);
+            tmem_ld<32>(tS + c + 32, s + 32);
+            tmem_ld_wait();
+            if (tail) {
+              const uint32_t lo = sees(kb, c), hi = sees(kb, c + 32);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int t0 = kb + q * 32 - prefix;        // node of the word's first column
-              uint32_t see = t0 >= 0 ? 0u : t0 <= -32 ? 0xffffffffu : (1u << -t0) - 1u;
-              if (t0 > -32 && valid) {
-                const int i = t0 >> 5;
-                const uint32_t* row = anc + node * kAncWords;
-                const uint32_t lo = i >= 0 && i < kAncWords ? row[i] : 0u;
-                const uint32_t up = i + 1 < kAncWords ? row[i + 1] : 0u;
-                see |= __funnelshift_r(lo, up, t0 & 31);
+              for (int i = 0; i < 32; ++i) {
+                if (!((lo >> i) & 1u)) s[i] = -INFINITY;
+                if (!((hi >> i) & 1u)) s[32 + i] = -INFINITY;
               }
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!((see >> c) & 1u)) s[q * 32 + c] = -INFINITY;
             }
-          }
-          float mx = fmaxf(s[0], s[1]);
+            float x[8];
 #pragma unroll
-          for (int c = 2; c < kKeys; ++c) mx = fmaxf(mx, s[c]);
+            for (int i = 0; i < 8; ++i) x[i] = fmaxf(s[i], s[8 + i]);
+#pragma unroll
+            for (int q = 2; q < 8; ++q)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], s[8 * q + i]);
+            mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+          }
           mx *= sl2;
           const bool grow = mx > m + kLazyLog2;
           if (__any_sync(0xffffffffu, grow)) {
@@ -565,20 +678,39 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
               }
             }
           }
-          const float mu = m == -INFINITY ? 0.f : m;
-          float sum0 = 0.f, sum1 = 0.f;
+          const float2 k2 = make_float2(sl2, sl2);
+          const float mu = m == -INFINITY ? 0.f : -m;
+          const float2 mu2 = make_float2(mu, mu);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll 1
+          for (int c = 0; c < kKeys; c += 64) {
+            float s[64];
+            tmem_ld<32>(tS + c, s);
+            tmem_ld<32>(tS + c + 32, s + 32);
+            tmem_ld_wait();
+            if (tail) {
+              const uint32_t lo = sees(kb, c), hi = sees(kb, c + 32);
 #pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) {
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              p[i] = pack2(ex2(fmaf(s[c * 32 + 2 * i], sl2, -mu)), ex2(fmaf(s[c * 32 + 2 * i + 1], sl2, -mu)));
-              sum0 += __uint_as_float(p[i] << 16);
-              sum1 += __uint_as_float(p[i] & 0xffff0000u);
+              for (int i = 0; i < 32; ++i) {
+                if (!((lo >> i) & 1u)) s[i] = -INFINITY;
+                if (!((hi >> i) & 1u)) s[32 + i] = -INFINITY;
+              }
             }
-            tmem_st16(tS + c * 16, p);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t p[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 z = fma2(make_float2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), k2, mu2);
+                p[i] = pack2(ex2(z.x), ex2(z.y));
+                const float2 back = make_float2(__uint_as_float(p[i] << 16), __uint_as_float(p[i] & 0xffff0000u));
+                if (i & 1) sum1 = add2(sum1, back); else sum0 = add2(sum0, back);
+              }
+              // P overlays S: columns [c / 2, c / 2 + 32) have been read by this thread
+              tmem_st16(tS + c / 2 + q * 16, p);
+            }
           }
-          l += sum0 + sum1;
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_st_wait();
           tc_fence_before();
         }
@@ -595,86 +727,104 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
       }
-      float fac = 1.f;
-      if (join) {
-        s_ml[w * kRows + r] = make_float2(m, l);
-        if (!meet()) break;
-        const float2 other = s_ml[(w ^ 1) * kRows + r];
-        const float top = fmaxf(m, other.x);
-        fac = m == -INFINITY ? 0.f : ex2(m - top);
-        const float ofac = other.x == -INFINITY ? 0.f : ex2(other.x - top);
-        l = l * fac + other.y * ofac;
-        m = top;
-      }
-      // columns this thread writes: all of its row, or its half of a joined row
-      const int c0 = join ? w * (D / 32) : 0, c1 = join ? (w + 1) * (D / 32) : done > 0 ? D / 16 : 0;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int prow = (g.two ? w : 0) * kRows + r;
-      const int64_t pslot = (int64_t)(blockIdx.x * 2 + slot_id) * t.part_rows + prow;
-      if (!g.whole && valid && c1 > 0 && (!join || w == 0)) t.part_ml[pslot] = make_float2(m, l);
-      const uint32_t* dirt = dirty + (sg % kDirtyBufs) * kAncWords;
-      bool dirt_any = false;
+      // Where both groups hold a part, each hands the other half of its columns, D / 4 at a time,
+      // through the second Q tile (not in use by a segment with one row tile).
+      constexpr int kHand = D / 4;
+      float4* stage = reinterpret_cast<float4*>(smem + L::Q + L::TILE);   // [2][kHand / 4][128]
+      auto hand = [&](int round) {
 #pragma unroll
-      for (int i = 0; i < kAncWords; ++i) dirt_any |= dirt[i] != 0;
-      float4* stage = reinterpret_cast<float4*>(smem + L::STAGE);
-#pragma unroll 1
-      for (int i = 0; i < D / 16; ++i) {
-        if (join && i >= D / 32) break;
-        float o[16];
-        if (join) {
-          // hand the other group its columns of this row, take this group's columns of the other part
-          tmem_ld16(tO + ((w ^ 1) * (D / 32) + i) * 16, o);
+        for (int c = 0; c < kHand; c += 16) {
+          float o[16];
+          tmem_ld16(tO + ((w ^ 1) * 2 + round) * kHand + c, o);
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            stage[w * 512 + e * 128 + r] = make_float4(o[4 * e] * fac, o[4 * e + 1] * fac, o[4 * e + 2] * fac, o[4 * e + 3] * fac);
+            stage[(w * (kHand / 4) + c / 4 + e) * kRows + r] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      };
+      float fac = 1.f, ofac = 0.f;
+      if (join) {
+        if (sg > 0) {
+          ok = join_over(sg - 1);   // the other group has read what the last join handed over
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        }
+        s_ml[w * kRows + r] = make_float2(m, l);
+        hand(0);
+        if (!(ok = meet())) break;
+        const float2 other = s_ml[(w ^ 1) * kRows + r];
+        const float top = fmaxf(m, other.x);
+        fac = m == -INFINITY ? 0.f : ex2(m - top);
+        ofac = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+        l = l * fac + other.y * ofac;
+        m = top;
+      }
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const int64_t pslot = (int64_t)(blockIdx.x * 2 + g.slot) * t.part_rows + (g.two ? w : 0) * kRows + r;
+      if (!g.whole && valid && done > 0 && (!join || w == 0)) t.part_ml[pslot] = make_float2(m, l);
+      const uint32_t* dirt = dirty + (sg % kRing) * kAncWords;
+      bool dirt_any = false;
+#pragma unroll
+      for (int i = 0; i < kAncWords; ++i) dirt_any |= dirt[i] != 0;
+      // columns this thread writes: all of its row, or its half of a joined row
+      const int c_end = join ? (w + 1) * (D / 2) : done > 0 ? D : 0;
+#pragma unroll 1
+      for (int c = join ? w * (D / 2) : 0; c < c_end; c += 16) {
+        const int in = c - w * (D / 2);                        // place in this group's half
+        if (join && in == kHand) {
+          if (!(ok = meet())) break;
+          hand(1);
           if (!(ok = meet())) break;
         }
-        if (c0 + i < c1) {
-          tmem_ld16(tO + (c0 + i) * 16, o);
-          tmem_ld_wait();
-          if (join) {
+        float o[16];
+        __syncwarp();
+        tmem_ld16(tO + c, o);
+        tmem_ld_wait();
+        if (join) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 v = stage[(w ^ 1) * 512 + e * 128 + r];
-              o[4 * e] = o[4 * e] * fac + v.x;
-              o[4 * e + 1] = o[4 * e + 1] * fac + v.y;
-              o[4 * e + 2] = o[4 * e + 2] * fac + v.z;
-              o[4 * e + 3] = o[4 * e + 3] * fac + v.w;
-            }
-          }
-          if (valid) {
-            if (dirt_any) {
-              // V elements that were not finite count for the rows that see their node
-              for (int d = 0; d < g.s.n; ++d) {
-                if (!((dirt[d >> 5] & anc[node * kAncWords + (d >> 5)]) >> (d & 31) & 1u)) continue;
-                const int key = prefix + d, id = a.block_tables[(int64_t)g.b * a.max_blocks + key / a.block_size];
-                const bf16* v = static_cast<const bf16*>(a.v_cache) + (int64_t)id * a.block_stride +
-                                ((int64_t)g.h * a.block_size + key % a.block_size) * D + (c0 + i) * 16;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float x = __bfloat162float(v[e]);
-                  if (!isfinite(x)) o[e] += x;
-                }
-              }
-            }
-            if (g.whole) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) +
-                                                    ((int64_t)(g.s.q0 + node) * nq + head) * D + (c0 + i) * 16);
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                dst[e] = make_uint4(pack2(o[8 * e] * inv, o[8 * e + 1] * inv), pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                    pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(t.part_o + pslot * D + (c0 + i) * 16);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float4 v = stage[((w ^ 1) * (kHand / 4) + (in % kHand) / 4 + e) * kRows + r];
+            o[4 * e] = o[4 * e] * fac + v.x * ofac;
+            o[4 * e + 1] = o[4 * e + 1] * fac + v.y * ofac;
+            o[4 * e + 2] = o[4 * e + 2] * fac + v.z * ofac;
+            o[4 * e + 3] = o[4 * e + 3] * fac + v.w * ofac;
           }
         }
-        if (join && !(ok = meet())) break;
+        if (valid) {
+          if (dirt_any) {
+            // V elements that were not finite count for the rows that see their node
+            for (int d = 0; d < g.n; ++d) {
+              if (!((dirt[d >> 5] & anc[node * kAncWords + (d >> 5)]) >> (d & 31) & 1u)) continue;
+              const int key = prefix + d, id = a.block_tables[(int64_t)g.b * a.max_blocks + key / a.block_size];
+              const bf16* v = static_cast<const bf16*>(a.v_cache) + (int64_t)id * a.block_stride +
+                              ((int64_t)g.h * a.block_size + key % a.block_size) * D + c;
+#pragma unroll 1
+              for (int e = 0; e < 16; ++e) {
+                const float x = __bfloat162float(v[e]);
+#pragma unroll
+                for (int f = 0; f < 16; ++f)
+                  if (f == e && !isfinite(x)) o[f] += x;
+              }
+            }
+          }
+          if (g.whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + ((int64_t)(g.q0 + node) * nq + head) * D + c);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              dst[e] = make_uint4(pack2(o[8 * e] * inv, o[8 * e + 1] * inv), pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                  pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(t.part_o + pslot * D + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
       }
+      if (!ok) break;
+      if (join) fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&joined[sg % kRing]);
       tc_fence_before();  // O is read before the next segment's first product overwrites it
+      ++sg;
     }
   }
 
@@ -685,67 +835,82 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     tmem_dealloc(tmem, 512);
   }
 
-  // ---- join the parts of items that a share cut (none where every item is one tile)
-  if (*s_max_nt <= 1) return;
+  // ---- join the parts of items that a share cut: a warp per (row, KV head, four query heads)
+  if (plan.whole) return;
   cg::this_grid().sync();
-  const int nq = a.num_kv_heads * G;
-  for (int64_t it = (int64_t)blockIdx.x * (kThreads / 32) + warp; it < (int64_t)a.rows * nq;
-       it += (int64_t)grid * (kThreads / 32)) {
-    const int row = (int)(it / nq), head = (int)(it % nq), h = head / G;
+  constexpr int kHeads = 4;
+  const int nq = a.num_kv_heads * G, quads = (G + kHeads - 1) / kHeads;
+  const int tasks = a.rows * a.num_kv_heads * quads;
+  for (int it = blockIdx.x + gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
+    const int row = it / (a.num_kv_heads * quads), hq = it % (a.num_kv_heads * quads);
+    const int h = hq / quads, g0 = hq % quads * kHeads;
     int lo = 0, up = a.batch;
     while (up - lo > 1) {
       const int mid = (lo + up) >> 1;
-      if (a.cu_seqlens_q[mid] <= row) lo = mid; else up = mid;
+      if (rows[mid].q0 <= row) lo = mid; else up = mid;
     }
-    const int b = lo;
-    if (pu[b + 1] == pu[b]) continue;                      // no keys, or a tree that was left out
-    const Seq s = seq_of(a, b);
-    const int node = row - s.q0;
-    if (node < 0 || node >= s.n) continue;                 // rows behind the last sequence
+    const int b = lo, unit0 = rows[b].unit;
+    if (rows[b + 1].unit == unit0) continue;               // a tree that was left out
+    const int node = row - rows[b].q0;
+    if (node < 0 || node >= plan.nodes(b)) continue;       // rows behind the last sequence
+    const int nt = plan.tiles(b), pr = plan.pairs(b);
     const int rt = node / per, pair = rt / 2;
-    const bool two = s.n > (2 * pair + 1) * per;
-    const int prow = (two ? rt & 1 : 0) * kRows + (node % per) * G + head % G;
-    const Chunks c = chunks_of(s.nt, s.pairs, share);
+    const bool two = plan.nodes(b) > (2 * pair + 1) * per;
+    const int prow = (two ? rt & 1 : 0) * kRows + (node % per) * G + g0;
+    const Chunks c = plan.chunks(nt, pr);
     constexpr int V = D / 32;
-    float acc[V], top = -INFINITY, l = 0.f;
+    float acc[kHeads][V], top[kHeads], l[kHeads];
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int q = 0; q < kHeads; ++q) {
+      top[q] = -INFINITY;
+      l[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[q][i] = 0.f;
+    }
     bool whole = false;
     for (int ci = 0; ci < c.n && !whole; ++ci) {
       const int start = c.start(ci), clen = c.start(ci + 1) - start;
-      const int u0 = pu[b] + (h * s.nt + start) * s.pairs + pair * clen, u1 = u0 + clen;
-      // the CTA whose share holds u0: the largest x with x * W / grid <= u0
-      int x = (int)(((int64_t)u0 * grid + grid - 1) / W);
-      while (share_lo(x, W, grid) > u0) --x;
-      while (share_lo(x + 1, W, grid) <= u0) ++x;
-      for (; x < grid && share_lo(x, W, grid) < u1; ++x) {
-        const int lo_x = share_lo(x, W, grid);
-        if (share_lo(x + 1, W, grid) == lo_x) continue;    // an empty share
-        if (c.n == 1 && lo_x <= u0 && share_lo(x + 1, W, grid) >= u1) { whole = true; break; }
-        const int64_t ps = (int64_t)(x * 2 + (lo_x >= u0 ? 0 : 1)) * t.part_rows + prow;
-        const float2 ml = __ldcg(t.part_ml + ps);
-        const float* po = t.part_o + ps * D + lane * V;
-        float v[V];
-        if constexpr (V == 4) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(po));
-          v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
-          const float2 f = __ldcg(reinterpret_cast<const float2*>(po));
-          v[0] = f.x; v[1] = f.y;
-        }
-        const float nt = fmaxf(top, ml.x);
-        const float fa = top == -INFINITY ? 0.f : ex2(top - nt), fb = ml.x == -INFINITY ? 0.f : ex2(ml.x - nt);
+      const int u0 = unit0 + (h * nt + start) * pr + pair * clen;
+      const int x0 = plan.cta(u0), x1 = plan.cta(u0 + clen - 1);
+      if (c.n == 1 && x0 == x1) { whole = true; break; }
+      for (int x = x0; x <= x1; ++x) {
+        const int64_t ps = (int64_t)(x * 2 + (plan.lo(x) >= u0 ? 0 : 1)) * t.part_rows + prow;
+        float2 ml[kHeads];
+        float v[kHeads][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = acc[i] * fa + v[i] * fb;
-        l = l * fa + ml.y * fb;
-        top = nt;
+        for (int q = 0; q < kHeads; ++q) {
+          if (g0 + q >= G) continue;
+          ml[q] = __ldcg(t.part_ml + ps + q);
+          const float* po = t.part_o + (ps + q) * D + lane * V;
+          if constexpr (V == 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(po));
+            v[q][0] = f.x; v[q][1] = f.y; v[q][2] = f.z; v[q][3] = f.w;
+          } else {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(po));
+            v[q][0] = f.x; v[q][1] = f.y;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kHeads; ++q) {
+          if (g0 + q >= G) continue;
+          const float mt = fmaxf(top[q], ml[q].x);
+          const float fa = top[q] == -INFINITY ? 0.f : ex2(top[q] - mt), fb = ml[q].x == -INFINITY ? 0.f : ex2(ml[q].x - mt);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[q][i] = acc[q][i] * fa + v[q][i] * fb;
+          l[q] = l[q] * fa + ml[q].y * fb;
+          top[q] = mt;
+        }
       }
     }
     if (whole) continue;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + ((int64_t)row * nq + head) * D + lane * V);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) dst[i] = pack2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    for (int q = 0; q < kHeads; ++q) {
+      if (g0 + q >= G) continue;
+      const float inv = l[q] > 0.f ? 1.f / l[q] : 0.f;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + ((int64_t)row * nq + h * G + g0 + q) * D + lane * V);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) dst[i] = pack2(acc[q][2 * i] * inv, acc[q][2 * i + 1] * inv);
+    }
   }
 }
 

@@ -138,6 +138,26 @@ def test_tree_attention(dev, nodes, ctx, nq, nkv, D, bs, kind):
         ops.check_status(got.device)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes,ctx,nq,nkv,D,bs", [
+    ([64], [9000], 32, 4, 128, 256),                 # one request over every SM: parts of one item joined
+    ([256, 100], [2500, 4001], 8, 2, 128, 64),       # the largest tree
+    ([200], [6000], 16, 1, 64, 128),                 # 25 row tiles of one KV head, key chunks
+    ([3, 0, 31, 1, 90], [5000, 7, 1290, 0, 777], 32, 4, 128, 32),
+    ([1] * 7, [1500, 20, 3000, 1, 900, 4000, 130], 4, 2, 64, 16),
+    ([2] * 300, list(range(300)), 8, 8, 64, 16),
+    ([1] * 2300, [i % 5 for i in range(2300)], 4, 4, 64, 8),   # more sequences than one launch takes
+])
+@pytest.mark.parametrize("kind", ["random", "chain"])
+def test_tree_attention_large(nodes, ctx, nq, nkv, D, bs, kind):
+    b = Batch("cuda", nodes, ctx, nq, nkv, D, bs, kind)
+    out = torch.full_like(b.q, 7.0)
+    b.check(ops.tree_attention(*b.args(), out=out))
+    ops.check_status(out.device)
+    again = ops.tree_attention(*b.args())
+    assert torch.equal(out, again)                   # the same shares, joined in the same order
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("mode", ["token", "channel"])
 @pytest.mark.parametrize("D,bs", [(128, 64), (64, 16)])
