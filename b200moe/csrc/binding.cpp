@@ -792,7 +792,8 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   const bool int8 = k_cache.scalar_type() == torch::kInt8;
   TORCH_CHECK(int8 || k_cache.scalar_type() == torch::kBFloat16, "cache must be bf16 or int8");
   check_tree(cu, lens, tables, parents, q.device(), max_q_len);
-  check_aligned(q, "q"); check_aligned(out, "out"); check_aligned(k_cache, "k"); check_aligned(v_cache, "v");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(out.data_ptr()) & 31) == 0, "out must start on a 32-byte boundary");
+  check_aligned(q, "q"); check_aligned(k_cache, "k"); check_aligned(v_cache, "v");
   TORCH_CHECK(block_stride * k_cache.element_size() % 16 == 0, "cache blocks must be multiples of 16 bytes");
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   TORCH_CHECK(parents.numel() == q.size(0), "parents must hold one entry per row of q");

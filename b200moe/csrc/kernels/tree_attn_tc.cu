@@ -56,7 +56,8 @@ namespace {
 namespace cg = cooperative_groups;
 using bf16 = __nv_bfloat16;
 
-constexpr int kRows = 128, kKeys = 128;
+constexpr int kRows = 128, kKeys = 128;   // of a tile
+constexpr int kSub = 64;                  // keys of one score buffer
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
@@ -77,7 +78,7 @@ struct Lay {
   static constexpr int DIRTY = ML + 2 * kRows * 8;
   static constexpr int SEG = DIRTY + kRing * kAncWords * 4;   // [kRing] segments
   static constexpr int BARS = SEG + kRing * 64;
-  static constexpr int NBARS = 5 * SLOTS + 2 + 6 + 3 + 2 * kRing;
+  static constexpr int NBARS = 5 * SLOTS + 2 + 12 + 3 + 2 * kRing;
   static constexpr int TAB = BARS + NBARS * 8 + 32;           // per sequence: Row, then one more
   static int smem(int batch) { return TAB + (batch + 1) * 16 + 1024; }
 };
@@ -91,6 +92,19 @@ struct TcArgs {
 };
 
 __device__ __forceinline__ uint32_t sw_off(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+
+// Whether a phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 
 __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -142,6 +156,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+// 32 bytes in one store
+__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 // two fp32 operations in one instruction, each rounded to nearest
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -229,6 +249,19 @@ struct Seg {
 };
 static_assert(sizeof(Seg) == 64, "segment ring");
 
+// The key tiles of a segment that softmax group w takes, in runs of 64 keys.
+struct Own {
+  int first, step, subs;
+  __device__ __forceinline__ Own(const Seg& g, int gt, int w) {
+    step = g.two ? 1 : 2;
+    first = g.two || (gt & 1) == w ? g.t0 : g.t0 + 1;
+    const int n = first < g.t1 ? (g.t1 - 1 - first) / step + 1 : 0;
+    // the sequence's last keys may not reach the second half of their tile
+    subs = 2 * n - (n > 0 && g.len - (first + (n - 1) * step) * kKeys <= kSub ? 1 : 0);
+  }
+  __device__ __forceinline__ int tile(int s) const { return first + (s >> 1) * step; }
+};
+
 __device__ __forceinline__ Seg seg_at(const Plan& p, int u, int lo, int hi) {
   Seg g;
   g.b = p.at(u, false);
@@ -274,10 +307,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   uint64_t* v_empty = v_ready + kSlots;
   uint64_t* q_full = v_empty + kSlots;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;         // [2] per softmax group
-  uint64_t* p_full = s_full + 2;
-  uint64_t* pv_done = p_full + 2;
-  uint64_t* fin = pv_done + 2;            // [2] an issuer's last products
+  uint64_t* s_full = q_empty + 1;         // [2][2] per softmax group and score buffer
+  uint64_t* p_full = s_full + 4;          // [2][2]
+  uint64_t* pv_done = p_full + 4;         // [2][2]
+  uint64_t* fin = pv_done + 4;            // [2] an issuer's last products
   uint64_t* both = fin + 2;               // the eight softmax warps meet
   uint64_t* joined = both + 1;            // [kRing] the softmax warps are done with the segment's join
   uint64_t* seg_full = joined + kRing;    // [kRing]
@@ -324,9 +357,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     mbar_init(q_full, 1);
     mbar_init(q_empty, 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_full[2 * i + k], 1);
+        mbar_init(&p_full[2 * i + k], 4);
+        mbar_init(&pv_done[2 * i + k], 1);
+      }
       mbar_init(&fin[i], 1);
     }
     mbar_init(both, 8);
@@ -466,47 +501,80 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // ================================================================ MMA issuer of group w
     if (lane == 0) {
       const int w = warp - 1;
-      const uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys);
+      const uint32_t idesc_s = umma_idesc_bf16(kRows, kSub);
       const uint32_t idesc_pv = umma_idesc_bf16(kRows, D) | (1u << 16);  // B (V) is MN-major
       const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
-      int gt = 0, sg = 0, mine = 0;   // tiles of the CTA, segments, tiles of this group
+      int gt = 0, sg = 0, mine = 0;   // tiles of the CTA, segments, runs of this group
       bool ok = true;
       Seg g;
       for (; ok && segment(sg, g); ++sg) {
-        if (!mbar_wait(q_full, sg & 1, status, kStatusTimeoutFull, abort_flag)) { ok = false; break; }
+        if (!mbar_wait(q_full, sg & 1, status, kStatusTimeoutFull, abort_flag)) break;
         const uint32_t qa = smem_u32(smem + L::Q + (g.two ? w : 0) * L::TILE);
-        bool first = true;
-        for (int j = g.t0; j < g.t1; ++j, ++gt) {
-          if (!g.two && (gt & 1) != w) continue;
-          const int slot = gt % kSlots;
-          const uint32_t ph = (gt / kSlots) & 1;
-          // S overlays the group's last P: that product has to be done
-          if (mine > 0 && !mbar_wait(&pv_done[w], (mine - 1) & 1, status, kStatusTimeoutAccEmpty, abort_flag)) { ok = false; break; }
-          if (!mbar_wait(&k_full[slot], ph, status, kStatusTimeoutFull, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t kb = smem_u32(smem + L::K + slot * L::TILE);
+        const Own own(g, gt, w);
+        auto issue_s = [&](int s) {
+          const int slot = (gt + own.tile(s) - g.t0) % kSlots, buf = (mine + s) & 1;
+          const uint32_t kb = smem_u32(smem + L::K + slot * L::TILE) + (s & 1) * (kSub * 128);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * L::HALF + (k & 3) * 32;
-            umma_f16_ss(tS, umma_sdesc_sw128(qa + off), umma_sdesc_sw128(kb + off), idesc_s, k > 0 ? 1u : 0u);
+            umma_f16_ss(tS + buf * kSub, umma_sdesc_sw128(qa + off), umma_sdesc_sw128(kb + off), idesc_s, k > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
-          umma_commit(&k_empty[slot]);
-          if (!g.two) umma_commit(&k_empty[slot]);   // the other group does not read this tile
-          if (!mbar_wait(&p_full[w], mine & 1, status, kStatusTimeoutConv, abort_flag)) { ok = false; break; }
-          if (!mbar_wait(&v_ready[slot], ph, status, kStatusTimeoutFull, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t vb = smem_u32(smem + L::V + slot * L::TILE);
+          umma_commit(&s_full[2 * w + buf]);
+          if ((s & 1) || s + 1 == own.subs) {
+            umma_commit(&k_empty[slot]);
+            if (!g.two) umma_commit(&k_empty[slot]);   // the other group does not read this tile
+          }
+        };
+        auto issue_pv = [&](int s) {
+          const int slot = (gt + own.tile(s) - g.t0) % kSlots, buf = (mine + s) & 1;
+          const uint32_t vb = smem_u32(smem + L::V + slot * L::TILE) + (s & 1) * (kSub * 128);
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_f16_ts(tO, tS + k * 8, sdesc_mn(vb + k * 16 * 128, L::HALF), idesc_pv, (!first || k > 0) ? 1u : 0u);
-          umma_commit(&pv_done[w]);
-          umma_commit(&v_empty[slot]);
-          if (!g.two) umma_commit(&v_empty[slot]);
-          first = false;
-          ++mine;
+          for (int k = 0; k < kSub / 16; ++k)
+            umma_f16_ts(tO, tS + buf * kSub + k * 8, sdesc_mn(vb + k * 16 * 128, L::HALF), idesc_pv, (s > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&pv_done[2 * w + buf]);
+          if ((s & 1) || s + 1 == own.subs) {
+            umma_commit(&v_empty[slot]);
+            if (!g.two) umma_commit(&v_empty[slot]);
+          }
+        };
+        // Scores run up to two runs ahead; whichever product has its inputs goes first (waiting for
+        // the next K here would hold back the product that frees a V tile).
+        int si = 0, pi = 0;
+        uint64_t since = 0;
+        while (pi < own.subs) {
+          bool did = false;
+          if (si < own.subs && si < pi + 2) {
+            const int at = gt + own.tile(si) - g.t0;
+            // the scores overlay the P of the run two before
+            if ((si < 2 || mbar_test(&pv_done[2 * w + ((mine + si) & 1)], ((mine + si - 2) >> 1) & 1)) &&
+                ((si & 1) || mbar_test(&k_full[at % kSlots], (at / kSlots) & 1))) {
+              tc_fence_after();
+              issue_s(si++);
+              did = true;
+            }
+          }
+          if (pi < si && mbar_test(&p_full[2 * w + ((mine + pi) & 1)], ((mine + pi) >> 1) & 1)) {
+            const int at = gt + own.tile(pi) - g.t0;
+            if ((pi & 1) || mbar_test(&v_ready[at % kSlots], (at / kSlots) & 1)) {
+              tc_fence_after();
+              issue_pv(pi++);
+              did = true;
+            }
+          }
+          if (did) {
+            since = 0;
+          } else if (since == 0) {
+            since = globaltimer_ns();
+          } else if (*abort_flag || globaltimer_ns() - since > kWaitLimitNs) {
+            if (!*abort_flag) record_status(status, kStatusTimeoutConv);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
         }
         if (!ok) break;
+        mine += own.subs;
+        gt += g.t1 - g.t0;
         // the segment's products are done (its Q, and every K and V phase before the next)
         umma_commit(q_empty);
       }
@@ -580,6 +648,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const bool here = mbar_wait(both, syncs++ & 1, status, kStatusTimeoutFlag, abort_flag);
       return __all_sync(0xffffffffu, here) != 0;
     };
+    // product i of this group has been added to O (the one two before it is known to be)
+    auto pv_over = [&](int i) {
+      return mbar_wait(&pv_done[2 * w + (i & 1)], (i >> 1) & 1, status, kStatusTimeoutAccEmpty, abort_flag);
+    };
     Seg g;
     while (ok && __all_sync(0xffffffffu, segment(sg, g))) {
       const int prefix = g.len - g.n;
@@ -621,42 +693,37 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         return see;
       };
       float m = -INFINITY, l = 0.f;
-      int done = 0;                              // tiles of this group in the segment
-      for (int j = g.t0; j < g.t1; ++j, ++gt) {
-        if (!g.two && (gt & 1) != w) continue;
-        ok = mbar_wait(&s_full[w], mine & 1, status, kStatusTimeoutAccFull, abort_flag);
+      const Own own(g, gt, w);
+      const int done = own.subs;
+#pragma unroll 1
+      for (int i = 0; i < own.subs; ++i, ++mine) {
+        const int buf = mine & 1;
+        const uint32_t tb = tS + buf * kSub;
+        ok = mbar_wait(&s_full[2 * w + buf], (mine >> 1) & 1, status, kStatusTimeoutAccFull, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (any) {
-          const int kb = j * kKeys;
-          const bool tail = kb + kKeys > prefix;
-          // The row goes through registers twice, 64 columns at a time: a loop of two keeps the
-          // code small (a cold instruction cache costs more than the second read of TMEM).
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < kKeys; c += 64) {
-            float s[64];
-            tmem_ld<32>(tS + c, s);
-            tmem_ld<32>(tS + c + 32, s + 32);
-            tmem_ld_wait();
-            if (tail) {
-              const uint32_t lo = sees(kb, c), hi = sees(kb, c + 32);
+          const int kb = own.tile(i) * kKeys + (i & 1) * kSub;
+          float s[kSub];
+          tmem_ld<32>(tb, s);
+          tmem_ld<32>(tb + 32, s + 32);
+          tmem_ld_wait();
+          if (kb + kSub > prefix) {
+            const uint32_t lo = sees(kb, 0), hi = sees(kb, 32);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                if (!((lo >> i) & 1u)) s[i] = -INFINITY;
-                if (!((hi >> i) & 1u)) s[32 + i] = -INFINITY;
-              }
+            for (int e = 0; e < 32; ++e) {
+              if (!((lo >> e) & 1u)) s[e] = -INFINITY;
+              if (!((hi >> e) & 1u)) s[32 + e] = -INFINITY;
             }
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = fmaxf(s[i], s[8 + i]);
-#pragma unroll
-            for (int q = 2; q < 8; ++q)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], s[8 * q + i]);
-            mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
           }
-          mx *= sl2;
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fmaxf(s[e], s[8 + e]);
+#pragma unroll
+          for (int q = 2; q < 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], s[8 * q + e]);
+          const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sl2;
           const bool grow = mx > m + kLazyLog2;
           if (__any_sync(0xffffffffu, grow)) {
             float alpha = 1.f;
@@ -665,7 +732,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
               m = mx;
               l *= alpha;
             }
-            if (done > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+              // the product before this one may still be adding to O
+              ok = pv_over(mine - 1);
+              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 float o[16];
@@ -673,7 +744,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 tmem_ld_wait();
                 uint32_t ou[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ou[i] = __float_as_uint(o[i] * alpha);
+                for (int e = 0; e < 16; ++e) ou[e] = __float_as_uint(o[e] * alpha);
                 tmem_st16(tO + c * 16, ou);
               }
             }
@@ -682,48 +753,31 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           const float mu = m == -INFINITY ? 0.f : -m;
           const float2 mu2 = make_float2(mu, mu);
           float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll 1
-          for (int c = 0; c < kKeys; c += 64) {
-            float s[64];
-            tmem_ld<32>(tS + c, s);
-            tmem_ld<32>(tS + c + 32, s + 32);
-            tmem_ld_wait();
-            if (tail) {
-              const uint32_t lo = sees(kb, c), hi = sees(kb, c + 32);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                if (!((lo >> i) & 1u)) s[i] = -INFINITY;
-                if (!((hi >> i) & 1u)) s[32 + i] = -INFINITY;
-              }
+          for (int q = 0; q < 2; ++q) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 z = fma2(make_float2(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), k2, mu2);
+              p[e] = pack2(ex2(z.x), ex2(z.y));
+              const float2 back = make_float2(__uint_as_float(p[e] << 16), __uint_as_float(p[e] & 0xffff0000u));
+              if (e & 1) sum1 = add2(sum1, back); else sum0 = add2(sum0, back);
             }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t p[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 z = fma2(make_float2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), k2, mu2);
-                p[i] = pack2(ex2(z.x), ex2(z.y));
-                const float2 back = make_float2(__uint_as_float(p[i] << 16), __uint_as_float(p[i] & 0xffff0000u));
-                if (i & 1) sum1 = add2(sum1, back); else sum0 = add2(sum0, back);
-              }
-              // P overlays S: columns [c / 2, c / 2 + 32) have been read by this thread
-              tmem_st16(tS + c / 2 + q * 16, p);
-            }
+            tmem_st16(tb + q * 16, p);           // P overlays its scores, which this thread has read
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_st_wait();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[w]);
-        ++mine;
-        ++done;
+        if (lane == 0) mbar_arrive(&p_full[2 * w + buf]);
       }
+      gt += g.t1 - g.t0;
       if (!ok) break;
       // ---------------------------------------------------------------- epilogue
       const bool join = !g.two && g.t1 - g.t0 > 1;   // both groups hold a part of every row
       if (done > 0) {
-        ok = mbar_wait(&pv_done[w], (mine - 1) & 1, status, kStatusTimeoutAccEmpty, abort_flag);
+        ok = pv_over(mine - 1);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
       }
@@ -759,8 +813,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         m = top;
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int64_t pslot = (int64_t)(blockIdx.x * 2 + g.slot) * t.part_rows + (g.two ? w : 0) * kRows + r;
-      if (!g.whole && valid && done > 0 && (!join || w == 0)) t.part_ml[pslot] = make_float2(m, l);
+      const int64_t pblk = blockIdx.x * 2 + g.slot;
+      const int prow = (g.two ? w : 0) * kRows + r;
+      if (!g.whole && valid && done > 0 && (!join || w == 0)) t.part_ml[pblk * t.part_rows + prow] = make_float2(m, l);
       const uint32_t* dirt = dirty + (sg % kRing) * kAncWords;
       bool dirt_any = false;
 #pragma unroll
@@ -807,15 +862,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             }
           }
           if (g.whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + ((int64_t)(g.q0 + node) * nq + head) * D + c);
+            uint32_t v[8];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              dst[e] = make_uint4(pack2(o[8 * e] * inv, o[8 * e + 1] * inv), pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                  pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+            for (int e = 0; e < 8; ++e) v[e] = pack2(o[2 * e] * inv, o[2 * e + 1] * inv);
+            st32(static_cast<bf16*>(a.out) + ((int64_t)(g.q0 + node) * nq + head) * D + c, v);
           } else {
-            float4* dst = reinterpret_cast<float4*>(t.part_o + pslot * D + c);
+            // columns by fours, rows inside: a warp's stores are contiguous
+            float4* dst = reinterpret_cast<float4*>(t.part_o) + (pblk * (D / 4) + c / 4) * t.part_rows + prow;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) dst[e * t.part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
       }
@@ -835,82 +890,75 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     tmem_dealloc(tmem, 512);
   }
 
-  // ---- join the parts of items that a share cut: a warp per (row, KV head, four query heads)
+  // ---- join the parts of items that a share cut: a lane per row (node and query head) and 16 columns
   if (plan.whole) return;
   cg::this_grid().sync();
-  constexpr int kHeads = 4;
-  const int nq = a.num_kv_heads * G, quads = (G + kHeads - 1) / kHeads;
-  const int tasks = a.rows * a.num_kv_heads * quads;
-  for (int it = blockIdx.x + gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
-    const int row = it / (a.num_kv_heads * quads), hq = it % (a.num_kv_heads * quads);
-    const int h = hq / quads, g0 = hq % quads * kHeads;
+  const int nq = a.num_kv_heads * G, qrows = a.rows * G, groups = (qrows + 31) / 32;
+  const int64_t tasks = (int64_t)groups * a.num_kv_heads * (D / 16);
+  for (int64_t it = blockIdx.x + (int64_t)gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
+    const int c4 = (int)(it % (D / 16)) * 4, h = (int)(it / (D / 16) % a.num_kv_heads);
+    const int qr = (int)(it / (D / 16) / a.num_kv_heads) * 32 + lane;
+    if (qr >= qrows) continue;
+    const int row = qr / G, hg = qr % G;
     int lo = 0, up = a.batch;
     while (up - lo > 1) {
       const int mid = (lo + up) >> 1;
       if (rows[mid].q0 <= row) lo = mid; else up = mid;
     }
     const int b = lo, unit0 = rows[b].unit;
-    if (rows[b + 1].unit == unit0) continue;               // a tree that was left out
     const int node = row - rows[b].q0;
-    if (node < 0 || node >= plan.nodes(b)) continue;       // rows behind the last sequence
+    // nothing to do for a tree that was left out and for rows behind the last sequence
+    if (rows[b + 1].unit == unit0 || node < 0 || node >= plan.nodes(b)) continue;
     const int nt = plan.tiles(b), pr = plan.pairs(b);
     const int rt = node / per, pair = rt / 2;
     const bool two = plan.nodes(b) > (2 * pair + 1) * per;
-    const int prow = (two ? rt & 1 : 0) * kRows + (node % per) * G + g0;
+    const int prow = (two ? rt & 1 : 0) * kRows + (node % per) * G + hg;
     const Chunks c = plan.chunks(nt, pr);
-    constexpr int V = D / 32;
-    float acc[kHeads][V], top[kHeads], l[kHeads];
+    float acc[16], top = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int q = 0; q < kHeads; ++q) {
-      top[q] = -INFINITY;
-      l[q] = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[q][i] = 0.f;
-    }
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool whole = false;
     for (int ci = 0; ci < c.n && !whole; ++ci) {
       const int start = c.start(ci), clen = c.start(ci + 1) - start;
       const int u0 = unit0 + (h * nt + start) * pr + pair * clen;
       const int x0 = plan.cta(u0), x1 = plan.cta(u0 + clen - 1);
       if (c.n == 1 && x0 == x1) { whole = true; break; }
-      for (int x = x0; x <= x1; ++x) {
-        const int64_t ps = (int64_t)(x * 2 + (plan.lo(x) >= u0 ? 0 : 1)) * t.part_rows + prow;
-        float2 ml[kHeads];
-        float v[kHeads][V];
+      for (int x = x0; x <= x1; x += 2) {
+        float2 ml[2];
+        float4 v[2][4];
 #pragma unroll
-        for (int q = 0; q < kHeads; ++q) {
-          if (g0 + q >= G) continue;
-          ml[q] = __ldcg(t.part_ml + ps + q);
-          const float* po = t.part_o + (ps + q) * D + lane * V;
-          if constexpr (V == 4) {
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(po));
-            v[q][0] = f.x; v[q][1] = f.y; v[q][2] = f.z; v[q][3] = f.w;
-          } else {
-            const float2 f = __ldcg(reinterpret_cast<const float2*>(po));
-            v[q][0] = f.x; v[q][1] = f.y;
-          }
+        for (int k = 0; k < 2; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.f);
+          if (x + k > x1) continue;
+          const int64_t pblk = (x + k) * 2 + (plan.lo(x + k) >= u0 ? 0 : 1);
+          ml[k] = __ldcg(t.part_ml + pblk * t.part_rows + prow);
+          const float4* po = reinterpret_cast<const float4*>(t.part_o) + (pblk * (D / 4) + c4) * t.part_rows + prow;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[k][e] = __ldcg(po + e * t.part_rows);
         }
 #pragma unroll
-        for (int q = 0; q < kHeads; ++q) {
-          if (g0 + q >= G) continue;
-          const float mt = fmaxf(top[q], ml[q].x);
-          const float fa = top[q] == -INFINITY ? 0.f : ex2(top[q] - mt), fb = ml[q].x == -INFINITY ? 0.f : ex2(ml[q].x - mt);
+        for (int k = 0; k < 2; ++k) {
+          if (x + k > x1) continue;
+          const float mt = fmaxf(top, ml[k].x);
+          const float fa = top == -INFINITY ? 0.f : ex2(top - mt), fb = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - mt);
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[q][i] = acc[q][i] * fa + v[q][i] * fb;
-          l[q] = l[q] * fa + ml[q].y * fb;
-          top[q] = mt;
+          for (int e = 0; e < 4; ++e) {
+            acc[4 * e] = acc[4 * e] * fa + v[k][e].x * fb;
+            acc[4 * e + 1] = acc[4 * e + 1] * fa + v[k][e].y * fb;
+            acc[4 * e + 2] = acc[4 * e + 2] * fa + v[k][e].z * fb;
+            acc[4 * e + 3] = acc[4 * e + 3] * fa + v[k][e].w * fb;
+          }
+          l = l * fa + ml[k].y * fb;
+          top = mt;
         }
       }
     }
     if (whole) continue;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t v[8];
 #pragma unroll
-    for (int q = 0; q < kHeads; ++q) {
-      if (g0 + q >= G) continue;
-      const float inv = l[q] > 0.f ? 1.f / l[q] : 0.f;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + ((int64_t)row * nq + h * G + g0 + q) * D + lane * V);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) dst[i] = pack2(acc[q][2 * i] * inv, acc[q][2 * i + 1] * inv);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    st32(static_cast<bf16*>(a.out) + ((int64_t)row * nq + h * G + hg) * D + c4 * 4, v);
   }
 }
 
