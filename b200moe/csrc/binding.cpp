@@ -932,8 +932,9 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
                   (*t)->scalar_type() == (t == &ids ? torch::kInt32 : torch::kFloat32),
                   "ids (int32) and weights (fp32) must be [tokens, topk]");
   c10::cuda::CUDAGuard guard(x.device());
-  auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor logits = torch::empty({T, E}, f32), h = torch::empty({T * topk, I}, f32);
+  // [slots | hidden rows | logits | counters]
+  const int64_t n_slots = T * topk * H, n_h = T * topk * I, n_logits = (T * E + 3) / 4 * 4;
+  Tensor ws = torch::empty({n_slots + n_h + n_logits + H / 32}, x.options().dtype(torch::kFloat32));
   b200::MoeFewArgs a{};
   a.x = x.data_ptr();
   a.router = router.data_ptr();
@@ -947,8 +948,10 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
   a.out = out.data_ptr();
   a.ids = ptr_or_null<int>(ids);
   a.weights = ptr_or_null<float>(weights);
-  a.logits = logits.data_ptr<float>();
-  a.h = h.data_ptr();
+  a.slots = ws.data_ptr<float>();
+  a.h = a.slots + n_slots;
+  a.logits = a.slots + n_slots + n_h;
+  a.done = reinterpret_cast<int*>(a.logits + n_logits);
   a.status = status.data_ptr<int>();
   b200::moe_few(a, stream());
 }

@@ -22,8 +22,11 @@ struct MoeFewArgs {
   void* out;                 // [T, H] bf16
   int* ids;                  // [T, topk] chosen experts, may be null
   float* weights;            // [T, topk] their weights, may be null
-  float* logits;             // workspace [T, E]
-  void* h;                   // workspace [T * topk, I] fp32
+  // workspace, 16-byte aligned
+  float* logits;             // [T, E]
+  void* h;                   // [2, T * topk, I] bf16: hidden values and what their rounding leaves
+  float* slots;              // [T * topk, H]
+  int* done;                 // [H / 32]
   int* status;
 };
 void moe_few(const MoeFewArgs& a, cudaStream_t s);
