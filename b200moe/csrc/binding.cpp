@@ -932,9 +932,11 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
                   (*t)->scalar_type() == (t == &ids ? torch::kInt32 : torch::kFloat32),
                   "ids (int32) and weights (fp32) must be [tokens, topk]");
   c10::cuda::CUDAGuard guard(x.device());
-  // [slots | hidden rows | logits | counters]
-  const int64_t n_slots = T * topk * H, n_h = T * topk * I, n_logits = (T * E + 3) / 4 * 4;
-  Tensor ws = torch::empty({n_slots + n_h + n_logits + H / 32}, x.options().dtype(torch::kFloat32));
+  // [slots | hidden rows | their factors | x as f16 | logits | x factors | counters], floats
+  const int64_t P = T * topk, at_h = P * H, at_hf = at_h + P * I, at_x = at_hf + P * (I / 16), at_l = at_x + T * H / 2,
+                at_xf = at_l + (T * E + 3) / 4 * 4, at_done = at_xf + (T + 3) / 4 * 4;
+  Tensor ws = torch::empty({at_done + H / 32}, x.options().dtype(torch::kFloat32));
+  float* const w = ws.data_ptr<float>();
   b200::MoeFewArgs a{};
   a.x = x.data_ptr();
   a.router = router.data_ptr();
@@ -948,10 +950,13 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
   a.out = out.data_ptr();
   a.ids = ptr_or_null<int>(ids);
   a.weights = ptr_or_null<float>(weights);
-  a.slots = ws.data_ptr<float>();
-  a.h = a.slots + n_slots;
-  a.logits = a.slots + n_slots + n_h;
-  a.done = reinterpret_cast<int*>(a.logits + n_logits);
+  a.slots = w;
+  a.h = w + at_h;
+  a.h_factor = w + at_hf;
+  a.x16 = w + at_x;
+  a.logits = w + at_l;
+  a.x_factor = w + at_xf;
+  a.done = reinterpret_cast<int*>(w + at_done);
   a.status = status.data_ptr<int>();
   b200::moe_few(a, stream());
 }

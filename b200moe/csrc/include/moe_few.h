@@ -24,7 +24,10 @@ struct MoeFewArgs {
   float* weights;            // [T, topk] their weights, may be null
   // workspace, 16-byte aligned
   float* logits;             // [T, E]
-  void* h;                   // [2, T * topk, I] bf16: hidden values and what their rounding leaves
+  void* x16;                 // e4m3 weights: [T, H] f16, x / x_factor
+  float* x_factor;           // [T]
+  void* h;                   // [T * topk, I] f16, h / h_factor (e4m3 weights), or [2, T * topk, I] bf16
+  float* h_factor;           // [T * topk, I / 16]
   float* slots;              // [T * topk, H]
   int* done;                 // [H / 32]
   int* status;

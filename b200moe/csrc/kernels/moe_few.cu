@@ -11,28 +11,32 @@
 // Nearly all the time goes into reading the touched experts' weights once, so the
 // kernel is built around that stream.  Four warps (a team) take 32 weight rows of one
 // expert -- 16 gate and the 16 up rows beside them, or 32 rows of Wd -- and a quarter of
-// K each.  Every warp brings its own weights into its own ring of three 4 KB stages
-// with bulk copies that its first lane issues, so nothing but the two grid barriers
-// ever drains the stream: a ring is refilled across items, and in front of the second
-// barrier with the first rows of Wd.  16 warps x 12 KB keep up to 192 KB per SM in
-// flight.  The products are warp-level MMAs with the weights as the 16-row operand and
-// up to 16 tokens as columns.  K is permuted alike in both operands so that a lane's
-// operand is 16 contiguous weights of a row.  e4m3 becomes bf16 exactly; the block
-// scale multiplies the fp32 sum of each 64 weights, so a weight counts as exactly
-// q * scale.  Hidden values enter the second product as two bf16 (value and rest),
-// 16 bits of each.  The quarters of K are added in order through shared memory.  The
-// rows of Wd write fp32 (token, k) slots, and the team that finishes the last expert of
+// K each, for up to 8 of its tokens at a time.  Every lane brings what it multiplies
+// itself, weights and tokens alike, into its own places of a ring per warp (16-byte
+// asynchronous copies): no bank conflict lies on the way, any weight layout is an address
+// rule, and nothing that comes from memory is waited for in a register.  The ring is
+// refilled across items, and in front of the second grid barrier with the first rows of
+// Wd.  The products are warp-level MMAs with the weights as the 16-row operand and the
+// tokens as columns.  K is permuted alike in both operands so that a lane's operand is 16
+// weights of a row.
+//
+// Operand types.  e4m3 converts to f16 exactly in one instruction for two values (bf16
+// would take four), so the tokens enter as f16 too: each row of x times the power of
+// two that brings its largest value to [2^14, 2^15), which keeps every bit of a bf16
+// value down to 2^-28 of the row's largest, and hidden values with such a factor for
+// each 16 of them (11 bits of each value).  The factors and the block scale multiply
+// fp32 sums of 64 products, so a weight counts as exactly q * scale.  With bf16
+// weights x enters as it is and a hidden value as two bf16, value and rest.
+//
+// The quarters of K are added in order through shared memory.  The rows of Wd write fp32 (token, k) slots, and the team that finishes the last expert of
 // a block of 32 columns adds the token's slots in the order of the top-k.
 //
 // Rounding points: the logits and the routing weights are rounded to bf16 (those of the
-// model's router), the output once.  Every wait for a copy is bounded (sm100.cuh); after
-// one gives up the warps run on without waiting and the status word says so.
+// model's router), the output once.
 #include <cooperative_groups.h>
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -54,7 +58,8 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTeam = 4;                 // warps of a team, each a part of K
 constexpr int kTeams = kWarps / kTeam;
-constexpr int kStages = 3, kStageBytes = 4096;
+constexpr int kRingBytes = 12928;        // of a warp
+constexpr int kCols = 8;                 // tokens of one pass
 
 // fp64 -> bf16 in one rounding: fp32 with round-to-odd keeps the bit that decides a tie.
 __device__ __forceinline__ float bf16_of(double v) {
@@ -68,6 +73,7 @@ struct Shared {
   int start[kFewMaxExperts + 1];        // first pair of each expert
   int touched[kFewMaxExperts];          // experts with at least one token
   int n_touched;
+  int2 warp_sums[kFewMaxExperts / 32];
   short pair[kFewMaxTokens * kFewMaxTopk];   // pairs (token * topk + k) in (expert, token) order
   short sel_e[kFewMaxTokens * kFewMaxTopk];
   float sel_w[kFewMaxTokens * kFewMaxTopk];
@@ -76,14 +82,18 @@ struct Shared {
 // Logits of experts blockIdx.x, blockIdx.x + gridDim.x, ...: a product of two bf16 is exact in
 // fp32 and the sum of four stays so for nearly all of them; beyond that the sum runs in fp64,
 // because a logit is rounded to bf16 and a wrong last bit there can change the experts.
-__device__ void few_logits(const MoeFewArgs& a) {
+__device__ void few_logits(const MoeFewArgs& a, double* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // few tokens: several warps share one, a part of K each
+  const int share = a.T > 8 ? 1 : a.T > 4 ? 2 : a.T > 2 ? 4 : a.T > 1 ? 8 : 16;
+  const int sub = warp % share;
   for (int e = blockIdx.x; e < a.E; e += gridDim.x) {
     const bf16* wr = static_cast<const bf16*>(a.router) + (int64_t)e * a.H;
-    for (int t = warp; t < a.T; t += kWarps) {
+    for (int t = warp / share; t < a.T; t += kWarps / share) {
       const bf16* xr = static_cast<const bf16*>(a.x) + (int64_t)t * a.H;
       double acc = 0.0;
-      for (int c = lane * 8; c < a.H; c += 256) {
+#pragma unroll 4
+      for (int c = (sub * 32 + lane) * 8; c < a.H; c += share * 256) {
         const uint4 wv = *reinterpret_cast<const uint4*>(wr + c), xv = *reinterpret_cast<const uint4*>(xr + c);
         const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w}, xu[4] = {xv.x, xv.y, xv.z, xv.w};
         float p[8];
@@ -97,58 +107,107 @@ __device__ void few_logits(const MoeFewArgs& a) {
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      if (lane == 0) a.logits[t * a.E + e] = bf16_of(acc);
+      if (share == 1) {
+        if (lane == 0) a.logits[t * a.E + e] = bf16_of(acc);
+      } else if (lane == 0) {
+        red[warp] = acc;
+      }
+    }
+    if (share > 1) {
+      __syncthreads();
+      if (threadIdx.x < a.T) {
+        double acc = 0.0;
+        for (int i = 0; i < share; ++i) acc += red[threadIdx.x * share + i];
+        a.logits[threadIdx.x * a.E + e] = bf16_of(acc);
+      }
+      __syncthreads();
     }
   }
 }
 
+// The power of two f with |v| / f in [2^14, 2^15) for the largest |v| = top of a row; 1 where top
+// is not finite, the smallest normal number where it is zero or tiny.
+__device__ __forceinline__ float factor_of(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23);   // biased exponent, sign is 0
+  return e == 255 ? 1.f : __uint_as_float((uint32_t)max(e - 14, 1) << 23);
+}
+
+// f16 rows of x and their factors: row t by CTA gridDim.x - 1 - t.
+__device__ void few_rows(const MoeFewArgs& a, float* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int t = gridDim.x - 1 - blockIdx.x; t < a.T; t += gridDim.x) {
+    const bf16* xr = static_cast<const bf16*>(a.x) + (int64_t)t * a.H;
+    uint32_t top = 0;   // largest |x| as bits: an infinity or NaN is above every number
+    for (int c = threadIdx.x * 2; c < a.H; c += kThreads * 2) {
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(xr + c) & 0x7fff7fffu;
+      top = max(top, max(v << 16, v & 0xffff0000u));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) red[warp] = __uint_as_float(top);
+    __syncthreads();
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) top = max(top, __float_as_uint(red[i]));
+    const float f = factor_of(__uint_as_float(top)), inv = 1.f / f;   // a power of two: exact
+    for (int c = threadIdx.x * 2; c < a.H; c += kThreads * 2) {
+      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(xr + c));
+      *reinterpret_cast<__half2*>(static_cast<__half*>(a.x16) + (int64_t)t * a.H + c) = __floats2half2_rn(v.x * inv, v.y * inv);
+    }
+    if (threadIdx.x == 0) a.x_factor[t] = f;
+    __syncthreads();
+  }
+}
+
 // Top-k and weights of every token and the pairs in expert order; every CTA does all of it.
+template <int EPL>
 __device__ void few_route(const MoeFewArgs& a, Shared& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int EPL = kFewMaxExperts / 32;
-  for (int e = threadIdx.x; e < a.E; e += kThreads) s.mask[e] = 0;
+  for (int e = threadIdx.x; e < kFewMaxExperts; e += kThreads) s.mask[e] = 0;
+  __syncthreads();
   for (int t = warp; t < a.T; t += kWarps) {
     float v[EPL];
     uint32_t key[EPL];
 #pragma unroll
+    for (int j = 0; j < EPL; ++j) v[j] = j * 32 + lane < a.E ? __ldcg(a.logits + t * a.E + j * 32 + lane) : -INFINITY;
+#pragma unroll
     for (int j = 0; j < EPL; ++j) {
       const int e = j * 32 + lane;
-      v[j] = e < a.E ? __ldcg(a.logits + t * a.E + e) : -INFINITY;
       // (logit, lowest id first) as one unsigned key: bf16 bits in order, then 0xffff - id
       uint32_t u = __float_as_uint(v[j]) >> 16;
       u = (u & 0x8000u) ? (0xffffu ^ u) : (u | 0x8000u);
       key[j] = e < a.E ? (u << 16) | (0xffffu - e) : 0u;
     }
-    int pick = 0;
-    float mx = 0.f, w = 0.f, wsum = 0.f, sum = 0.f;
+    uint32_t mine = 0;             // lane k: the k-th key
+    uint32_t first = 0;
     for (int k = 0; k < a.topk; ++k) {
-      uint32_t best = 0;
+      uint32_t best = key[0];
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) best = max(best, key[j]);
+      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
       best = __reduce_max_sync(0xffffffffu, best);
-      const int e = 0xffff - (int)(best & 0xffffu);
-      uint32_t u = best >> 16;
-      u = (u & 0x8000u) ? (u & 0x7fffu) : (0xffffu ^ u);
-      const float l = __uint_as_float(u << 16);
-      if (k == 0) {
-        mx = l;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) sum += j * 32 + lane < a.E ? expf(v[j] - mx) : 0.f;
-        sum = warp_sum(sum);
-      }
-      const float p = expf(l - mx) / sum;
-      wsum += p;
-      if (lane == k) { pick = e; w = p; }
+      if (k == 0) first = best;
+      if (lane == k) mine = best;
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
         if (key[j] == best) key[j] = 0u;
     }
+    auto logit_of = [](uint32_t k) {
+      const uint32_t u = k >> 16;
+      return __uint_as_float(((u & 0x8000u) ? (u & 0x7fffu) : (0xffffu ^ u)) << 16);
+    };
+    const float mx = logit_of(first);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) sum += expf(v[j] - mx);     // no expert: exp(-inf) = 0
+    sum = warp_sum(sum);
+    float w = lane < a.topk ? expf(logit_of(mine) - mx) / sum : 0.f;
+    const float wsum = warp_sum(w);
     if (lane < a.topk) {
       if (a.renorm) w /= wsum;
       w = __bfloat162float(__float2bfloat16(w));
-      const int p = t * a.topk + lane;
+      const int p = t * a.topk + lane, pick = 0xffff - (int)(mine & 0xffffu);
       s.sel_e[p] = (short)pick;
       s.sel_w[p] = w;
+      atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[pick]), 1ull << t);
       if (blockIdx.x == 0) {
         if (a.ids != nullptr) a.ids[p] = pick;
         if (a.weights != nullptr) a.weights[p] = w;
@@ -156,43 +215,64 @@ __device__ void few_route(const MoeFewArgs& a, Shared& s) {
     }
   }
   __syncthreads();
-  const int pairs = a.T * a.topk;
-  for (int p = threadIdx.x; p < pairs; p += kThreads)
-    atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[s.sel_e[p]]), 1ull << (p / a.topk));
-  __syncthreads();
-  if (warp == 0) {
-    int at = 0, nt = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 32) {
-      const int e = e0 + lane;
-      const int c = e < a.E ? __popcll(s.mask[e]) : 0;
-      int incl = c;
+  // first pair of every expert and the list of touched ones: a thread per expert
+  const int e = threadIdx.x;
+  int c = 0, incl = 0;
+  unsigned has = 0;
+  if (e < kFewMaxExperts) {
+    c = __popcll(s.mask[e]);
+    incl = c;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      if (e < a.E) s.start[e] = at + incl - c;
-      const unsigned has = __ballot_sync(0xffffffffu, c > 0);
-      if (c > 0) s.touched[nt + __popc(has & ((1u << lane) - 1))] = e;
-      nt += __popc(has);
-      at += __shfl_sync(0xffffffffu, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
     }
-    if (lane == 0) { s.start[a.E] = at; s.n_touched = nt; }
+    has = __ballot_sync(0xffffffffu, c > 0);
+    if (lane == 31) s.warp_sums[warp] = make_int2(incl, __popc(has));
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += kThreads) {
-    const int e = s.sel_e[p], t = p / a.topk;
-    s.pair[s.start[e] + __popcll(s.mask[e] & ((1ull << t) - 1))] = (short)p;
+  if (e < kFewMaxExperts) {
+    int at = 0, nt = 0;
+#pragma unroll
+    for (int i = 0; i < kFewMaxExperts / 32; ++i) {
+      const int2 x = s.warp_sums[i];
+      if (i < warp) { at += x.x; nt += x.y; }
+    }
+    s.start[e] = at + incl - c;
+    if (c > 0) s.touched[nt + __popc(has & ((1u << lane) - 1))] = e;
+    if (e == kFewMaxExperts - 1) {
+      s.n_touched = nt + __popc(has);
+      s.start[kFewMaxExperts] = a.T * a.topk;
+    }
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.T * a.topk; p += kThreads) {
+    const int x = s.sel_e[p], t = p / a.topk;
+    s.pair[s.start[x] + __popcll(s.mask[x] & ((1ull << t) - 1))] = (short)p;
   }
   __syncthreads();
 }
 
-constexpr int kRing = kWarps * kStages * kStageBytes;
+constexpr int kRing = kWarps * kRingBytes;
 constexpr int kRed = kRing;                                  // [kWarps][8][32] floats
-constexpr int kBars = kRed + kWarps * 8 * 32 * 4;            // [kWarps][kStages]
-constexpr int kShared = kBars + kWarps * kStages * 8 + 64;   // Shared
-constexpr int kSmem = kShared + (int)sizeof(Shared) + 1024;
+constexpr int kShared = kRed + kWarps * 8 * 32 * 4;          // Shared
+constexpr int kSmem = kShared + (int)sizeof(Shared);
 static_assert(kSmem <= 232448, "shared memory budget");
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 16 or 4 bytes, zeros where there is nothing to copy
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_or_zero(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest N groups have landed
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -201,15 +281,20 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two e4m3 -> two bf16, exactly (every e4m3 value is a bf16 value; NaN stays NaN).
-__device__ __forceinline__ uint32_t bf16x2_of(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
-  return *reinterpret_cast<const uint32_t*>(&b);
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One pass of a team over 32 weight rows of an expert for up to 16 of its tokens.
+// Two e4m3 -> two f16, exactly (NaN stays NaN).
+__device__ __forceinline__ uint32_t f16x2_of(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One pass of a team over 32 weight rows of an expert for up to kCols of its tokens.
 struct Item {
   int e, block;        // expert; block of 16 hidden units (phase 0) or of 32 outputs (phase 1)
   int first, cnt;      // pairs [first, first + cnt) of the expert-ordered list
@@ -217,27 +302,26 @@ struct Item {
 
 template <bool FP8>
 struct Few {
-  static constexpr int KPS = FP8 ? 2 : 1;              // runs of 64 K per stage
-  static constexpr int BLOCK = FP8 ? 1024 : 2048;      // 16 rows of one run
+  static constexpr int PER = FP8 ? 1 : 2;              // 16-byte pieces of a lane's 16 weights
+  // A stage of the ring holds a run of 64 K: weights [4 * PER][32 lanes] x 16 bytes, tokens [2 or 4][32] x 16
+  // bytes and, for e4m3, the hidden values' factors [32] and the two block scales.
+  static constexpr int W = 2048 * PER, B = FP8 ? 1024 : 2048;
+  static constexpr int kStageBytes = FP8 ? W + B + 128 : W + B;
+  static constexpr int kStages = FP8 ? 4 : 2;
+  static_assert(kStages * (kStageBytes + (FP8 ? 16 : 0)) <= kRingBytes, "ring");
   const MoeFewArgs& a;
-  const CUtensorMap& m13;
-  const CUtensorMap& m2;
   Shared& s;
-  uint8_t* ring;                   // this warp's stages
-  uint64_t* bars;
-  volatile int* abort_flag;
+  uint8_t* ring;
   int lane, part, team, teams;     // part: quarter of K; team: over the grid
 
   // ------------------------------------------------------------ the stream of items
   // Items of phase 0 (gate and up rows) and phase 1 (rows of Wd); each is a run of passes.
   __device__ __forceinline__ int blocks(int phase) const { return phase ? a.H / 32 : a.I / 16; }
-  __device__ __forceinline__ int k_runs(int phase) const { return (phase ? a.I : a.H) / 64; }
-  __device__ __forceinline__ int run0(int phase) const { return k_runs(phase) * part / kTeam; }
-  __device__ __forceinline__ int run1(int phase) const { return k_runs(phase) * (part + 1) / kTeam; }
-  __device__ __forceinline__ int stages(int phase) const { return (run1(phase) - run0(phase) + KPS - 1) / KPS; }
+  __device__ __forceinline__ int run0(int phase) const { return (phase ? a.I : a.H) / 64 * part / kTeam; }
+  __device__ __forceinline__ int run1(int phase) const { return (phase ? a.I : a.H) / 64 * (part + 1) / kTeam; }
 
   struct Cursor {
-    int phase, i, pass, st;        // item of the phase, pass of 16 tokens, stage; phase 2: over
+    int phase, i, pass, st;        // item of the phase, pass of kCols tokens, run; phase 2: over
   };
   __device__ __forceinline__ Item item(const Cursor& c) const {
     Item it;
@@ -250,13 +334,9 @@ struct Few {
       x = c.i - it.block * s.n_touched;
     }
     it.e = s.touched[x];
-    it.first = s.start[it.e] + c.pass * 16;
-    it.cnt = min(16, s.start[it.e + 1] - it.first);
+    it.first = s.start[it.e] + c.pass * kCols;
+    it.cnt = s.start[it.e + 1] - it.first;             // of this pass and those behind it
     return it;
-  }
-  __device__ __forceinline__ int passes(const Cursor& c) const {
-    const int e = s.touched[c.phase == 0 ? c.i / blocks(0) : c.i % s.n_touched];
-    return (s.start[e + 1] - s.start[e] + 15) / 16;
   }
   __device__ __forceinline__ bool settle(Cursor& c) const {   // to the first item at or behind c.i; false: over
     while (c.phase < 2 && c.i >= s.n_touched * blocks(c.phase)) {
@@ -265,245 +345,294 @@ struct Few {
     }
     return c.phase < 2;
   }
-  // next stage of this warp in stream order (items in which it has no K are passed over)
-  __device__ __forceinline__ bool to_stage(Cursor& c) const {
-    while (settle(c)) {
-      if (c.st < stages(c.phase)) return true;
-      c.st = 0;
-      if (++c.pass >= passes(c)) { c.pass = 0; c.i += teams; }
+
+  // The pass whose runs are being brought in, resolved once.
+  struct Ahead {
+    Cursor c;
+    int left, runs;                // tokens of this pass and behind it; this warp's runs of 64 K
+    const uint8_t* p0;             // this lane's weights of rows g of the two row blocks
+    const uint8_t* p1;
+    int row8, run;                 // bytes from row g to row g + 8, and to the next run
+    const uint16_t* tok;           // this lane's token or hidden row; null: none
+    const float* fac;              // its factors
+    const float* sc;               // lanes 0 and 1: block scales of a row block
+    int k0;
+    bool more;
+  };
+  __device__ __forceinline__ void resolve(Ahead& h) const {
+    for (;;) {
+      h.more = settle(h.c);
+      if (!h.more) return;
+      h.k0 = run0(h.c.phase);
+      h.runs = run1(h.c.phase) - h.k0;
+      if (h.runs > 0) break;
+      h.c.i += teams;              // no K for this warp in this phase
     }
-    return false;
+    const Item it = item(h.c);
+    h.left = it.cnt;
+    const int N = h.c.phase ? a.H : 2 * a.I, K = h.c.phase ? a.I : a.H;
+    const int row0 = h.c.phase ? it.block * 32 : it.block * 16, row1 = h.c.phase ? row0 + 16 : a.I + row0;
+    const int g = lane >> 2, t = lane & 3;
+    const uint8_t* w = static_cast<const uint8_t*>(h.c.phase ? a.w2 : a.w13) + (int64_t)it.e * N * K * (FP8 ? 1 : 2);
+    if (FP8 && a.tiled) {
+      // [row / 128][K / 64][128][64]; 16-byte chunk u of a row at u ^ ((row >> 1) & 3)
+      w += (int64_t)h.k0 * 8192 + g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
+      h.p0 = w + (int64_t)(row0 >> 7) * K * 128 + (row0 & 127) * 64;
+      h.p1 = w + (int64_t)(row1 >> 7) * K * 128 + (row1 & 127) * 64;
+      h.row8 = 512;
+      h.run = 8192;
+    } else {
+      const int row = K * (FP8 ? 1 : 2);
+      h.run = FP8 ? 64 : 128;
+      w += (int64_t)h.k0 * h.run + t * 16;
+      h.p0 = w + (int64_t)(row0 + g) * row;
+      h.p1 = w + (int64_t)(row1 + g) * row;
+      h.row8 = 8 * row;
+    }
+    h.tok = nullptr;
+    if (g < it.cnt) {
+      const int p = s.pair[it.first + g];
+      if (h.c.phase == 0) h.tok = static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + (int64_t)(p / a.topk) * a.H;
+      else h.tok = static_cast<const uint16_t*>(a.h) + (int64_t)p * a.I;
+      h.tok += h.k0 * 64 + t * (FP8 ? 16 : 8);
+      h.fac = a.h_factor + (int64_t)p * (a.I / 16) + h.k0 * 4 + t;
+    }
+    if (FP8)
+      h.sc = (h.c.phase ? a.s2 : a.s13) + ((int64_t)it.e * (N >> 7) + ((lane == 0 ? row0 : row1) >> 7)) * (K >> 7);
+    h.c.st = 0;
+  }
+  __device__ __forceinline__ void copy_weights(const Ahead& h, int slot) const {
+    const uint32_t dst = smem_u32(ring + slot * kStageBytes + lane * 16);
+    const uint8_t* q0 = h.p0 + (int64_t)h.c.st * h.run;
+    const uint8_t* q1 = h.p1 + (int64_t)h.c.st * h.run;
+#pragma unroll
+    for (int v = 0; v < PER; ++v) {
+      copy16(dst + (0 * PER + v) * 512, q0 + v * 64);
+      copy16(dst + (1 * PER + v) * 512, q0 + h.row8 + v * 64);
+      copy16(dst + (2 * PER + v) * 512, q1 + v * 64);
+      copy16(dst + (3 * PER + v) * 512, q1 + h.row8 + v * 64);
+    }
+    if (FP8 && lane < 2)
+      copy4_or_zero(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.c.st) >> 1), true);
+  }
+  __device__ __forceinline__ void copy_tokens(const Ahead& h, int slot, int64_t plane) const {
+    const uint32_t dst = smem_u32(ring + slot * kStageBytes + W + lane * 16);
+    const bool have = h.tok != nullptr;
+    const uint16_t* src = have ? h.tok + h.c.st * 64 : static_cast<const uint16_t*>(a.x);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      copy16_or_zero(dst + v * 512, src + v * (FP8 ? 8 : 32), have);
+      if (!FP8 && h.c.phase == 1) copy16_or_zero(dst + (2 + v) * 512, src + (have ? plane : 0) + v * 32, have);
+    }
+    if (FP8 && h.c.phase == 1)
+      copy4_or_zero(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), have ? h.fac + h.c.st * 4 : a.s2, have);
+  }
+  __device__ __forceinline__ void step(Ahead& h) const {
+    if (++h.c.st < h.runs) return;
+    h.c.st = 0;
+    if (h.left > kCols) {
+      ++h.c.pass;
+    } else {
+      h.c.pass = 0;
+      h.c.i += teams;
+    }
+    resolve(h);
   }
 
-  // the copies of one stage (one lane)
-  __device__ __forceinline__ void issue(const Cursor& c, int slot) const {
-    const Item it = item(c);
-    const int k0 = run0(c.phase) + c.st * KPS, n = min(KPS, run1(c.phase) - k0);
-    uint8_t* dst = ring + slot * kStageBytes;
-    uint64_t* bar = &bars[slot];
-    mbar_arrive_expect_tx(bar, n * 2 * BLOCK);
-    const int N = c.phase ? a.H : 2 * a.I, K = c.phase ? a.I : a.H;
-    const int row0 = c.phase ? it.block * 32 : it.block * 16, row1 = c.phase ? row0 + 16 : a.I + row0;
-    for (int k = 0; k < n; ++k) {
+  // acc[m] += 16 weight rows x 8 tokens of one run of 64 K
+  template <int P>
+  __device__ __forceinline__ void multiply(int slot, float (&acc)[2][4]) const {
+    constexpr int PLANES = !FP8 && P == 1 ? 2 : 1;
+    const int t = lane & 3;
+    const uint8_t* src = ring + slot * kStageBytes + lane * 16;
+    uint4 b[PLANES][2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int row = b ? row1 : row0;
-        uint8_t* d = dst + (k * 2 + b) * BLOCK;
-        if (FP8 && a.tiled) {
-          const uint8_t* w = static_cast<const uint8_t*>(c.phase ? a.w2 : a.w13);
-          bulk_load(d, w + (((int64_t)it.e * (N >> 7) + (row >> 7)) * (K >> 6) + k0 + k) * 8192 + (row & 127) * 64, BLOCK, bar);
-        } else {
-          tma_load_2d(d, c.phase ? &m2 : &m13, bar, (k0 + k) * 64, it.e * N + row);
+    for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) b[p][v] = *reinterpret_cast<const uint4*>(src + W + (p * 2 + v) * 512);
+    float sc[2][2] = {{1.f, 1.f}, {1.f, 1.f}};   // factors of the sums: [row block][column of this lane]
+    if constexpr (FP8) {
+      const float2 bs = *reinterpret_cast<const float2*>(ring + kStages * kStageBytes + slot * 16);
+      sc[0][0] = sc[0][1] = bs.x;
+      sc[1][0] = sc[1][1] = bs.y;
+      if constexpr (P == 1) {
+        // Each lane of a token holds 16 hidden values with a factor of their own: bring the four to
+        // the largest (a value that vanishes there is below 2^-24 of the others' largest).
+        const float f = *reinterpret_cast<const float*>(ring + slot * kStageBytes + W + B + lane * 4);
+        float m = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int d = (int)(__float_as_uint(f) >> 23) - (int)(__float_as_uint(m) >> 23);   // <= 0
+        const __half2 r = __float2half2_rn(d < -30 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23));
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          __half2* x = reinterpret_cast<__half2*>(&b[0][v]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], r);
+        }
+        const float top0 = __shfl_sync(0xffffffffu, m, t * 8), top1 = __shfl_sync(0xffffffffu, m, t * 8 + 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          sc[i][0] *= top0;
+          sc[i][1] *= top1;
         }
       }
     }
-  }
-
-  // ------------------------------------------------------------ products
-  // acc[m][n] += 16 rows x 8 tokens of this warp's K; B: bf16 rows of K elements, `planes` of them
-  // (value and rest) `plane` elements apart.
-  template <int NT, int PLANES, typename Load>
-  __device__ __forceinline__ void stage_mma(const Cursor& c, const Item& it, int slot, uint32_t parity, float (&acc)[2][NT][4],
-                                            const bf16* const (&rows)[NT], int64_t plane, Load load) {
-    const int k0 = run0(c.phase) + c.st * KPS, n = min(KPS, run1(c.phase) - k0);
-    const int g = lane >> 2, t = lane & 3;
-    uint4 b[KPS][NT][PLANES][2];
 #pragma unroll
-    for (int k = 0; k < KPS; ++k)
+    for (int m = 0; m < 2; ++m) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint4 w[2][PER];               // rows g and g + 8: 16 weights
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p)
+        for (int v = 0; v < PER; ++v) w[r][v] = *reinterpret_cast<const uint4*>(src + ((m * 2 + r) * PER + v) * 512);
 #pragma unroll
-          for (int v = 0; v < 2; ++v)
-            b[k][j][p][v] = k < n && rows[j] != nullptr ? load(rows[j] + p * plane + (k0 + k) * 64 + t * 16 + v * 8)
-                                                        : make_uint4(0, 0, 0, 0);
-    float sc[KPS][2];
-    if constexpr (FP8) {
-      const int N = c.phase ? a.H : 2 * a.I, kb = (c.phase ? a.I : a.H) / 128;
-      const int row0 = c.phase ? it.block * 32 : it.block * 16, row1 = c.phase ? row0 + 16 : a.I + row0;
-      const float* sp = (c.phase ? a.s2 : a.s13) + (int64_t)it.e * (N / 128) * kb;
-#pragma unroll
-      for (int k = 0; k < KPS; ++k) {
-        const int at = min(k0 + k, k_runs(c.phase) - 1) >> 1;
-        sc[k][0] = __ldg(sp + (row0 >> 7) * kb + at);
-        sc[k][1] = __ldg(sp + (row1 >> 7) * kb + at);
-      }
-    }
-    mbar_wait(&bars[slot], parity, a.status, kStatusTimeoutFull, abort_flag);
-    const uint8_t* src = ring + slot * kStageBytes;
-#pragma unroll
-    for (int k = 0; k < KPS; ++k) {
-      if (k >= n) break;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const uint8_t* blk = src + (k * 2 + m) * BLOCK;
-        float part_acc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part_acc[j][i] = 0.f;
-        uint4 w[2][FP8 ? 1 : 2];     // rows g and g + 8: 16 weights
+      for (int q = 0; q < 4; ++q) {   // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
+        uint32_t af[4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int row = g + 8 * r;
           if constexpr (FP8) {
-            w[r][0] = *reinterpret_cast<const uint4*>(blk + row * 64 + ((t ^ ((row >> 1) & 3)) << 4));
+            const uint4& y = w[r][0];
+            const uint32_t x = q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w;
+            af[r] = f16x2_of(x & 0xffffu);
+            af[r + 2] = f16x2_of(x >> 16);
           } else {
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-              w[r][v] = *reinterpret_cast<const uint4*>(blk + row * 128 + (((2 * t + v) ^ (row & 7)) << 4));
+            const uint4& x = w[r][q >> 1];
+            af[r] = q & 1 ? x.z : x.x;
+            af[r + 2] = q & 1 ? x.w : x.y;
           }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {   // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
-          uint32_t af[4];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if constexpr (FP8) {
-              const uint32_t x = q == 0 ? w[r][0].x : q == 1 ? w[r][0].y : q == 2 ? w[r][0].z : w[r][0].w;
-              af[r] = bf16x2_of(x & 0xffffu);
-              af[r + 2] = bf16x2_of(x >> 16);
-            } else {
-              const uint4& x = w[r][q >> 1];
-              af[r] = q & 1 ? x.z : x.x;
-              af[r + 2] = q & 1 ? x.w : x.y;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int p = 0; p < PLANES; ++p) {
-              const uint4& x = b[k][j][p][q >> 1];
-              mma_bf16(part_acc[j], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
-            }
+        for (int p = 0; p < PLANES; ++p) {
+          const uint4& x = b[p][q >> 1];
+          if constexpr (FP8) mma_f16(sum, af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
+          else mma_bf16(sum, af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
         }
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (FP8) acc[m][j][i] = fmaf(part_acc[j][i], sc[k][m], acc[m][j][i]);
-            else acc[m][j][i] += part_acc[j][i];
-          }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][i] = FP8 ? fmaf(sum[i], sc[m][i & 1], acc[m][i]) : acc[m][i] + sum[i];
     }
   }
 };
 
 template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
-moe_few_kernel(const __grid_constant__ CUtensorMap m13, const __grid_constant__ CUtensorMap m2, const MoeFewArgs a) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+moe_few_kernel(const MoeFewArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int last_s[kTeams];
   Shared& s = *reinterpret_cast<Shared*>(smem + kShared);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kBars + kWarps * kStages * 8);
-  int* last_s = reinterpret_cast<int*>(smem + kBars + kWarps * kStages * 8 + 4);   // [kTeams]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int team_in = warp / kTeam, tt = threadIdx.x % (kTeam * 32);
   cg::grid_group grid = cg::this_grid();
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBars) + warp * kStages;
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
-    if (warp == 0) *abort_flag = 0;
-    fence_barrier_init();
-  }
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.H / 32; i += kThreads) a.done[i] = 0;
-  few_logits(a);
+  few_logits(a, reinterpret_cast<double*>(smem + kRed));
+  if (FP8) few_rows(a, reinterpret_cast<float*>(smem + kRed));
   grid.sync();
-  few_route(a, s);
+  if (a.E <= 128) few_route<4>(a, s);
+  else few_route<kFewMaxExperts / 32>(a, s);
 
-  Few<FP8> few{a, m13, m2, s, smem + warp * kStages * kStageBytes, bars, abort_flag, lane, warp % kTeam,
+  Few<FP8> few{a, s, smem + warp * kRingBytes, lane, warp % kTeam,
                team_in * (int)gridDim.x + (int)blockIdx.x, kTeams * (int)gridDim.x};
   using Cursor = typename Few<FP8>::Cursor;
-  Cursor ahead{0, few.team, 0, 0}, at{0, few.team, 0, 0};
-  int issued = 0, used = 0;
-  auto refill = [&]() {   // keep the ring full, across items and phases
-    while (issued < used + kStages && few.to_stage(ahead)) {
-      if (lane == 0 && !*abort_flag) few.issue(ahead, issued % kStages);
-      ++issued;
-      ++ahead.st;
-    }
-  };
-  refill();
-
+  using Ahead = typename Few<FP8>::Ahead;
+  constexpr int kStages = Few<FP8>::kStages;
   float* red = reinterpret_cast<float*>(smem + kRed) + team_in * (kTeam * 256);   // [kTeam][8][32]
-  bf16* hid = static_cast<bf16*>(a.h);
+  uint16_t* hid = static_cast<uint16_t*>(a.h);
   const int64_t hplane = (int64_t)a.T * a.topk * a.I;
-  const int g = lane >> 2;
+
+  Cursor at{0, few.team, 0, 0};
+  Ahead ahead{};
+  ahead.c = at;
+  few.resolve(ahead);
+  int slot = 0;                    // the ring's next stage
+  int early = 0;                   // stages of phase 1 brought in without their tokens, in front of the barrier
+  bool hidden_done = false;
+  auto issue = [&](int to) {       // the next run into the ring; an empty group behind the last one
+    if (ahead.more) {
+      few.copy_weights(ahead, to);
+      if (ahead.c.phase == 0 || hidden_done) few.copy_tokens(ahead, to, hplane);
+      else ++early;
+      few.step(ahead);
+    }
+    copies_commit();
+  };
+  for (int i = 0; i < kStages; ++i) issue(i);
 
   auto run_phase = [&](auto phase_c) {
     constexpr int P = decltype(phase_c)::value;
+    if (P == 1) {
+      // the tokens of the stages that came in early
+      hidden_done = true;
+      Ahead late{};
+      late.c = Cursor{1, few.team, 0, 0};
+      if (early > 0) few.resolve(late);
+      for (int i = 0; i < early; ++i) {
+        few.copy_tokens(late, (slot + i) % kStages, hplane);
+        few.step(late);
+      }
+      copies_commit();
+      copies_wait<0>();
+    }
     while (few.settle(at) && at.phase == P) {
-      const Item it = few.item(at);
-      auto pass = [&](auto nt_c) {
-        constexpr int NT = decltype(nt_c)::value;
-        float acc[2][NT][4];
-        const bf16* rows[NT];
+      Item it = few.item(at);
+      const bool over = it.cnt <= kCols;         // the item's last pass
+      it.cnt = min(it.cnt, kCols);
+      float acc[2][4] = {};
+      const int runs = few.run1(P) - few.run0(P);
+#pragma unroll 1
+      for (int k = 0; k < runs; ++k) {
+        copies_wait<kStages - 1>();
+        __syncwarp();                            // the scales come in through two lanes
+        few.template multiply<P>(slot, acc);
+        __syncwarp();
+        issue(slot);
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+      }
+      // the quarters of K, added in order
+      named_barrier_sync(1 + team_in, kTeam * 32);    // the last sums have been read
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+        for (int i = 0; i < 4; ++i) red[(warp % kTeam) * 256 + (m * 4 + i) * 32 + lane] = acc[m][i];
+      named_barrier_sync(1 + team_in, kTeam * 32);
+      // thread = (token, row): the 16 rows of a token side by side
+      const int n = tt >> 4, row = tt & 15;
+      const int ri = (row >> 3) * 2 + (n & 1), rl = (row & 7) * 4 + (n >> 1);
+      float v[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-          const int n = j * 8 + g;
-          rows[j] = nullptr;
-          if (n < it.cnt) {
-            const int p = s.pair[it.first + n];
-            rows[j] = P ? hid + (int64_t)p * a.I : static_cast<const bf16*>(a.x) + (int64_t)(p / a.topk) * a.H;
-          }
+      for (int m = 0; m < 2; ++m) {
+        v[m] = 0.f;
+#pragma unroll
+        for (int q = 0; q < kTeam; ++q) v[m] += red[q * 256 + (m * 4 + ri) * 32 + rl];
+      }
+      const int p = n < it.cnt ? s.pair[it.first + n] : -1;
+      if constexpr (P == 0) {
+        if (FP8 && p >= 0) {
+          const float f = a.x_factor[p / a.topk];
+          v[0] *= f;
+          v[1] *= f;
         }
-        for (at.st = 0; at.st < few.stages(P); ++at.st) {
-          const int slot = used % kStages;
-          const uint32_t parity = (used / kStages) & 1;
-          if constexpr (P == 0)
-            few.template stage_mma<NT, 1>(at, it, slot, parity, acc, rows, 0,
-                                          [](const bf16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); });
-          else
-            few.template stage_mma<NT, 2>(at, it, slot, parity, acc, rows, hplane,
-                                          [](const bf16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); });
-          __syncwarp();
-          ++used;
-          refill();
-        }
-        at.st = 0;
-        // the quarters of K, added in order: thread = (accumulator register, lane)
+        const float hv = v[0] / (1.f + expf(-v[0])) * v[1];
+        if constexpr (FP8) {
+          uint32_t top = __float_as_uint(hv) & 0x7fffffffu;   // NaN and infinity are above every number
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          named_barrier_sync(1 + team_in, kTeam * 32);    // the last sums have been read
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[(warp % kTeam) * 256 + (m * 4 + i) * 32 + lane] = acc[m][j][i];
-          named_barrier_sync(1 + team_in, kTeam * 32);
-          const int i = tt >> 5, l = tt & 31;
-          float v[2];
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            v[m] = 0.f;
-#pragma unroll
-            for (int q = 0; q < kTeam; ++q) v[m] += red[q * 256 + (m * 4 + i) * 32 + l];
+          for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float f = factor_of(__uint_as_float(top));
+          if (p >= 0) {
+            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + it.block * 16 + row] = __float2half_rn(hv * (1.f / f));
+            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + it.block] = f;
           }
-          const int n = j * 8 + (l & 3) * 2 + (i & 1), row = (l >> 2) + 8 * (i >> 1);
-          if (n < it.cnt) {
-            const int64_t p = s.pair[it.first + n];
-            if constexpr (P == 0) {
-              const float hv = v[0] / (1.f + expf(-v[0])) * v[1];
-              const bf16 top = __float2bfloat16(hv);
-              bf16* dst = hid + p * a.I + it.block * 16 + row;
-              dst[0] = top;
-              dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
-            } else {
-              float* dst = a.slots + p * a.H + it.block * 32 + row;
-              dst[0] = v[0];
-              dst[16] = v[1];
-            }
-          }
+        } else if (p >= 0) {
+          const bf16 top = __float2bfloat16(hv);
+          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + it.block * 16 + row;
+          dst[0] = top;
+          dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
         }
-      };
-      if (it.cnt <= 8) pass(std::integral_constant<int, 1>{});
-      else pass(std::integral_constant<int, 2>{});
-      const bool over = at.pass + 1 >= few.passes(at);
+      } else if (p >= 0) {
+        float* dst = a.slots + (int64_t)p * a.H + it.block * 32 + row;
+        dst[0] = v[0];
+        dst[16] = v[1];
+      }
       if constexpr (P == 1) {
         if (over) {
           // the team that brings a block's last expert adds the slots of every token
@@ -544,48 +673,13 @@ moe_few_kernel(const __grid_constant__ CUtensorMap m13, const __grid_constant__ 
   run_phase(std::integral_constant<int, 0>{});
   grid.sync();
   run_phase(std::integral_constant<int, 1>{});
-  if (*abort_flag) {
-    // a wait gave up: let the copies already issued land before the CTA exits
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
-  }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    cudaDriverEntryPointQueryResult q;
-    void* p = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || p == nullptr)
-      throw std::runtime_error("cuTensorMapEncodeTiled entry point not available");
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }();
-  return fn;
-}
-
-// Row-major weights [rows, K]: boxes of 64 K x 16 rows, in the swizzle the lanes read without
-// bank conflicts (64-byte rows for e4m3, 128-byte rows for bf16).
-void weight_map(CUtensorMap* map, const void* w, bool fp8, int64_t rows, int K) {
-  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)K * (fp8 ? 1 : 2)};
-  const cuuint32_t box[2] = {64, 16}, estr[2] = {1, 1};
-  const CUresult r = encode_fn()(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                 const_cast<void*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 fp8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) throw std::runtime_error("moe_few weight map: encode failed " + std::to_string((int)r));
 }
 
 template <bool FP8>
 void launch(const MoeFewArgs& a, cudaStream_t s) {
   MoeFewArgs args = a;
-  CUtensorMap m13{}, m2{};
-  if (!(FP8 && a.tiled)) {
-    weight_map(&m13, a.w13, FP8, (int64_t)a.E * 2 * a.I, a.H);
-    weight_map(&m2, a.w2, FP8, (int64_t)a.E * a.H, a.I);
-  }
   smem_opt_in(moe_few_kernel<FP8>, kSmem);
-  void* params[] = {&m13, &m2, &args};
+  void* params[] = {&args};
   // every CTA waits for the others: a cooperative launch places all of them at once or fails
   const cudaError_t e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(moe_few_kernel<FP8>),
                                                     dim3(device_sm_count()), dim3(kThreads), params, kSmem, s);
