@@ -294,12 +294,6 @@ __device__ __forceinline__ uint32_t f16x2_of(uint32_t two) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One pass of a team over 32 weight rows of an expert for up to kCols of its tokens.
-struct Item {
-  int e, block;        // expert; block of 16 hidden units (phase 0) or of 32 outputs (phase 1)
-  int first, cnt;      // pairs [first, first + cnt) of the expert-ordered list
-};
-
 template <bool FP8>
 struct Few {
   static constexpr int PER = FP8 ? 1 : 2;              // 16-byte pieces of a lane's 16 weights
@@ -315,41 +309,43 @@ struct Few {
   int lane, part, team, teams;     // part: quarter of K; team: over the grid
 
   // ------------------------------------------------------------ the stream of items
-  // Items of phase 0 (gate and up rows) and phase 1 (rows of Wd); each is a run of passes.
+  // Items of phase 0 (gate and up rows; an expert's blocks together) and of phase 1 (rows of Wd; a
+  // block's experts together, so that its sum is over early).  A team takes the team-th of equal
+  // runs of either order, and an item is as many passes as its tokens need.
   __device__ __forceinline__ int blocks(int phase) const { return phase ? a.H / 32 : a.I / 16; }
   __device__ __forceinline__ int run0(int phase) const { return (phase ? a.I : a.H) / 64 * part / kTeam; }
   __device__ __forceinline__ int run1(int phase) const { return (phase ? a.I : a.H) / 64 * (part + 1) / kTeam; }
 
   struct Cursor {
-    int phase, i, pass, st;        // item of the phase, pass of kCols tokens, run; phase 2: over
+    int phase, left;               // phase 2: over; items left in the phase, this one among them
+    int x, block, pass;            // touched expert, block, pass of kCols tokens
   };
-  __device__ __forceinline__ Item item(const Cursor& c) const {
-    Item it;
-    int x;
-    if (c.phase == 0) {            // an expert's blocks side by side on different SMs
-      x = c.i / blocks(0);
-      it.block = c.i - x * blocks(0);
-    } else {                       // a block's experts together, so its sum is over early
-      it.block = c.i / s.n_touched;
-      x = c.i - it.block * s.n_touched;
-    }
-    it.e = s.touched[x];
-    it.first = s.start[it.e] + c.pass * kCols;
-    it.cnt = s.start[it.e + 1] - it.first;             // of this pass and those behind it
-    return it;
+  __device__ __forceinline__ Cursor begin(int phase) const {
+    Cursor c;
+    c.phase = phase;
+    const int n = s.n_touched * blocks(phase), lo = n / teams * team + min(team, n % teams);
+    c.left = n / teams + (team < n % teams ? 1 : 0);
+    const int inner = phase ? s.n_touched : blocks(0), o = lo / inner;
+    c.x = phase ? lo - o * inner : o;
+    c.block = phase ? o : lo - o * inner;
+    c.pass = 0;
+    return c;
   }
-  __device__ __forceinline__ bool settle(Cursor& c) const {   // to the first item at or behind c.i; false: over
-    while (c.phase < 2 && c.i >= s.n_touched * blocks(c.phase)) {
-      ++c.phase;
-      c.i = team;
+  __device__ __forceinline__ int expert(const Cursor& c) const { return s.touched[c.x]; }
+  __device__ __forceinline__ void next(Cursor& c) const {      // behind the item's last pass
+    c.pass = 0;
+    if (--c.left == 0) return;
+    if (c.phase == 0) {
+      if (++c.block == blocks(0)) { c.block = 0; ++c.x; }
+    } else {
+      if (++c.x == s.n_touched) { c.x = 0; ++c.block; }
     }
-    return c.phase < 2;
   }
 
   // The pass whose runs are being brought in, resolved once.
   struct Ahead {
     Cursor c;
-    int left, runs;                // tokens of this pass and behind it; this warp's runs of 64 K
+    int st, runs, tokens;          // run of 64 K, runs of this warp; tokens of this pass and behind it
     const uint8_t* p0;             // this lane's weights of rows g of the two row blocks
     const uint8_t* p1;
     int row8, run;                 // bytes from row g to row g + 8, and to the next run
@@ -357,54 +353,55 @@ struct Few {
     const float* fac;              // its factors
     const float* sc;               // lanes 0 and 1: block scales of a row block
     int k0;
-    bool more;
   };
+  __device__ __forceinline__ bool more(const Ahead& h) const { return h.c.phase < 2; }
   __device__ __forceinline__ void resolve(Ahead& h) const {
-    for (;;) {
-      h.more = settle(h.c);
-      if (!h.more) return;
-      h.k0 = run0(h.c.phase);
-      h.runs = run1(h.c.phase) - h.k0;
-      if (h.runs > 0) break;
-      h.c.i += teams;              // no K for this warp in this phase
+    // a phase that is over, or in which this warp has no K, is passed over
+    while (h.c.phase < 2 && (h.c.left <= 0 || run0(h.c.phase) == run1(h.c.phase))) {
+      if (h.c.phase == 1) { h.c.phase = 2; return; }
+      h.c = begin(1);
     }
-    const Item it = item(h.c);
-    h.left = it.cnt;
-    const int N = h.c.phase ? a.H : 2 * a.I, K = h.c.phase ? a.I : a.H;
-    const int row0 = h.c.phase ? it.block * 32 : it.block * 16, row1 = h.c.phase ? row0 + 16 : a.I + row0;
+    if (h.c.phase == 2) return;
+    const int ph = h.c.phase, e = expert(h.c), first = s.start[e] + h.c.pass * kCols;
+    h.tokens = s.start[e + 1] - first;
+    h.st = 0;
+    h.k0 = run0(ph);
+    h.runs = run1(ph) - h.k0;
+    const int N = ph ? a.H : 2 * a.I, K = ph ? a.I : a.H;
+    const int row0 = ph ? h.c.block * 32 : h.c.block * 16, row1 = ph ? row0 + 16 : a.I + row0;
     const int g = lane >> 2, t = lane & 3;
-    const uint8_t* w = static_cast<const uint8_t*>(h.c.phase ? a.w2 : a.w13) + (int64_t)it.e * N * K * (FP8 ? 1 : 2);
+    const uint8_t* w = static_cast<const uint8_t*>(ph ? a.w2 : a.w13);
     if (FP8 && a.tiled) {
       // [row / 128][K / 64][128][64]; 16-byte chunk u of a row at u ^ ((row >> 1) & 3)
-      w += (int64_t)h.k0 * 8192 + g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
-      h.p0 = w + (int64_t)(row0 >> 7) * K * 128 + (row0 & 127) * 64;
-      h.p1 = w + (int64_t)(row1 >> 7) * K * 128 + (row1 & 127) * 64;
+      w += g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
+      const uint32_t tiles = K >> 6, r0 = (uint32_t)(e * N + row0), r1 = (uint32_t)(e * N + row1);
+      h.p0 = w + (uint64_t)((r0 >> 7) * tiles + h.k0) * 8192 + (r0 & 127) * 64;
+      h.p1 = w + (uint64_t)((r1 >> 7) * tiles + h.k0) * 8192 + (r1 & 127) * 64;
       h.row8 = 512;
       h.run = 8192;
     } else {
-      const int row = K * (FP8 ? 1 : 2);
+      const uint32_t row = K * (FP8 ? 1 : 2);
       h.run = FP8 ? 64 : 128;
-      w += (int64_t)h.k0 * h.run + t * 16;
-      h.p0 = w + (int64_t)(row0 + g) * row;
-      h.p1 = w + (int64_t)(row1 + g) * row;
+      w += h.k0 * h.run + t * 16;
+      h.p0 = w + (uint64_t)(uint32_t)(e * N + row0 + g) * row;
+      h.p1 = w + (uint64_t)(uint32_t)(e * N + row1 + g) * row;
       h.row8 = 8 * row;
     }
     h.tok = nullptr;
-    if (g < it.cnt) {
-      const int p = s.pair[it.first + g];
-      if (h.c.phase == 0) h.tok = static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + (int64_t)(p / a.topk) * a.H;
-      else h.tok = static_cast<const uint16_t*>(a.h) + (int64_t)p * a.I;
+    if (g < h.tokens) {
+      const int p = s.pair[first + g];
+      if (ph == 0) h.tok = static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + (p / a.topk) * a.H;
+      else h.tok = static_cast<const uint16_t*>(a.h) + p * a.I;
       h.tok += h.k0 * 64 + t * (FP8 ? 16 : 8);
-      h.fac = a.h_factor + (int64_t)p * (a.I / 16) + h.k0 * 4 + t;
+      h.fac = a.h_factor + p * (a.I / 16) + h.k0 * 4 + t;
     }
     if (FP8)
-      h.sc = (h.c.phase ? a.s2 : a.s13) + ((int64_t)it.e * (N >> 7) + ((lane == 0 ? row0 : row1) >> 7)) * (K >> 7);
-    h.c.st = 0;
+      h.sc = (ph ? a.s2 : a.s13) + (uint64_t)((uint32_t)(e * N + (lane == 0 ? row0 : row1)) >> 7) * (K >> 7);
   }
   __device__ __forceinline__ void copy_weights(const Ahead& h, int slot) const {
     const uint32_t dst = smem_u32(ring + slot * kStageBytes + lane * 16);
-    const uint8_t* q0 = h.p0 + (int64_t)h.c.st * h.run;
-    const uint8_t* q1 = h.p1 + (int64_t)h.c.st * h.run;
+    const uint8_t* q0 = h.p0 + (int64_t)h.st * h.run;
+    const uint8_t* q1 = h.p1 + (int64_t)h.st * h.run;
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
       copy16(dst + (0 * PER + v) * 512, q0 + v * 64);
@@ -413,29 +410,24 @@ struct Few {
       copy16(dst + (3 * PER + v) * 512, q1 + h.row8 + v * 64);
     }
     if (FP8 && lane < 2)
-      copy4_or_zero(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.c.st) >> 1), true);
+      copy4_or_zero(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.st) >> 1), true);
   }
   __device__ __forceinline__ void copy_tokens(const Ahead& h, int slot, int64_t plane) const {
     const uint32_t dst = smem_u32(ring + slot * kStageBytes + W + lane * 16);
     const bool have = h.tok != nullptr;
-    const uint16_t* src = have ? h.tok + h.c.st * 64 : static_cast<const uint16_t*>(a.x);
+    const uint16_t* src = have ? h.tok + h.st * 64 : static_cast<const uint16_t*>(a.x);
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       copy16_or_zero(dst + v * 512, src + v * (FP8 ? 8 : 32), have);
       if (!FP8 && h.c.phase == 1) copy16_or_zero(dst + (2 + v) * 512, src + (have ? plane : 0) + v * 32, have);
     }
     if (FP8 && h.c.phase == 1)
-      copy4_or_zero(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), have ? h.fac + h.c.st * 4 : a.s2, have);
+      copy4_or_zero(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), have ? h.fac + h.st * 4 : a.s2, have);
   }
   __device__ __forceinline__ void step(Ahead& h) const {
-    if (++h.c.st < h.runs) return;
-    h.c.st = 0;
-    if (h.left > kCols) {
-      ++h.c.pass;
-    } else {
-      h.c.pass = 0;
-      h.c.i += teams;
-    }
+    if (++h.st < h.runs) return;
+    if (h.tokens > kCols) ++h.c.pass;
+    else next(h.c);
     resolve(h);
   }
 
@@ -540,15 +532,14 @@ moe_few_kernel(const MoeFewArgs a) {
   uint16_t* hid = static_cast<uint16_t*>(a.h);
   const int64_t hplane = (int64_t)a.T * a.topk * a.I;
 
-  Cursor at{0, few.team, 0, 0};
   Ahead ahead{};
-  ahead.c = at;
+  ahead.c = few.begin(0);
   few.resolve(ahead);
   int slot = 0;                    // the ring's next stage
   int early = 0;                   // stages of phase 1 brought in without their tokens, in front of the barrier
   bool hidden_done = false;
   auto issue = [&](int to) {       // the next run into the ring; an empty group behind the last one
-    if (ahead.more) {
+    if (few.more(ahead)) {
       few.copy_weights(ahead, to);
       if (ahead.c.phase == 0 || hidden_done) few.copy_tokens(ahead, to, hplane);
       else ++early;
@@ -564,7 +555,7 @@ moe_few_kernel(const MoeFewArgs a) {
       // the tokens of the stages that came in early
       hidden_done = true;
       Ahead late{};
-      late.c = Cursor{1, few.team, 0, 0};
+      late.c = few.begin(1);
       if (early > 0) few.resolve(late);
       for (int i = 0; i < early; ++i) {
         few.copy_tokens(late, (slot + i) % kStages, hplane);
@@ -573,12 +564,12 @@ moe_few_kernel(const MoeFewArgs a) {
       copies_commit();
       copies_wait<0>();
     }
-    while (few.settle(at) && at.phase == P) {
-      Item it = few.item(at);
-      const bool over = it.cnt <= kCols;         // the item's last pass
-      it.cnt = min(it.cnt, kCols);
+    const int runs = few.run1(P) - few.run0(P);
+    Cursor at = few.begin(P);
+    int summed = 0;                              // experts of the block that this team has finished
+    while (at.left > 0) {
+      const int e = few.expert(at), first = s.start[e] + at.pass * kCols, cnt = s.start[e + 1] - first;
       float acc[2][4] = {};
-      const int runs = few.run1(P) - few.run0(P);
 #pragma unroll 1
       for (int k = 0; k < runs; ++k) {
         copies_wait<kStages - 1>();
@@ -605,7 +596,7 @@ moe_few_kernel(const MoeFewArgs a) {
 #pragma unroll
         for (int q = 0; q < kTeam; ++q) v[m] += red[q * 256 + (m * 4 + ri) * 32 + rl];
       }
-      const int p = n < it.cnt ? s.pair[it.first + n] : -1;
+      const int p = n < cnt ? s.pair[first + n] : -1;
       if constexpr (P == 0) {
         if (FP8 && p >= 0) {
           const float f = a.x_factor[p / a.topk];
@@ -619,30 +610,36 @@ moe_few_kernel(const MoeFewArgs a) {
           for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           const float f = factor_of(__uint_as_float(top));
           if (p >= 0) {
-            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + it.block * 16 + row] = __float2half_rn(hv * (1.f / f));
-            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + it.block] = f;
+            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + at.block * 16 + row] = __float2half_rn(hv * (1.f / f));
+            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + at.block] = f;
           }
         } else if (p >= 0) {
           const bf16 top = __float2bfloat16(hv);
-          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + it.block * 16 + row;
+          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + at.block * 16 + row;
           dst[0] = top;
           dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
         }
       } else if (p >= 0) {
-        float* dst = a.slots + (int64_t)p * a.H + it.block * 32 + row;
+        float* dst = a.slots + (int64_t)p * a.H + at.block * 32 + row;
         dst[0] = v[0];
         dst[16] = v[1];
       }
+      if (cnt > kCols) { ++at.pass; continue; }
+      const int block = at.block;
+      few.next(at);
       if constexpr (P == 1) {
-        if (over) {
-          // the team that brings a block's last expert adds the slots of every token
+        ++summed;
+        if (at.left == 0 || at.block != block) {
+          // Experts of a block are counted when a team leaves it; the team that brings the last ones
+          // adds the slots of every token.
           __threadfence();
           named_barrier_sync(1 + team_in, kTeam * 32);
-          if (tt == 0) last_s[team_in] = atomicAdd(&a.done[it.block], 1) == s.n_touched - 1;
+          if (tt == 0) last_s[team_in] = atomicAdd(&a.done[block], summed) + summed == s.n_touched;
           named_barrier_sync(1 + team_in, kTeam * 32);
+          summed = 0;
           if (last_s[team_in]) {
             __threadfence();
-            const int c = it.block * 32 + (tt & 7) * 4;
+            const int c = block * 32 + (tt & 7) * 4;
             for (int t = tt >> 3; t < a.T; t += kTeam * 4) {
               float4 v[kFewMaxTopk];
 #pragma unroll
@@ -667,7 +664,6 @@ moe_few_kernel(const MoeFewArgs a) {
           }
         }
       }
-      if (over) { at.pass = 0; at.i += few.teams; } else { ++at.pass; }
     }
   };
   run_phase(std::integral_constant<int, 0>{});
