@@ -932,10 +932,11 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
                   (*t)->scalar_type() == (t == &ids ? torch::kInt32 : torch::kFloat32),
                   "ids (int32) and weights (fp32) must be [tokens, topk]");
   c10::cuda::CUDAGuard guard(x.device());
-  // [slots | hidden rows | their factors | x as f16 | logits | x factors | counters], floats
+  // [slots | hidden rows | their factors | x as f16 | logits | x factors | selection | counters], floats
   const int64_t P = T * topk, at_h = P * H, at_hf = at_h + P * I, at_x = at_hf + P * (I / 16), at_l = at_x + T * H / 2,
-                at_xf = at_l + (T * E + 3) / 4 * 4, at_done = at_xf + (T + 3) / 4 * 4;
-  Tensor ws = torch::empty({at_done + H / 32}, x.options().dtype(torch::kFloat32));
+                at_xf = at_l + (T * E + 3) / 4 * 4, at_sel = at_xf + (T + 3) / 4 * 4,
+                at_done = at_sel + 2 * P;
+  Tensor ws = torch::empty({at_done + H / 128}, x.options().dtype(torch::kFloat32));
   float* const w = ws.data_ptr<float>();
   b200::MoeFewArgs a{};
   a.x = x.data_ptr();
@@ -956,6 +957,7 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
   a.x16 = w + at_x;
   a.logits = w + at_l;
   a.x_factor = w + at_xf;
+  a.sel = reinterpret_cast<int2*>(w + at_sel);
   a.done = reinterpret_cast<int*>(w + at_done);
   a.status = status.data_ptr<int>();
   b200::moe_few(a, stream());

@@ -29,7 +29,8 @@ struct MoeFewArgs {
   void* h;                   // [T * topk, I] f16, h / h_factor (e4m3 weights), or [2, T * topk, I] bf16
   float* h_factor;           // [T * topk, I / 16]
   float* slots;              // [T * topk, H]
-  int* done;                 // [H / 32]
+  int2* sel;                 // [T * topk] chosen experts and weights
+  int* done;                 // [H / 128]
   int* status;
 };
 void moe_few(const MoeFewArgs& a, cudaStream_t s);

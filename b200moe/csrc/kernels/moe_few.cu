@@ -68,22 +68,64 @@ __device__ __forceinline__ float bf16_of(double v) {
   return __bfloat162float(__float2bfloat16(f));
 }
 
+constexpr int kPairs = kFewMaxTokens * kFewMaxTopk;
+
+// Routing tables.  A pass is up to kCols tokens of one expert; passes are in expert order.
 struct Shared {
   uint64_t mask[kFewMaxExperts];        // tokens of each expert
-  int start[kFewMaxExperts + 1];        // first pair of each expert
-  int touched[kFewMaxExperts];          // experts with at least one token
-  int n_touched;
   int2 warp_sums[kFewMaxExperts / 32];
-  short pair[kFewMaxTokens * kFewMaxTopk];   // pairs (token * topk + k) in (expert, token) order
-  short sel_e[kFewMaxTokens * kFewMaxTopk];
-  float sel_w[kFewMaxTokens * kFewMaxTopk];
+  int passes;
+  short start[kFewMaxExperts + 2];      // first pair of each expert
+  uint8_t pass_e[kPairs];               // expert of each pass
+  short pass_first[kPairs];             // its first pair and how many
+  uint8_t pass_cnt[kPairs];
+  uint8_t token[kPairs];                // token of each pair, in (expert, token) order
+  short pair[kPairs];                   // token * topk + k of each pair
+  uint8_t sel_e[kPairs];
+  float sel_w[kPairs];
 };
 
 // Logits of experts blockIdx.x, blockIdx.x + gridDim.x, ...: a product of two bf16 is exact in
 // fp32 and the sum of four stays so for nearly all of them; beyond that the sum runs in fp64,
 // because a logit is rounded to bf16 and a wrong last bit there can change the experts.
+// Exact products of eight bf16 pairs, summed by fours in fp32, the rest in fp64.
+__device__ __forceinline__ double dot8(const uint4& w, const uint4& x) {
+  const uint32_t wu[4] = {w.x, w.y, w.z, w.w}, xu[4] = {x.x, x.y, x.z, x.w};
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[2 * i] = __uint_as_float(wu[i] << 16) * __uint_as_float(xu[i] << 16);
+    p[2 * i + 1] = __uint_as_float(wu[i] & 0xffff0000u) * __uint_as_float(xu[i] & 0xffff0000u);
+  }
+  return (double)((p[0] + p[1]) + (p[2] + p[3])) + (double)((p[4] + p[5]) + (p[6] + p[7]));
+}
+
 __device__ void few_logits(const MoeFewArgs& a, double* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.T > kWarps) {
+    // many tokens: tiles of 16 tokens (a warp each) x 4 experts, so x is not read once per expert
+    const int groups = (a.T + kWarps - 1) / kWarps, tiles = groups * ((a.E + 3) / 4);
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+      const int t = i % groups * kWarps + warp, e0 = i / groups * 4;
+      if (t >= a.T) continue;
+      const bf16* xr = static_cast<const bf16*>(a.x) + t * a.H;
+      const bf16* wr = static_cast<const bf16*>(a.router) + e0 * a.H;   // the last rows are repeated below
+      double acc[4] = {0.0, 0.0, 0.0, 0.0};
+      for (int c = lane * 8; c < a.H; c += 256) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[j] += dot8(__ldg(reinterpret_cast<const uint4*>(wr + min(j, a.E - 1 - e0) * a.H + c)), xv);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+        if (lane == j && e0 + j < a.E) a.logits[t * a.E + e0 + j] = bf16_of(acc[j]);
+      }
+    }
+    return;
+  }
   // few tokens: several warps share one, a part of K each
   const int share = a.T > 8 ? 1 : a.T > 4 ? 2 : a.T > 2 ? 4 : a.T > 1 ? 8 : 16;
   const int sub = warp % share;
@@ -92,18 +134,9 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
     for (int t = warp / share; t < a.T; t += kWarps / share) {
       const bf16* xr = static_cast<const bf16*>(a.x) + (int64_t)t * a.H;
       double acc = 0.0;
-#pragma unroll 4
+#pragma unroll 2
       for (int c = (sub * 32 + lane) * 8; c < a.H; c += share * 256) {
-        const uint4 wv = *reinterpret_cast<const uint4*>(wr + c), xv = *reinterpret_cast<const uint4*>(xr + c);
-        const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w}, xu[4] = {xv.x, xv.y, xv.z, xv.w};
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[2 * i] = __uint_as_float(wu[i] << 16) * __uint_as_float(xu[i] << 16);
-          p[2 * i + 1] = __uint_as_float(wu[i] & 0xffff0000u) * __uint_as_float(xu[i] & 0xffff0000u);
-        }
-        acc += (double)((p[0] + p[1]) + (p[2] + p[3]));
-        acc += (double)((p[4] + p[5]) + (p[6] + p[7]));
+        acc += dot8(*reinterpret_cast<const uint4*>(wr + c), *reinterpret_cast<const uint4*>(xr + c));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
@@ -158,97 +191,130 @@ __device__ void few_rows(const MoeFewArgs& a, float* red) {
   }
 }
 
-// Top-k and weights of every token and the pairs in expert order; every CTA does all of it.
+// Top-k and weights of token t by one warp: lane k < topk gets the k-th expert and its weight.
 template <int EPL>
-__device__ void few_route(const MoeFewArgs& a, Shared& s) {
+__device__ __forceinline__ void few_topk(const MoeFewArgs& a, int t, int lane, int& pick, float& w) {
+  float v[EPL];
+  uint32_t key[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) v[j] = j * 32 + lane < a.E ? __ldcg(a.logits + t * a.E + j * 32 + lane) : -INFINITY;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = j * 32 + lane;
+    // (logit, lowest id first) as one unsigned key: bf16 bits in order, then 0xffff - id
+    uint32_t u = __float_as_uint(v[j]) >> 16;
+    u = (u & 0x8000u) ? (0xffffu ^ u) : (u | 0x8000u);
+    key[j] = e < a.E ? (u << 16) | (0xffffu - e) : 0u;
+  }
+  uint32_t mine = 0;               // lane k: the k-th key
+  uint32_t first = 0;
+  for (int k = 0; k < a.topk; ++k) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (k == 0) first = best;
+    if (lane == k) mine = best;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (key[j] == best) key[j] = 0u;
+  }
+  auto logit_of = [](uint32_t k) {
+    const uint32_t u = k >> 16;
+    return __uint_as_float(((u & 0x8000u) ? (u & 0x7fffu) : (0xffffu ^ u)) << 16);
+  };
+  const float mx = logit_of(first);
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) sum += expf(v[j] - mx);       // no expert: exp(-inf) = 0
+  sum = warp_sum(sum);
+  w = lane < a.topk ? expf(logit_of(mine) - mx) / sum : 0.f;
+  const float wsum = warp_sum(w);
+  if (a.renorm) w /= wsum;
+  w = __bfloat162float(__float2bfloat16(w));
+  pick = 0xffff - (int)(mine & 0xffffu);
+}
+
+// The routing tables, in every CTA.  Up to 16 tokens every CTA does the top-k of all; more tokens are
+// spread over the CTAs and exchanged, which costs a barrier and saves a CTA the later rounds of 16.
+template <int EPL>
+__device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < kFewMaxExperts; e += kThreads) s.mask[e] = 0;
+  const bool spread = a.T > kWarps;
+  if (spread) {
+    const int t = blockIdx.x + warp * gridDim.x;             // tokens side by side on different SMs
+    if (t < a.T) {
+      int pick;
+      float w;
+      few_topk<EPL>(a, t, lane, pick, w);
+      if (lane < a.topk) {
+        __stcg(a.sel + t * a.topk + lane, make_int2(pick, __float_as_int(w)));
+        if (a.ids != nullptr) a.ids[t * a.topk + lane] = pick;
+        if (a.weights != nullptr) a.weights[t * a.topk + lane] = w;
+      }
+    }
+    grid.sync();
+  }
   __syncthreads();
   for (int t = warp; t < a.T; t += kWarps) {
-    float v[EPL];
-    uint32_t key[EPL];
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) v[j] = j * 32 + lane < a.E ? __ldcg(a.logits + t * a.E + j * 32 + lane) : -INFINITY;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = j * 32 + lane;
-      // (logit, lowest id first) as one unsigned key: bf16 bits in order, then 0xffff - id
-      uint32_t u = __float_as_uint(v[j]) >> 16;
-      u = (u & 0x8000u) ? (0xffffu ^ u) : (u | 0x8000u);
-      key[j] = e < a.E ? (u << 16) | (0xffffu - e) : 0u;
+    int pick = 0;
+    float w = 0.f;
+    if (spread) {
+      if (lane < a.topk) {
+        const int2 x = __ldcg(a.sel + t * a.topk + lane);
+        pick = x.x;
+        w = __int_as_float(x.y);
+      }
+    } else {
+      few_topk<EPL>(a, t, lane, pick, w);
     }
-    uint32_t mine = 0;             // lane k: the k-th key
-    uint32_t first = 0;
-    for (int k = 0; k < a.topk; ++k) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
-      best = __reduce_max_sync(0xffffffffu, best);
-      if (k == 0) first = best;
-      if (lane == k) mine = best;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (key[j] == best) key[j] = 0u;
-    }
-    auto logit_of = [](uint32_t k) {
-      const uint32_t u = k >> 16;
-      return __uint_as_float(((u & 0x8000u) ? (u & 0x7fffu) : (0xffffu ^ u)) << 16);
-    };
-    const float mx = logit_of(first);
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) sum += expf(v[j] - mx);     // no expert: exp(-inf) = 0
-    sum = warp_sum(sum);
-    float w = lane < a.topk ? expf(logit_of(mine) - mx) / sum : 0.f;
-    const float wsum = warp_sum(w);
     if (lane < a.topk) {
-      if (a.renorm) w /= wsum;
-      w = __bfloat162float(__float2bfloat16(w));
-      const int p = t * a.topk + lane, pick = 0xffff - (int)(mine & 0xffffu);
-      s.sel_e[p] = (short)pick;
+      const int p = t * a.topk + lane;
+      s.sel_e[p] = (uint8_t)pick;
       s.sel_w[p] = w;
       atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[pick]), 1ull << t);
-      if (blockIdx.x == 0) {
+      if (!spread && blockIdx.x == 0) {
         if (a.ids != nullptr) a.ids[p] = pick;
         if (a.weights != nullptr) a.weights[p] = w;
       }
     }
   }
   __syncthreads();
-  // first pair of every expert and the list of touched ones: a thread per expert
+  // first pair and passes of every expert: a thread per expert
   const int e = threadIdx.x;
-  int c = 0, incl = 0;
-  unsigned has = 0;
+  int c = 0, np = 0, ci = 0, ni = 0;
   if (e < kFewMaxExperts) {
-    c = __popcll(s.mask[e]);
-    incl = c;
+    c = ci = __popcll(s.mask[e]);
+    np = ni = (c + kCols - 1) / kCols;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+      const int cu = __shfl_up_sync(0xffffffffu, ci, o), nu = __shfl_up_sync(0xffffffffu, ni, o);
+      if (lane >= o) { ci += cu; ni += nu; }
     }
-    has = __ballot_sync(0xffffffffu, c > 0);
-    if (lane == 31) s.warp_sums[warp] = make_int2(incl, __popc(has));
+    if (lane == 31) s.warp_sums[warp] = make_int2(ci, ni);
   }
   __syncthreads();
   if (e < kFewMaxExperts) {
-    int at = 0, nt = 0;
 #pragma unroll
     for (int i = 0; i < kFewMaxExperts / 32; ++i) {
       const int2 x = s.warp_sums[i];
-      if (i < warp) { at += x.x; nt += x.y; }
+      if (i < warp) { ci += x.x; ni += x.y; }
     }
-    s.start[e] = at + incl - c;
-    if (c > 0) s.touched[nt + __popc(has & ((1u << lane) - 1))] = e;
-    if (e == kFewMaxExperts - 1) {
-      s.n_touched = nt + __popc(has);
-      s.start[kFewMaxExperts] = a.T * a.topk;
+    s.start[e] = (short)(ci - c);
+    for (int i = 0; i < np; ++i) {
+      const int q = ni - np + i;
+      s.pass_e[q] = (uint8_t)e;
+      s.pass_first[q] = (short)(ci - c + i * kCols);
+      s.pass_cnt[q] = (uint8_t)min(kCols, c - i * kCols);
     }
+    if (e == kFewMaxExperts - 1) s.passes = ni;
   }
   __syncthreads();
   for (int p = threadIdx.x; p < a.T * a.topk; p += kThreads) {
-    const int x = s.sel_e[p], t = p / a.topk;
-    s.pair[s.start[x] + __popcll(s.mask[x] & ((1ull << t) - 1))] = (short)p;
+    const int x = s.sel_e[p], t = p / a.topk, at = s.start[x] + __popcll(s.mask[x] & ((1ull << t) - 1));
+    s.pair[at] = (short)p;
+    s.token[at] = (uint8_t)t;
   }
   __syncthreads();
 }
@@ -262,12 +328,8 @@ static_assert(kSmem <= 232448, "shared memory budget");
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// 16 or 4 bytes, zeros where there is nothing to copy
-__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4_or_zero(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all but the newest N groups have landed
@@ -309,46 +371,50 @@ struct Few {
   int lane, part, team, teams;     // part: quarter of K; team: over the grid
 
   // ------------------------------------------------------------ the stream of items
-  // Items of phase 0 (gate and up rows; an expert's blocks together) and of phase 1 (rows of Wd; a
-  // block's experts together, so that its sum is over early).  A team takes the team-th of equal
-  // runs of either order, and an item is as many passes as its tokens need.
-  __device__ __forceinline__ int blocks(int phase) const { return phase ? a.H / 32 : a.I / 16; }
+  // An item is a pass against a block of rows: 16 gate and up rows (phase 0) or 32 rows of Wd (phase 1).
+  // Blocks are parts of a tile of 128 rows.  Order of phase 0: pass, tile, block; of phase 1: tile, pass,
+  // block, so that the sums of 128 outputs are over early.  A team takes the team-th of equal runs of
+  // either order, and within a tile only addresses move on.
+  __device__ __forceinline__ int tiles(int phase) const { return (phase ? a.H : a.I) >> 7; }
+  __device__ __forceinline__ static constexpr int subs(int phase) { return phase ? 4 : 8; }
   __device__ __forceinline__ int run0(int phase) const { return (phase ? a.I : a.H) / 64 * part / kTeam; }
   __device__ __forceinline__ int run1(int phase) const { return (phase ? a.I : a.H) / 64 * (part + 1) / kTeam; }
 
   struct Cursor {
     int phase, left;               // phase 2: over; items left in the phase, this one among them
-    int x, block, pass;            // touched expert, block, pass of kCols tokens
+    int q, tile, sub;              // pass, tile of rows, block of the tile
   };
   __device__ __forceinline__ Cursor begin(int phase) const {
     Cursor c;
     c.phase = phase;
-    const int n = s.n_touched * blocks(phase), lo = n / teams * team + min(team, n % teams);
+    const int n = s.passes * tiles(phase) * subs(phase), lo = n / teams * team + min(team, n % teams);
     c.left = n / teams + (team < n % teams ? 1 : 0);
-    const int inner = phase ? s.n_touched : blocks(0), o = lo / inner;
-    c.x = phase ? lo - o * inner : o;
-    c.block = phase ? o : lo - o * inner;
-    c.pass = 0;
+    const int inner = phase ? s.passes : tiles(phase), x = lo / subs(phase), o = x / inner;
+    c.sub = lo % subs(phase);
+    c.q = phase ? x - o * inner : o;
+    c.tile = phase ? o : x - o * inner;
     return c;
   }
-  __device__ __forceinline__ int expert(const Cursor& c) const { return s.touched[c.x]; }
-  __device__ __forceinline__ void next(Cursor& c) const {      // behind the item's last pass
-    c.pass = 0;
-    if (--c.left == 0) return;
+  // to the next item; true: in the same tile and pass
+  __device__ __forceinline__ bool next(Cursor& c) const {
+    if (--c.left == 0) return false;
+    if (++c.sub < subs(c.phase)) return true;
+    c.sub = 0;
     if (c.phase == 0) {
-      if (++c.block == blocks(0)) { c.block = 0; ++c.x; }
+      if (++c.tile == tiles(0)) { c.tile = 0; ++c.q; }
     } else {
-      if (++c.x == s.n_touched) { c.x = 0; ++c.block; }
+      if (++c.q == s.passes) { c.q = 0; ++c.tile; }
     }
+    return false;
   }
 
-  // The pass whose runs are being brought in, resolved once.
+  // The item whose runs are being brought in.
   struct Ahead {
     Cursor c;
-    int st, runs, tokens;          // run of 64 K, runs of this warp; tokens of this pass and behind it
-    const uint8_t* p0;             // this lane's weights of rows g of the two row blocks
-    const uint8_t* p1;
-    int row8, run;                 // bytes from row g to row g + 8, and to the next run
+    int st, runs;                  // run of 64 K, runs of this warp
+    const uint8_t* w0;             // this lane's weights of rows g of the two row blocks, run st
+    const uint8_t* w1;
+    int row8, run, block;          // bytes from row g to row g + 8, to the next run, to the next block
     const uint16_t* tok;           // this lane's token or hidden row; null: none
     const float* fac;              // its factors
     const float* sc;               // lanes 0 and 1: block scales of a row block
@@ -362,73 +428,80 @@ struct Few {
       h.c = begin(1);
     }
     if (h.c.phase == 2) return;
-    const int ph = h.c.phase, e = expert(h.c), first = s.start[e] + h.c.pass * kCols;
-    h.tokens = s.start[e + 1] - first;
+    const int ph = h.c.phase, e = s.pass_e[h.c.q];
     h.st = 0;
     h.k0 = run0(ph);
     h.runs = run1(ph) - h.k0;
     const int N = ph ? a.H : 2 * a.I, K = ph ? a.I : a.H;
-    const int row0 = ph ? h.c.block * 32 : h.c.block * 16, row1 = ph ? row0 + 16 : a.I + row0;
+    // rows of the first block of the tile, and of the block's second half
+    const uint32_t r0 = (uint32_t)(e * N + h.c.tile * 128), r1 = ph ? r0 : r0 + a.I;
     const int g = lane >> 2, t = lane & 3;
     const uint8_t* w = static_cast<const uint8_t*>(ph ? a.w2 : a.w13);
+    const int rows = ph ? 32 : 16;                     // of a block in either half
+    uint32_t row;                                      // bytes of a row
     if (FP8 && a.tiled) {
       // [row / 128][K / 64][128][64]; 16-byte chunk u of a row at u ^ ((row >> 1) & 3)
-      w += g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
-      const uint32_t tiles = K >> 6, r0 = (uint32_t)(e * N + row0), r1 = (uint32_t)(e * N + row1);
-      h.p0 = w + (uint64_t)((r0 >> 7) * tiles + h.k0) * 8192 + (r0 & 127) * 64;
-      h.p1 = w + (uint64_t)((r1 >> 7) * tiles + h.k0) * 8192 + (r1 & 127) * 64;
-      h.row8 = 512;
+      row = 64;
       h.run = 8192;
+      w += g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
+      h.w0 = w + (uint64_t)((r0 >> 7) * (K >> 6) + h.k0) * 8192;
+      h.w1 = w + (uint64_t)((r1 >> 7) * (K >> 6) + h.k0) * 8192;
     } else {
-      const uint32_t row = K * (FP8 ? 1 : 2);
+      row = K * (FP8 ? 1 : 2);
       h.run = FP8 ? 64 : 128;
       w += h.k0 * h.run + t * 16;
-      h.p0 = w + (uint64_t)(uint32_t)(e * N + row0 + g) * row;
-      h.p1 = w + (uint64_t)(uint32_t)(e * N + row1 + g) * row;
-      h.row8 = 8 * row;
+      h.w0 = w + (uint64_t)(r0 + g) * row;
+      h.w1 = w + (uint64_t)(r1 + g) * row;
     }
+    h.row8 = 8 * row;
+    h.block = rows * row;
+    h.w0 += h.c.sub * h.block;
+    h.w1 += h.c.sub * h.block + (ph ? 16 * row : 0);
+    h.block -= h.runs * h.run;                         // from behind the last run
     h.tok = nullptr;
-    if (g < h.tokens) {
-      const int p = s.pair[first + g];
-      if (ph == 0) h.tok = static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + (p / a.topk) * a.H;
-      else h.tok = static_cast<const uint16_t*>(a.h) + p * a.I;
+    if (g < s.pass_cnt[h.c.q]) {
+      const int at = s.pass_first[h.c.q] + g;
+      h.tok = ph == 0 ? static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + s.token[at] * a.H
+                      : static_cast<const uint16_t*>(a.h) + s.pair[at] * a.I;
       h.tok += h.k0 * 64 + t * (FP8 ? 16 : 8);
-      h.fac = a.h_factor + p * (a.I / 16) + h.k0 * 4 + t;
+      if (FP8) h.fac = a.h_factor + s.pair[at] * (a.I / 16) + h.k0 * 4 + t;
     }
-    if (FP8)
-      h.sc = (ph ? a.s2 : a.s13) + (uint64_t)((uint32_t)(e * N + (lane == 0 ? row0 : row1)) >> 7) * (K >> 7);
+    if (FP8) h.sc = (ph ? a.s2 : a.s13) + (uint64_t)((lane == 0 ? r0 : r1) >> 7) * (K >> 7);
   }
   __device__ __forceinline__ void copy_weights(const Ahead& h, int slot) const {
     const uint32_t dst = smem_u32(ring + slot * kStageBytes + lane * 16);
-    const uint8_t* q0 = h.p0 + (int64_t)h.st * h.run;
-    const uint8_t* q1 = h.p1 + (int64_t)h.st * h.run;
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
-      copy16(dst + (0 * PER + v) * 512, q0 + v * 64);
-      copy16(dst + (1 * PER + v) * 512, q0 + h.row8 + v * 64);
-      copy16(dst + (2 * PER + v) * 512, q1 + v * 64);
-      copy16(dst + (3 * PER + v) * 512, q1 + h.row8 + v * 64);
+      copy16(dst + (0 * PER + v) * 512, h.w0 + v * 64);
+      copy16(dst + (1 * PER + v) * 512, h.w0 + h.row8 + v * 64);
+      copy16(dst + (2 * PER + v) * 512, h.w1 + v * 64);
+      copy16(dst + (3 * PER + v) * 512, h.w1 + h.row8 + v * 64);
     }
-    if (FP8 && lane < 2)
-      copy4_or_zero(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.st) >> 1), true);
+    if (FP8 && lane < 2) copy4(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.st) >> 1));
   }
+  // A lane without a token leaves its place as it is: what stands there makes a column nobody reads.
   __device__ __forceinline__ void copy_tokens(const Ahead& h, int slot, int64_t plane) const {
+    if (h.tok == nullptr) return;
     const uint32_t dst = smem_u32(ring + slot * kStageBytes + W + lane * 16);
-    const bool have = h.tok != nullptr;
-    const uint16_t* src = have ? h.tok + h.st * 64 : static_cast<const uint16_t*>(a.x);
+    const uint16_t* src = h.tok + h.st * 64;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      copy16_or_zero(dst + v * 512, src + v * (FP8 ? 8 : 32), have);
-      if (!FP8 && h.c.phase == 1) copy16_or_zero(dst + (2 + v) * 512, src + (have ? plane : 0) + v * 32, have);
+      copy16(dst + v * 512, src + v * (FP8 ? 8 : 32));
+      if (!FP8 && h.c.phase == 1) copy16(dst + (2 + v) * 512, src + plane + v * 32);
     }
-    if (FP8 && h.c.phase == 1)
-      copy4_or_zero(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), have ? h.fac + h.st * 4 : a.s2, have);
+    if (FP8 && h.c.phase == 1) copy4(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), h.fac + h.st * 4);
   }
   __device__ __forceinline__ void step(Ahead& h) const {
+    h.w0 += h.run;
+    h.w1 += h.run;
     if (++h.st < h.runs) return;
-    if (h.tokens > kCols) ++h.c.pass;
-    else next(h.c);
-    resolve(h);
+    if (next(h.c)) {
+      h.st = 0;
+      h.w0 += h.block;
+      h.w1 += h.block;
+    } else {
+      resolve(h);
+    }
   }
 
   // acc[m] += 16 weight rows x 8 tokens of one run of 64 K
@@ -516,12 +589,12 @@ moe_few_kernel(const MoeFewArgs a) {
   const int team_in = warp / kTeam, tt = threadIdx.x % (kTeam * 32);
   cg::grid_group grid = cg::this_grid();
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < a.H / 32; i += kThreads) a.done[i] = 0;
+    for (int i = threadIdx.x; i < a.H / 128; i += kThreads) a.done[i] = 0;
   few_logits(a, reinterpret_cast<double*>(smem + kRed));
   if (FP8) few_rows(a, reinterpret_cast<float*>(smem + kRed));
   grid.sync();
-  if (a.E <= 128) few_route<4>(a, s);
-  else few_route<kFewMaxExperts / 32>(a, s);
+  if (a.E <= 128) few_route<4>(a, s, grid);
+  else few_route<kFewMaxExperts / 32>(a, s, grid);
 
   Few<FP8> few{a, s, smem + warp * kRingBytes, lane, warp % kTeam,
                team_in * (int)gridDim.x + (int)blockIdx.x, kTeams * (int)gridDim.x};
@@ -566,9 +639,10 @@ moe_few_kernel(const MoeFewArgs a) {
     }
     const int runs = few.run1(P) - few.run0(P);
     Cursor at = few.begin(P);
-    int summed = 0;                              // experts of the block that this team has finished
+    int summed = 0;                              // items of the tile that this team has finished
     while (at.left > 0) {
-      const int e = few.expert(at), first = s.start[e] + at.pass * kCols, cnt = s.start[e + 1] - first;
+      const int first = s.pass_first[at.q], cnt = s.pass_cnt[at.q];
+      const int col = at.tile * 128 + at.sub * (P ? 32 : 16);
       float acc[2][4] = {};
 #pragma unroll 1
       for (int k = 0; k < runs; ++k) {
@@ -599,7 +673,7 @@ moe_few_kernel(const MoeFewArgs a) {
       const int p = n < cnt ? s.pair[first + n] : -1;
       if constexpr (P == 0) {
         if (FP8 && p >= 0) {
-          const float f = a.x_factor[p / a.topk];
+          const float f = a.x_factor[s.token[first + n]];
           v[0] *= f;
           v[1] *= f;
         }
@@ -610,37 +684,36 @@ moe_few_kernel(const MoeFewArgs a) {
           for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           const float f = factor_of(__uint_as_float(top));
           if (p >= 0) {
-            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + at.block * 16 + row] = __float2half_rn(hv * (1.f / f));
-            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + at.block] = f;
+            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + col + row] = __float2half_rn(hv * (1.f / f));
+            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + (col >> 4)] = f;
           }
         } else if (p >= 0) {
           const bf16 top = __float2bfloat16(hv);
-          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + at.block * 16 + row;
+          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + col + row;
           dst[0] = top;
           dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
         }
       } else if (p >= 0) {
-        float* dst = a.slots + (int64_t)p * a.H + at.block * 32 + row;
+        float* dst = a.slots + (int64_t)p * a.H + col + row;
         dst[0] = v[0];
         dst[16] = v[1];
       }
-      if (cnt > kCols) { ++at.pass; continue; }
-      const int block = at.block;
+      const int tile = at.tile;
       few.next(at);
       if constexpr (P == 1) {
         ++summed;
-        if (at.left == 0 || at.block != block) {
-          // Experts of a block are counted when a team leaves it; the team that brings the last ones
+        if (at.left == 0 || at.tile != tile) {
+          // Items of a tile are counted when a team leaves it; the team that brings the last ones
           // adds the slots of every token.
           __threadfence();
           named_barrier_sync(1 + team_in, kTeam * 32);
-          if (tt == 0) last_s[team_in] = atomicAdd(&a.done[block], summed) + summed == s.n_touched;
+          if (tt == 0) last_s[team_in] = atomicAdd(&a.done[tile], summed) + summed == s.passes * 4;
           named_barrier_sync(1 + team_in, kTeam * 32);
           summed = 0;
           if (last_s[team_in]) {
             __threadfence();
-            const int c = block * 32 + (tt & 7) * 4;
-            for (int t = tt >> 3; t < a.T; t += kTeam * 4) {
+            const int c = tile * 128 + (tt & 31) * 4;
+            for (int t = tt >> 5; t < a.T; t += kTeam) {
               float4 v[kFewMaxTopk];
 #pragma unroll
               for (int k = 0; k < kFewMaxTopk; ++k)
