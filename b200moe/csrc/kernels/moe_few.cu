@@ -9,9 +9,9 @@
 // logits and after the experts' hidden rows.
 //
 // Nearly all the time goes into reading the touched experts' weights once, so the
-// kernel is built around that stream.  Four warps (a team) take 32 weight rows of one
-// expert -- 16 gate and the 16 up rows beside them, or 32 rows of Wd -- and a quarter of
-// K each, for up to 8 of its tokens at a time.  Every lane brings what it multiplies
+// kernel is built around that stream.  A team of four, two or one warps takes 32 weight
+// rows of one expert -- 16 gate and the 16 up rows beside them, or 32 rows of Wd -- and
+// each warp its part of K, for up to 8 of its tokens at a time.  Every lane brings what it multiplies
 // itself, weights and tokens alike, into its own places of a ring per warp (16-byte
 // asynchronous copies): no bank conflict lies on the way, any weight layout is an address
 // rule, and nothing that comes from memory is waited for in a register.  The ring is
@@ -28,7 +28,7 @@
 // fp32 sums of 64 products, so a weight counts as exactly q * scale.  With bf16
 // weights x enters as it is and a hidden value as two bf16, value and rest.
 //
-// The quarters of K are added in order through shared memory.  The rows of Wd write fp32 (token, k) slots, and the team that finishes the last expert of
+// The parts of K are added in order through shared memory.  The rows of Wd write fp32 (token, k) slots, and the team that finishes the last expert of
 // a block of 32 columns adds the token's slots in the order of the top-k.
 //
 // Rounding points: the logits and the routing weights are rounded to bf16 (those of the
@@ -56,9 +56,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTeam = 4;                 // warps of a team, each a part of K
-constexpr int kTeams = kWarps / kTeam;
-constexpr int kRingBytes = 12928;        // of a warp
+constexpr int kRingBytes = 12832;        // of a warp
 constexpr int kCols = 8;                 // tokens of one pass
 
 // fp64 -> bf16 in one rounding: fp32 with round-to-odd keeps the bit that decides a tie.
@@ -72,7 +70,7 @@ constexpr int kPairs = kFewMaxTokens * kFewMaxTopk;
 
 // Routing tables.  A pass is up to kCols tokens of one expert; passes are in expert order.
 struct Shared {
-  uint64_t mask[kFewMaxExperts];        // tokens of each expert
+  uint32_t mask[2][kFewMaxExperts];     // tokens of each expert, 32 to a word
   int2 warp_sums[kFewMaxExperts / 32];
   int passes;
   short start[kFewMaxExperts + 2];      // first pair of each expert
@@ -111,6 +109,7 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
       const bf16* xr = static_cast<const bf16*>(a.x) + t * a.H;
       const bf16* wr = static_cast<const bf16*>(a.router) + e0 * a.H;   // the last rows are repeated below
       double acc[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 2
       for (int c = lane * 8; c < a.H; c += 256) {
         const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
 #pragma unroll
@@ -134,7 +133,7 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
     for (int t = warp / share; t < a.T; t += kWarps / share) {
       const bf16* xr = static_cast<const bf16*>(a.x) + (int64_t)t * a.H;
       double acc = 0.0;
-#pragma unroll 2
+#pragma unroll 8
       for (int c = (sub * 32 + lane) * 8; c < a.H; c += share * 256) {
         acc += dot8(*reinterpret_cast<const uint4*>(wr + c), *reinterpret_cast<const uint4*>(xr + c));
       }
@@ -191,6 +190,15 @@ __device__ void few_rows(const MoeFewArgs& a, float* red) {
   }
 }
 
+// n / d for 0 <= n < 2^24, without the compiler's division.
+__device__ __forceinline__ int quotient(int n, int d) {
+  int q = (int)__fdividef((float)n, (float)d);
+  const int r = n - q * d;
+  if (r < 0) --q;
+  if (r >= d) ++q;
+  return q;
+}
+
 // Top-k and weights of token t by one warp: lane k < topk gets the k-th expert and its weight.
 template <int EPL>
 __device__ __forceinline__ void few_topk(const MoeFewArgs& a, int t, int lane, int& pick, float& w) {
@@ -240,7 +248,7 @@ __device__ __forceinline__ void few_topk(const MoeFewArgs& a, int t, int lane, i
 template <int EPL>
 __device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < kFewMaxExperts; e += kThreads) s.mask[e] = 0;
+  for (int e = threadIdx.x; e < 2 * kFewMaxExperts; e += kThreads) (&s.mask[0][0])[e] = 0;
   const bool spread = a.T > kWarps;
   if (spread) {
     const int t = blockIdx.x + warp * gridDim.x;             // tokens side by side on different SMs
@@ -273,7 +281,7 @@ __device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) 
       const int p = t * a.topk + lane;
       s.sel_e[p] = (uint8_t)pick;
       s.sel_w[p] = w;
-      atomicOr(reinterpret_cast<unsigned long long*>(&s.mask[pick]), 1ull << t);
+      atomicOr(&s.mask[t >> 5][pick], 1u << (t & 31));
       if (!spread && blockIdx.x == 0) {
         if (a.ids != nullptr) a.ids[p] = pick;
         if (a.weights != nullptr) a.weights[p] = w;
@@ -285,7 +293,7 @@ __device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) 
   const int e = threadIdx.x;
   int c = 0, np = 0, ci = 0, ni = 0;
   if (e < kFewMaxExperts) {
-    c = ci = __popcll(s.mask[e]);
+    c = ci = __popc(s.mask[0][e]) + __popc(s.mask[1][e]);
     np = ni = (c + kCols - 1) / kCols;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -312,7 +320,9 @@ __device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) 
   }
   __syncthreads();
   for (int p = threadIdx.x; p < a.T * a.topk; p += kThreads) {
-    const int x = s.sel_e[p], t = p / a.topk, at = s.start[x] + __popcll(s.mask[x] & ((1ull << t) - 1));
+    const int x = s.sel_e[p], t = quotient(p, a.topk);
+    const uint32_t below = (1u << (t & 31)) - 1;
+    const int at = s.start[x] + (t < 32 ? __popc(s.mask[0][x] & below) : __popc(s.mask[0][x]) + __popc(s.mask[1][x] & below));
     s.pair[at] = (short)p;
     s.token[at] = (uint8_t)t;
   }
@@ -359,16 +369,17 @@ __device__ __forceinline__ uint32_t f16x2_of(uint32_t two) {
 template <bool FP8>
 struct Few {
   static constexpr int PER = FP8 ? 1 : 2;              // 16-byte pieces of a lane's 16 weights
-  // A stage of the ring holds a run of 64 K: weights [4 * PER][32 lanes] x 16 bytes, tokens [2 or 4][32] x 16
-  // bytes and, for e4m3, the hidden values' factors [32] and the two block scales.
+  // A stage of the ring holds two runs of 64 K, so that their products overlap.  A run: weights
+  // [4 * PER][32 lanes] x 16 bytes, tokens [2 or 4][32] x 16 bytes and, for e4m3, the hidden values'
+  // factors [32]; behind the stages the block scales, two for each run.
+  static constexpr int KPS = FP8 ? 2 : 1;
   static constexpr int W = 2048 * PER, B = FP8 ? 1024 : 2048;
-  static constexpr int kStageBytes = FP8 ? W + B + 128 : W + B;
-  static constexpr int kStages = FP8 ? 4 : 2;
-  static_assert(kStages * (kStageBytes + (FP8 ? 16 : 0)) <= kRingBytes, "ring");
+  static constexpr int kRunBytes = FP8 ? W + B + 128 : W + B, kStages = 2;
+  static_assert(kStages * KPS * (kRunBytes + (FP8 ? 8 : 0)) <= kRingBytes, "ring");
   const MoeFewArgs& a;
   Shared& s;
   uint8_t* ring;
-  int lane, part, team, teams;     // part: quarter of K; team: over the grid
+  int lane, part, kw, team, teams;  // part: of the kw parts of K; team: over the grid
 
   // ------------------------------------------------------------ the stream of items
   // An item is a pass against a block of rows: 16 gate and up rows (phase 0) or 32 rows of Wd (phase 1).
@@ -377,8 +388,25 @@ struct Few {
   // either order, and within a tile only addresses move on.
   __device__ __forceinline__ int tiles(int phase) const { return (phase ? a.H : a.I) >> 7; }
   __device__ __forceinline__ static constexpr int subs(int phase) { return phase ? 4 : 8; }
-  __device__ __forceinline__ int run0(int phase) const { return (phase ? a.I : a.H) / 64 * part / kTeam; }
-  __device__ __forceinline__ int run1(int phase) const { return (phase ? a.I : a.H) / 64 * (part + 1) / kTeam; }
+  // warps of a team (4, 2 or 1): the least rounds of items, each its runs and about one run's time more
+  __device__ __forceinline__ int team_warps(int phase) const {
+    const int n = s.passes * tiles(phase) * subs(phase), runs = (phase ? a.I : a.H) / 64;
+    int best = 4, cost = 1 << 30;
+#pragma unroll
+    for (int w = 4; w >= 1; w >>= 1) {
+      const int t = kWarps / w * (int)gridDim.x, c = (quotient(n + t - 1, t)) * (runs / w + 1);
+      if (c < cost) { cost = c; best = w; }
+    }
+    return best;
+  }
+  __device__ __forceinline__ void enter(int phase, int warp) {
+    kw = team_warps(phase);
+    part = warp & (kw - 1);
+    team = warp / kw * (int)gridDim.x + (int)blockIdx.x;
+    teams = kWarps / kw * (int)gridDim.x;
+  }
+  __device__ __forceinline__ int run0(int phase) const { return (phase ? a.I : a.H) / 64 * part / kw; }
+  __device__ __forceinline__ int run1(int phase) const { return (phase ? a.I : a.H) / 64 * (part + 1) / kw; }
 
   struct Cursor {
     int phase, left;               // phase 2: over; items left in the phase, this one among them
@@ -387,9 +415,10 @@ struct Few {
   __device__ __forceinline__ Cursor begin(int phase) const {
     Cursor c;
     c.phase = phase;
-    const int n = s.passes * tiles(phase) * subs(phase), lo = n / teams * team + min(team, n % teams);
-    c.left = n / teams + (team < n % teams ? 1 : 0);
-    const int inner = phase ? s.passes : tiles(phase), x = lo / subs(phase), o = x / inner;
+    const int n = s.passes * tiles(phase) * subs(phase), each = quotient(n, teams), over = n - each * teams;
+    const int lo = each * team + min(team, over);
+    c.left = each + (team < over ? 1 : 0);
+    const int inner = phase ? s.passes : tiles(phase), x = lo / subs(phase), o = quotient(x, inner);
     c.sub = lo % subs(phase);
     c.q = phase ? x - o * inner : o;
     c.tile = phase ? o : x - o * inner;
@@ -422,12 +451,7 @@ struct Few {
   };
   __device__ __forceinline__ bool more(const Ahead& h) const { return h.c.phase < 2; }
   __device__ __forceinline__ void resolve(Ahead& h) const {
-    // a phase that is over, or in which this warp has no K, is passed over
-    while (h.c.phase < 2 && (h.c.left <= 0 || run0(h.c.phase) == run1(h.c.phase))) {
-      if (h.c.phase == 1) { h.c.phase = 2; return; }
-      h.c = begin(1);
-    }
-    if (h.c.phase == 2) return;
+    if (h.c.left <= 0 || run0(h.c.phase) == run1(h.c.phase)) { h.c.phase = 2; return; }   // nothing (more) to bring in
     const int ph = h.c.phase, e = s.pass_e[h.c.q];
     h.st = 0;
     h.k0 = run0(ph);
@@ -468,8 +492,9 @@ struct Few {
     }
     if (FP8) h.sc = (ph ? a.s2 : a.s13) + (uint64_t)((lane == 0 ? r0 : r1) >> 7) * (K >> 7);
   }
-  __device__ __forceinline__ void copy_weights(const Ahead& h, int slot) const {
-    const uint32_t dst = smem_u32(ring + slot * kStageBytes + lane * 16);
+  // run st of the item into place r of the ring
+  __device__ __forceinline__ void copy_run(const Ahead& h, int r, int64_t plane) const {
+    const uint32_t dst = smem_u32(ring + r * kRunBytes + lane * 16);
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
       copy16(dst + (0 * PER + v) * 512, h.w0 + v * 64);
@@ -477,24 +502,22 @@ struct Few {
       copy16(dst + (2 * PER + v) * 512, h.w1 + v * 64);
       copy16(dst + (3 * PER + v) * 512, h.w1 + h.row8 + v * 64);
     }
-    if (FP8 && lane < 2) copy4(smem_u32(ring + kStages * kStageBytes + slot * 16 + lane * 4), h.sc + ((h.k0 + h.st) >> 1));
-  }
-  // A lane without a token leaves its place as it is: what stands there makes a column nobody reads.
-  __device__ __forceinline__ void copy_tokens(const Ahead& h, int slot, int64_t plane) const {
+    if (FP8 && lane < 2) copy4(smem_u32(ring + kStages * KPS * kRunBytes + r * 8 + lane * 4), h.sc + ((h.k0 + h.st) >> 1));
+    // A lane without a token leaves its place as it is: what stands there makes a column nobody reads.
     if (h.tok == nullptr) return;
-    const uint32_t dst = smem_u32(ring + slot * kStageBytes + W + lane * 16);
     const uint16_t* src = h.tok + h.st * 64;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      copy16(dst + v * 512, src + v * (FP8 ? 8 : 32));
-      if (!FP8 && h.c.phase == 1) copy16(dst + (2 + v) * 512, src + plane + v * 32);
+      copy16(dst + W + v * 512, src + v * (FP8 ? 8 : 32));
+      if (!FP8 && h.c.phase == 1) copy16(dst + W + (2 + v) * 512, src + plane + v * 32);
     }
-    if (FP8 && h.c.phase == 1) copy4(smem_u32(ring + slot * kStageBytes + W + B + lane * 4), h.fac + h.st * 4);
+    if (FP8 && h.c.phase == 1) copy4(smem_u32(ring + r * kRunBytes + W + B + lane * 4), h.fac + h.st * 4);
   }
-  __device__ __forceinline__ void step(Ahead& h) const {
+  // to the next run; true: of the same item
+  __device__ __forceinline__ bool step(Ahead& h) const {
     h.w0 += h.run;
     h.w1 += h.run;
-    if (++h.st < h.runs) return;
+    if (++h.st < h.runs) return true;
     if (next(h.c)) {
       h.st = 0;
       h.w0 += h.block;
@@ -502,79 +525,101 @@ struct Few {
     } else {
       resolve(h);
     }
+    return false;
   }
 
-  // acc[m] += 16 weight rows x 8 tokens of one run of 64 K
+  // acc[m] += 16 weight rows x 8 tokens of a stage's n runs (the products of a missing one are dropped)
   template <int P>
-  __device__ __forceinline__ void multiply(int slot, float (&acc)[2][4]) const {
+  __device__ __forceinline__ void multiply(int slot, int n, float (&acc)[2][4]) const {
     constexpr int PLANES = !FP8 && P == 1 ? 2 : 1;
     const int t = lane & 3;
-    const uint8_t* src = ring + slot * kStageBytes + lane * 16;
-    uint4 b[PLANES][2];
+    uint4 b[KPS][PLANES][2];
+    float sc[KPS][2][2];             // factors of the sums: [row block][column of this lane]
 #pragma unroll
-    for (int p = 0; p < PLANES; ++p)
+    for (int k = 0; k < KPS; ++k) {
+      const int r = slot * KPS + k;
+      const uint8_t* src = ring + r * kRunBytes + lane * 16;
 #pragma unroll
-      for (int v = 0; v < 2; ++v) b[p][v] = *reinterpret_cast<const uint4*>(src + W + (p * 2 + v) * 512);
-    float sc[2][2] = {{1.f, 1.f}, {1.f, 1.f}};   // factors of the sums: [row block][column of this lane]
-    if constexpr (FP8) {
-      const float2 bs = *reinterpret_cast<const float2*>(ring + kStages * kStageBytes + slot * 16);
-      sc[0][0] = sc[0][1] = bs.x;
-      sc[1][0] = sc[1][1] = bs.y;
-      if constexpr (P == 1) {
-        // Each lane of a token holds 16 hidden values with a factor of their own: bring the four to
-        // the largest (a value that vanishes there is below 2^-24 of the others' largest).
-        const float f = *reinterpret_cast<const float*>(ring + slot * kStageBytes + W + B + lane * 4);
-        float m = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int d = (int)(__float_as_uint(f) >> 23) - (int)(__float_as_uint(m) >> 23);   // <= 0
-        const __half2 r = __float2half2_rn(d < -30 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23));
+      for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          __half2* x = reinterpret_cast<__half2*>(&b[0][v]);
+        for (int v = 0; v < 2; ++v) b[k][p][v] = *reinterpret_cast<const uint4*>(src + W + (p * 2 + v) * 512);
+      if constexpr (FP8) {
+        const float2 bs = *reinterpret_cast<const float2*>(ring + kStages * KPS * kRunBytes + r * 8);
+        sc[k][0][0] = sc[k][0][1] = bs.x;
+        sc[k][1][0] = sc[k][1][1] = bs.y;
+        if constexpr (P == 1) {
+          // Each lane of a token holds 16 hidden values with a factor of their own: bring the four to
+          // the largest (a value that vanishes there is below 2^-24 of the others' largest).
+          const float f = *reinterpret_cast<const float*>(ring + r * kRunBytes + W + B + lane * 4);
+          float m = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const int d = (int)(__float_as_uint(f) >> 23) - (int)(__float_as_uint(m) >> 23);   // <= 0
+          const __half2 h = __float2half2_rn(d < -30 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], r);
-        }
-        const float top0 = __shfl_sync(0xffffffffu, m, t * 8), top1 = __shfl_sync(0xffffffffu, m, t * 8 + 4);
+          for (int v = 0; v < 2; ++v) {
+            __half2* x = reinterpret_cast<__half2*>(&b[k][0][v]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          sc[i][0] *= top0;
-          sc[i][1] *= top1;
+            for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], h);
+          }
+          const float top0 = __shfl_sync(0xffffffffu, m, t * 8), top1 = __shfl_sync(0xffffffffu, m, t * 8 + 4);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sc[k][i][0] *= top0;
+            sc[k][i][1] *= top1;
+          }
         }
       }
     }
+    float sum[KPS][2][4];
+#pragma unroll
+    for (int k = 0; k < KPS; ++k)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[k][m][i] = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint4 w[2][PER];               // rows g and g + 8: 16 weights
+      uint4 w[KPS][2][PER];          // rows g and g + 8: 16 weights
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int k = 0; k < KPS; ++k)
 #pragma unroll
-        for (int v = 0; v < PER; ++v) w[r][v] = *reinterpret_cast<const uint4*>(src + ((m * 2 + r) * PER + v) * 512);
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {   // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
-        uint32_t af[4];
+          for (int v = 0; v < PER; ++v)
+            w[k][r][v] = *reinterpret_cast<const uint4*>(ring + (slot * KPS + k) * kRunBytes + lane * 16 + ((m * 2 + r) * PER + v) * 512);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if constexpr (FP8) {
-            const uint4& y = w[r][0];
-            const uint32_t x = q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w;
-            af[r] = f16x2_of(x & 0xffffu);
-            af[r + 2] = f16x2_of(x >> 16);
-          } else {
-            const uint4& x = w[r][q >> 1];
-            af[r] = q & 1 ? x.z : x.x;
-            af[r + 2] = q & 1 ? x.w : x.y;
+      for (int q = 0; q < 4; ++q)     // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
+#pragma unroll
+        for (int k = 0; k < KPS; ++k) {
+          uint32_t af[4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (FP8) {
+              const uint4& y = w[k][r][0];
+              const uint32_t x = q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w;
+              af[r] = f16x2_of(x & 0xffffu);
+              af[r + 2] = f16x2_of(x >> 16);
+            } else {
+              const uint4& x = w[k][r][q >> 1];
+              af[r] = q & 1 ? x.z : x.x;
+              af[r + 2] = q & 1 ? x.w : x.y;
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p) {
+            const uint4& x = b[k][p][q >> 1];
+            if constexpr (FP8) mma_f16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
+            else mma_bf16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
           }
         }
+    }
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-          const uint4& x = b[p][q >> 1];
-          if constexpr (FP8) mma_f16(sum, af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
-          else mma_bf16(sum, af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
-        }
-      }
+    for (int k = 0; k < KPS; ++k) {
+      if (k >= n) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][i] = FP8 ? fmaf(sum[i], sc[m][i & 1], acc[m][i]) : acc[m][i] + sum[i];
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][i] = FP8 ? fmaf(sum[k][m][i], sc[k][m][i & 1], acc[m][i]) : acc[m][i] + sum[k][m][i];
     }
   }
 };
@@ -583,10 +628,9 @@ template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
 moe_few_kernel(const MoeFewArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int last_s[kTeams];
+  __shared__ int last_s[kWarps];
   Shared& s = *reinterpret_cast<Shared*>(smem + kShared);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int team_in = warp / kTeam, tt = threadIdx.x % (kTeam * 32);
   cg::grid_group grid = cg::this_grid();
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.H / 128; i += kThreads) a.done[i] = 0;
@@ -596,108 +640,100 @@ moe_few_kernel(const MoeFewArgs a) {
   if (a.E <= 128) few_route<4>(a, s, grid);
   else few_route<kFewMaxExperts / 32>(a, s, grid);
 
-  Few<FP8> few{a, s, smem + warp * kRingBytes, lane, warp % kTeam,
-               team_in * (int)gridDim.x + (int)blockIdx.x, kTeams * (int)gridDim.x};
+  Few<FP8> few{a, s, smem + warp * kRingBytes, lane};
   using Cursor = typename Few<FP8>::Cursor;
   using Ahead = typename Few<FP8>::Ahead;
-  constexpr int kStages = Few<FP8>::kStages;
-  float* red = reinterpret_cast<float*>(smem + kRed) + team_in * (kTeam * 256);   // [kTeam][8][32]
+  constexpr int kStages = Few<FP8>::kStages, KPS = Few<FP8>::KPS;
   uint16_t* hid = static_cast<uint16_t*>(a.h);
   const int64_t hplane = (int64_t)a.T * a.topk * a.I;
 
   Ahead ahead{};
-  ahead.c = few.begin(0);
-  few.resolve(ahead);
-  int slot = 0;                    // the ring's next stage
-  int early = 0;                   // stages of phase 1 brought in without their tokens, in front of the barrier
-  bool hidden_done = false;
-  auto issue = [&](int to) {       // the next run into the ring; an empty group behind the last one
-    if (few.more(ahead)) {
-      few.copy_weights(ahead, to);
-      if (ahead.c.phase == 0 || hidden_done) few.copy_tokens(ahead, to, hplane);
-      else ++early;
-      few.step(ahead);
-    }
-    copies_commit();
-  };
-  for (int i = 0; i < kStages; ++i) issue(i);
-
   auto run_phase = [&](auto phase_c) {
     constexpr int P = decltype(phase_c)::value;
-    if (P == 1) {
-      // the tokens of the stages that came in early
-      hidden_done = true;
-      Ahead late{};
-      late.c = few.begin(1);
-      if (early > 0) few.resolve(late);
-      for (int i = 0; i < early; ++i) {
-        few.copy_tokens(late, (slot + i) % kStages, hplane);
-        few.step(late);
-      }
-      copies_commit();
-      copies_wait<0>();
-    }
-    const int runs = few.run1(P) - few.run0(P);
+    few.enter(P, warp);
+    const int kw = few.kw, team_in = warp / kw, tt = threadIdx.x & (kw * 32 - 1);
+    float* red = reinterpret_cast<float*>(smem + kRed) + team_in * kw * 256;   // [kw][8][32]
     Cursor at = few.begin(P);
+    ahead.c = at;
+    few.resolve(ahead);
+    const int runs = few.run1(P) - few.run0(P), stages = (runs + KPS - 1) / KPS;
+    int slot = 0;                                // the ring's next stage
+    int fill = kStages;                          // stages to bring in before the first is used
     int summed = 0;                              // items of the tile that this team has finished
+#pragma unroll 1
     while (at.left > 0) {
       const int first = s.pass_first[at.q], cnt = s.pass_cnt[at.q];
       const int col = at.tile * 128 + at.sub * (P ? 32 : 16);
       float acc[2][4] = {};
 #pragma unroll 1
-      for (int k = 0; k < runs; ++k) {
-        copies_wait<kStages - 1>();
-        __syncwarp();                            // the scales come in through two lanes
-        few.template multiply<P>(slot, acc);
-        __syncwarp();
-        issue(slot);
-        slot = slot + 1 == kStages ? 0 : slot + 1;
+      for (int k = -fill; k < stages; ++k) {
+        if (k >= 0) {
+          copies_wait<kStages - 1>();
+          __syncwarp();                          // the scales come in through two lanes
+          few.template multiply<P>(slot, runs - k * KPS, acc);
+          __syncwarp();
+        }
+        if (few.more(ahead)) {                   // the next runs; an empty group behind the last
+          few.copy_run(ahead, slot * KPS, hplane);
+          if (few.step(ahead) && KPS > 1) {
+            few.copy_run(ahead, slot * KPS + KPS - 1, hplane);
+            few.step(ahead);
+          }
+        }
+        copies_commit();
+        slot ^= 1;
       }
-      // the quarters of K, added in order
-      named_barrier_sync(1 + team_in, kTeam * 32);    // the last sums have been read
+      fill = 0;
+      // the parts of K, added in order
+      auto team_sync = [&]() {
+        if (kw == 1) __syncwarp();
+        else named_barrier_sync(1 + team_in, kw * 32);
+      };
+      team_sync();                               // the last sums have been read
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[(warp % kTeam) * 256 + (m * 4 + i) * 32 + lane] = acc[m][i];
-      named_barrier_sync(1 + team_in, kTeam * 32);
-      // thread = (token, row): the 16 rows of a token side by side
-      const int n = tt >> 4, row = tt & 15;
-      const int ri = (row >> 3) * 2 + (n & 1), rl = (row & 7) * 4 + (n >> 1);
-      float v[2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        v[m] = 0.f;
-#pragma unroll
-        for (int q = 0; q < kTeam; ++q) v[m] += red[q * 256 + (m * 4 + ri) * 32 + rl];
-      }
-      const int p = n < cnt ? s.pair[first + n] : -1;
-      if constexpr (P == 0) {
-        if (FP8 && p >= 0) {
-          const float f = a.x_factor[s.token[first + n]];
-          v[0] *= f;
-          v[1] *= f;
+        for (int i = 0; i < 4; ++i) red[few.part * 256 + (m * 4 + i) * 32 + lane] = acc[m][i];
+      team_sync();
+#pragma unroll 1
+      for (int idx = tt; idx < 128; idx += kw * 32) {
+        // (token, row): the 16 rows of a token side by side
+        const int n = idx >> 4, row = idx & 15;
+        if (n >= cnt) break;                     // all of a half-warp
+        const int ri = (row >> 3) * 2 + (n & 1), rl = (row & 7) * 4 + (n >> 1);
+        float v[2] = {0.f, 0.f};
+        for (int q = 0; q < kw; ++q) {
+          v[0] += red[q * 256 + ri * 32 + rl];
+          v[1] += red[q * 256 + (4 + ri) * 32 + rl];
         }
-        const float hv = v[0] / (1.f + expf(-v[0])) * v[1];
-        if constexpr (FP8) {
-          uint32_t top = __float_as_uint(hv) & 0x7fffffffu;   // NaN and infinity are above every number
-#pragma unroll
-          for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float f = factor_of(__uint_as_float(top));
-          if (p >= 0) {
-            reinterpret_cast<__half*>(hid)[(int64_t)p * a.I + col + row] = __float2half_rn(hv * (1.f / f));
-            if (row == 0) a.h_factor[(int64_t)p * (a.I / 16) + (col >> 4)] = f;
+        const int p = s.pair[first + n];
+        if constexpr (P == 0) {
+          if (FP8) {
+            const float f = a.x_factor[s.token[first + n]];
+            v[0] *= f;
+            v[1] *= f;
           }
-        } else if (p >= 0) {
-          const bf16 top = __float2bfloat16(hv);
-          bf16* dst = reinterpret_cast<bf16*>(hid) + (int64_t)p * a.I + col + row;
-          dst[0] = top;
-          dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
+          const float hv = v[0] / (1.f + expf(-v[0])) * v[1];
+          if constexpr (FP8) {
+            const unsigned half = 0xffffu << (lane & 16);
+            uint32_t top = __float_as_uint(hv) & 0x7fffffffu;   // NaN and infinity are above every number
+            top = __reduce_max_sync(half, top);
+            const float f = factor_of(__uint_as_float(top));
+            reinterpret_cast<__half*>(hid)[p * a.I + col + row] = __float2half_rn(hv * (1.f / f));
+            if (row == 0) a.h_factor[p * (a.I / 16) + (col >> 4)] = f;
+          } else {
+            const bf16 top = __float2bfloat16(hv);
+            bf16* dst = reinterpret_cast<bf16*>(hid) + p * a.I + col + row;
+            dst[0] = top;
+            dst[hplane] = __float2bfloat16(hv - __bfloat162float(top));
+          }
+        } else {
+          float* dst = a.slots + (int64_t)p * a.H + col + row;
+          dst[0] = v[0];
+          dst[16] = v[1];
         }
-      } else if (p >= 0) {
-        float* dst = a.slots + (int64_t)p * a.H + col + row;
-        dst[0] = v[0];
-        dst[16] = v[1];
       }
+      __syncwarp();
       const int tile = at.tile;
       few.next(at);
       if constexpr (P == 1) {
@@ -706,14 +742,14 @@ moe_few_kernel(const MoeFewArgs a) {
           // Items of a tile are counted when a team leaves it; the team that brings the last ones
           // adds the slots of every token.
           __threadfence();
-          named_barrier_sync(1 + team_in, kTeam * 32);
+          team_sync();
           if (tt == 0) last_s[team_in] = atomicAdd(&a.done[tile], summed) + summed == s.passes * 4;
-          named_barrier_sync(1 + team_in, kTeam * 32);
+          team_sync();
           summed = 0;
           if (last_s[team_in]) {
             __threadfence();
             const int c = tile * 128 + (tt & 31) * 4;
-            for (int t = tt >> 5; t < a.T; t += kTeam) {
+            for (int t = tt >> 5; t < a.T; t += kw) {
               float4 v[kFewMaxTopk];
 #pragma unroll
               for (int k = 0; k < kFewMaxTopk; ++k)
@@ -741,6 +777,7 @@ moe_few_kernel(const MoeFewArgs a) {
   };
   run_phase(std::integral_constant<int, 0>{});
   grid.sync();
+  copies_wait<0>();
   run_phase(std::integral_constant<int, 1>{});
 }
 
