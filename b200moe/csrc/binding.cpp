@@ -932,7 +932,7 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
                   (*t)->scalar_type() == (t == &ids ? torch::kInt32 : torch::kFloat32),
                   "ids (int32) and weights (fp32) must be [tokens, topk]");
   c10::cuda::CUDAGuard guard(x.device());
-  // [slots | hidden rows | their factors | x as f16 | logits | x factors | selection | counters], floats
+  // [slots | hidden rows | their factors | x in e4m3 | logits | x factors | selection | counters], floats
   const int64_t P = T * topk, at_h = P * H, at_hf = at_h + P * I, at_x = at_hf + P * (I / 16), at_l = at_x + T * H / 2,
                 at_xf = at_l + (T * E + 3) / 4 * 4, at_sel = at_xf + (T + 3) / 4 * 4,
                 at_done = at_sel + 2 * P;
@@ -954,7 +954,7 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
   a.slots = w;
   a.h = w + at_h;
   a.h_factor = w + at_hf;
-  a.x16 = w + at_x;
+  a.x8 = w + at_x;
   a.logits = w + at_l;
   a.x_factor = w + at_xf;
   a.sel = reinterpret_cast<int2*>(w + at_sel);

@@ -24,7 +24,7 @@ struct MoeFewArgs {
   float* weights;            // [T, topk] their weights, may be null
   // workspace, 16-byte aligned
   float* logits;             // [T, E]
-  void* x16;                 // e4m3 weights: [T, H] f16, x / x_factor
+  void* x8;                  // e4m3 weights: [T, 2, H] e4m3, the two terms of x / x_factor
   float* x_factor;           // [T]
   void* h;                   // [T * topk, I] f16, h / h_factor (e4m3 weights), or [2, T * topk, I] bf16
   float* h_factor;           // [T * topk, I / 16]

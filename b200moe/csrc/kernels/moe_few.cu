@@ -20,13 +20,14 @@
 // tokens as columns.  K is permuted alike in both operands so that a lane's operand is 16
 // weights of a row.
 //
-// Operand types.  e4m3 converts to f16 exactly in one instruction for two values (bf16
-// would take four), so the tokens enter as f16 too: each row of x times the power of
-// two that brings its largest value to [2^14, 2^15), which keeps every bit of a bf16
-// value down to 2^-28 of the row's largest, and hidden values with such a factor for
-// each 16 of them (11 bits of each value).  The factors and the block scale multiply
-// fp32 sums of 64 products, so a weight counts as exactly q * scale.  With bf16
-// weights x enters as it is and a hidden value as two bf16, value and rest.
+// Operand types, e4m3 weights.  The first product takes them as they are.  A bf16 value has 8 significant
+// bits and an e4m3 value 4, so a token enters as two e4m3 terms: x / f = hi + lo / 16 with f the power of
+// two that brings the row's largest value to [2^7, 2^8).  That is exact down to 2^-14 of the largest value
+// and off by at most 2^-21 of it below.  (f16 operands would need a conversion of every weight, which cost
+// more instructions than all the rest of the loop.)  Hidden values keep 11 bits: f16 with a factor for
+// each 16 of them, against weights converted to f16 exactly.  Factors and block scales multiply fp32 sums
+// of 64 products, so a weight counts as exactly q * scale.  bf16 weights meet x as it is and a hidden
+// value as two bf16, value and rest.
 //
 // The parts of K are added in order through shared memory.  The rows of Wd write fp32 (token, k) slots, and the team that finishes the last expert of
 // a block of 32 columns adds the token's slots in the order of the top-k.
@@ -58,6 +59,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRingBytes = 12832;        // of a warp
 constexpr int kCols = 8;                 // tokens of one pass
+constexpr int kLastAdds = 2;             // tokens up to which the last team of a tile adds the slots
 
 // fp64 -> bf16 in one rounding: fp32 with round-to-odd keeps the bit that decides a tie.
 __device__ __forceinline__ float bf16_of(double v) {
@@ -109,7 +111,7 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
       const bf16* xr = static_cast<const bf16*>(a.x) + t * a.H;
       const bf16* wr = static_cast<const bf16*>(a.router) + e0 * a.H;   // the last rows are repeated below
       double acc[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 2
+#pragma unroll 4
       for (int c = lane * 8; c < a.H; c += 256) {
         const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
 #pragma unroll
@@ -157,14 +159,14 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
   }
 }
 
-// The power of two f with |v| / f in [2^14, 2^15) for the largest |v| = top of a row; 1 where top
-// is not finite, the smallest normal number where it is zero or tiny.
-__device__ __forceinline__ float factor_of(float top) {
-  const int e = (int)(__float_as_uint(top) >> 23);   // biased exponent, sign is 0
-  return e == 255 ? 1.f : __uint_as_float((uint32_t)max(e - 14, 1) << 23);
+// The power of two f with |v| / f in [2^top, 2^(top + 1)) for the largest |v| = m of a row; 1 where m is
+// not finite, the smallest normal number where it is zero or tiny.
+__device__ __forceinline__ float factor_of(float m, int top) {
+  const int e = (int)(__float_as_uint(m) >> 23);   // biased exponent, sign is 0
+  return e == 255 ? 1.f : __uint_as_float((uint32_t)max(e - top, 1) << 23);
 }
 
-// f16 rows of x and their factors: row t by CTA gridDim.x - 1 - t.
+// The two e4m3 terms of x and the rows' factors: row t by CTA gridDim.x - 1 - t.
 __device__ void few_rows(const MoeFewArgs& a, float* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int t = gridDim.x - 1 - blockIdx.x; t < a.T; t += gridDim.x) {
@@ -180,10 +182,16 @@ __device__ void few_rows(const MoeFewArgs& a, float* red) {
     top = 0;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) top = max(top, __float_as_uint(red[i]));
-    const float f = factor_of(__uint_as_float(top)), inv = 1.f / f;   // a power of two: exact
+    const float f = factor_of(__uint_as_float(top), 7), inv = 1.f / f;   // a power of two: exact
+    uint16_t* hi = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.x8) + (int64_t)t * 2 * a.H);
     for (int c = threadIdx.x * 2; c < a.H; c += kThreads * 2) {
       const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(xr + c));
-      *reinterpret_cast<__half2*>(static_cast<__half*>(a.x16) + (int64_t)t * a.H + c) = __floats2half2_rn(v.x * inv, v.y * inv);
+      const float2 w = make_float2(v.x * inv, v.y * inv);
+      const uint16_t h = __nv_cvt_float2_to_fp8x2(w, __NV_NOSAT, __NV_E4M3);
+      const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3);
+      const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+      hi[c / 2] = h;
+      hi[(c + a.H) / 2] = __nv_cvt_float2_to_fp8x2(make_float2((w.x - back.x) * 16.f, (w.y - back.y) * 16.f), __NV_NOSAT, __NV_E4M3);
     }
     if (threadIdx.x == 0) a.x_factor[t] = f;
     __syncthreads();
@@ -265,24 +273,24 @@ __device__ void few_route(const MoeFewArgs& a, Shared& s, cg::grid_group& grid) 
     grid.sync();
   }
   __syncthreads();
-  for (int t = warp; t < a.T; t += kWarps) {
-    int pick = 0;
-    float w = 0.f;
-    if (spread) {
-      if (lane < a.topk) {
-        const int2 x = __ldcg(a.sel + t * a.topk + lane);
-        pick = x.x;
-        w = __int_as_float(x.y);
-      }
-    } else {
-      few_topk<EPL>(a, t, lane, pick, w);
+  auto take = [&](int t, int p, int pick, float w) {
+    s.sel_e[p] = (uint8_t)pick;
+    s.sel_w[p] = w;
+    atomicOr(&s.mask[t >> 5][pick], 1u << (t & 31));
+  };
+  if (spread) {
+    for (int p = threadIdx.x; p < a.T * a.topk; p += kThreads) {
+      const int2 x = __ldcg(a.sel + p);
+      take(quotient(p, a.topk), p, x.x, __int_as_float(x.y));
     }
+  } else if (warp < a.T) {
+    int pick;
+    float w;
+    few_topk<EPL>(a, warp, lane, pick, w);
     if (lane < a.topk) {
-      const int p = t * a.topk + lane;
-      s.sel_e[p] = (uint8_t)pick;
-      s.sel_w[p] = w;
-      atomicOr(&s.mask[t >> 5][pick], 1u << (t & 31));
-      if (!spread && blockIdx.x == 0) {
+      const int p = warp * a.topk + lane;
+      take(warp, p, pick, w);
+      if (blockIdx.x == 0) {
         if (a.ids != nullptr) a.ids[p] = pick;
         if (a.weights != nullptr) a.weights[p] = w;
       }
@@ -353,6 +361,13 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                "{%0,%1,%2,%3};"
@@ -444,7 +459,8 @@ struct Few {
     const uint8_t* w0;             // this lane's weights of rows g of the two row blocks, run st
     const uint8_t* w1;
     int row8, run, block;          // bytes from row g to row g + 8, to the next run, to the next block
-    const uint16_t* tok;           // this lane's token or hidden row; null: none
+    const uint8_t* tok;            // this lane's token or hidden row; null: none
+    int tok_run, tok_piece;        // bytes to the next run, and between its two pieces of a run
     const float* fac;              // its factors
     const float* sc;               // lanes 0 and 1: block scales of a row block
     int k0;
@@ -485,9 +501,17 @@ struct Few {
     h.tok = nullptr;
     if (g < s.pass_cnt[h.c.q]) {
       const int at = s.pass_first[h.c.q] + g;
-      h.tok = ph == 0 ? static_cast<const uint16_t*>(FP8 ? a.x16 : a.x) + s.token[at] * a.H
-                      : static_cast<const uint16_t*>(a.h) + s.pair[at] * a.I;
-      h.tok += h.k0 * 64 + t * (FP8 ? 16 : 8);
+      if (FP8 && ph == 0) {          // two terms of 16 values
+        h.tok = static_cast<const uint8_t*>(a.x8) + s.token[at] * 2 * a.H + h.k0 * 64 + t * 16;
+        h.tok_run = 64;
+        h.tok_piece = a.H;
+      } else {                       // 16 values of two bytes
+        h.tok = ph == 0 ? static_cast<const uint8_t*>(a.x) + s.token[at] * a.H * 2
+                        : static_cast<const uint8_t*>(a.h) + s.pair[at] * a.I * 2;
+        h.tok += h.k0 * 128 + t * (FP8 ? 32 : 16);
+        h.tok_run = 128;
+        h.tok_piece = FP8 ? 16 : 64;
+      }
       if (FP8) h.fac = a.h_factor + s.pair[at] * (a.I / 16) + h.k0 * 4 + t;
     }
     if (FP8) h.sc = (ph ? a.s2 : a.s13) + (uint64_t)((lane == 0 ? r0 : r1) >> 7) * (K >> 7);
@@ -505,11 +529,11 @@ struct Few {
     if (FP8 && lane < 2) copy4(smem_u32(ring + kStages * KPS * kRunBytes + r * 8 + lane * 4), h.sc + ((h.k0 + h.st) >> 1));
     // A lane without a token leaves its place as it is: what stands there makes a column nobody reads.
     if (h.tok == nullptr) return;
-    const uint16_t* src = h.tok + h.st * 64;
+    const uint8_t* src = h.tok + h.st * h.tok_run;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      copy16(dst + W + v * 512, src + v * (FP8 ? 8 : 32));
-      if (!FP8 && h.c.phase == 1) copy16(dst + W + (2 + v) * 512, src + plane + v * 32);
+      copy16(dst + W + v * 512, src + v * h.tok_piece);
+      if (!FP8 && h.c.phase == 1) copy16(dst + W + (2 + v) * 512, src + plane * 2 + v * 64);
     }
     if (FP8 && h.c.phase == 1) copy4(smem_u32(ring + r * kRunBytes + W + B + lane * 4), h.fac + h.st * 4);
   }
@@ -570,13 +594,17 @@ struct Few {
         }
       }
     }
-    float sum[KPS][2][4];
+    constexpr bool E4 = FP8 && P == 0;
+    float sum[KPS][2][4], low[E4 ? KPS : 1][2][4];
 #pragma unroll
     for (int k = 0; k < KPS; ++k)
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[k][m][i] = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          sum[k][m][i] = 0.f;
+          if constexpr (E4) low[k][m][i] = 0.f;
+        }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       uint4 w[KPS][2][PER];          // rows g and g + 8: 16 weights
@@ -587,31 +615,42 @@ struct Few {
 #pragma unroll
           for (int v = 0; v < PER; ++v)
             w[k][r][v] = *reinterpret_cast<const uint4*>(ring + (slot * KPS + k) * kRunBytes + lane * 16 + ((m * 2 + r) * PER + v) * 512);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)     // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
+      if constexpr (E4) {             // 32 of the 64 K at a time: two words of each lane's 16 weights
 #pragma unroll
         for (int k = 0; k < KPS; ++k) {
-          uint32_t af[4];
+          const uint4 &lo = w[k][0][0], &hi = w[k][1][0], &bh = b[k][0][0], &bl = b[k][0][1];
+          mma_e4m3(sum[k][m], lo.x, hi.x, lo.y, hi.y, bh.x, bh.y);
+          mma_e4m3(low[k][m], lo.x, hi.x, lo.y, hi.y, bl.x, bl.y);
+          mma_e4m3(sum[k][m], lo.z, hi.z, lo.w, hi.w, bh.z, bh.w);
+          mma_e4m3(low[k][m], lo.z, hi.z, lo.w, hi.w, bl.z, bl.w);
+        }
+      } else {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if constexpr (FP8) {
-              const uint4& y = w[k][r][0];
-              const uint32_t x = q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w;
-              af[r] = f16x2_of(x & 0xffffu);
-              af[r + 2] = f16x2_of(x >> 16);
-            } else {
-              const uint4& x = w[k][r][q >> 1];
-              af[r] = q & 1 ? x.z : x.x;
-              af[r + 2] = q & 1 ? x.w : x.y;
+        for (int q = 0; q < 4; ++q)     // 16 of the 64 K: weights 4 q .. 4 q + 3 of each lane's 16
+#pragma unroll
+          for (int k = 0; k < KPS; ++k) {
+            uint32_t af[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if constexpr (FP8) {
+                const uint4& y = w[k][r][0];
+                const uint32_t x = q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w;
+                af[r] = f16x2_of(x & 0xffffu);
+                af[r + 2] = f16x2_of(x >> 16);
+              } else {
+                const uint4& x = w[k][r][q >> 1];
+                af[r] = q & 1 ? x.z : x.x;
+                af[r + 2] = q & 1 ? x.w : x.y;
+              }
+            }
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+              const uint4& x = b[k][p][q >> 1];
+              if constexpr (FP8) mma_f16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
+              else mma_bf16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
             }
           }
-#pragma unroll
-          for (int p = 0; p < PLANES; ++p) {
-            const uint4& x = b[k][p][q >> 1];
-            if constexpr (FP8) mma_f16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
-            else mma_bf16(sum[k][m], af, q & 1 ? x.z : x.x, q & 1 ? x.w : x.y);
-          }
-        }
+      }
     }
 #pragma unroll
     for (int k = 0; k < KPS; ++k) {
@@ -619,10 +658,37 @@ struct Few {
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] = FP8 ? fmaf(sum[k][m][i], sc[k][m][i & 1], acc[m][i]) : acc[m][i] + sum[k][m][i];
+        for (int i = 0; i < 4; ++i) {
+          float v = sum[k][m][i];
+          if constexpr (E4) v = fmaf(low[k][m][i], 0.0625f, v);
+          acc[m][i] = FP8 ? fmaf(v, sc[k][m][i & 1], acc[m][i]) : acc[m][i] + v;
+        }
     }
   }
 };
+
+// out[t, c .. c + 3]: the token's slots in the order of the top-k
+__device__ __forceinline__ void few_add(const MoeFewArgs& a, const Shared& s, int t, int c) {
+  float4 v[kFewMaxTopk];
+#pragma unroll
+  for (int k = 0; k < kFewMaxTopk; ++k)
+    if (k < a.topk) v[k] = __ldcg(reinterpret_cast<const float4*>(a.slots + (int64_t)(t * a.topk + k) * a.H + c));
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kFewMaxTopk; ++k)
+    if (k < a.topk) {
+      const float w = s.sel_w[t * a.topk + k];
+      y.x = fmaf(v[k].x, w, y.x);
+      y.y = fmaf(v[k].y, w, y.y);
+      y.z = fmaf(v[k].z, w, y.z);
+      y.w = fmaf(v[k].w, w, y.w);
+    }
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(y.x, y.y), hi = __floats2bfloat162_rn(y.z, y.w);
+  uint2 o;
+  o.x = *reinterpret_cast<const uint32_t*>(&lo);
+  o.y = *reinterpret_cast<const uint32_t*>(&hi);
+  *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + (int64_t)t * a.H + c) = o;
+}
 
 template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -646,6 +712,10 @@ moe_few_kernel(const MoeFewArgs a) {
   constexpr int kStages = Few<FP8>::kStages, KPS = Few<FP8>::KPS;
   uint16_t* hid = static_cast<uint16_t*>(a.h);
   const int64_t hplane = (int64_t)a.T * a.topk * a.I;
+
+  // One barrier more spreads the last sums over the grid; with a few tokens the team that brings the
+  // last product of a tile is sooner done with them.
+  const bool last_adds = a.T <= kLastAdds;
 
   Ahead ahead{};
   auto run_phase = [&](auto phase_c) {
@@ -718,7 +788,7 @@ moe_few_kernel(const MoeFewArgs a) {
             const unsigned half = 0xffffu << (lane & 16);
             uint32_t top = __float_as_uint(hv) & 0x7fffffffu;   // NaN and infinity are above every number
             top = __reduce_max_sync(half, top);
-            const float f = factor_of(__uint_as_float(top));
+            const float f = factor_of(__uint_as_float(top), 14);
             reinterpret_cast<__half*>(hid)[p * a.I + col + row] = __float2half_rn(hv * (1.f / f));
             if (row == 0) a.h_factor[p * (a.I / 16) + (col >> 4)] = f;
           } else {
@@ -738,9 +808,9 @@ moe_few_kernel(const MoeFewArgs a) {
       few.next(at);
       if constexpr (P == 1) {
         ++summed;
-        if (at.left == 0 || at.tile != tile) {
+        if (last_adds && (at.left == 0 || at.tile != tile)) {
           // Items of a tile are counted when a team leaves it; the team that brings the last ones
-          // adds the slots of every token.
+          // adds the slots of its columns.
           __threadfence();
           team_sync();
           if (tt == 0) last_s[team_in] = atomicAdd(&a.done[tile], summed) + summed == s.passes * 4;
@@ -748,28 +818,7 @@ moe_few_kernel(const MoeFewArgs a) {
           summed = 0;
           if (last_s[team_in]) {
             __threadfence();
-            const int c = tile * 128 + (tt & 31) * 4;
-            for (int t = tt >> 5; t < a.T; t += kw) {
-              float4 v[kFewMaxTopk];
-#pragma unroll
-              for (int k = 0; k < kFewMaxTopk; ++k)
-                if (k < a.topk) v[k] = __ldcg(reinterpret_cast<const float4*>(a.slots + (int64_t)(t * a.topk + k) * a.H + c));
-              float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-              for (int k = 0; k < kFewMaxTopk; ++k)
-                if (k < a.topk) {
-                  const float w = s.sel_w[t * a.topk + k];
-                  y.x = fmaf(v[k].x, w, y.x);
-                  y.y = fmaf(v[k].y, w, y.y);
-                  y.z = fmaf(v[k].z, w, y.z);
-                  y.w = fmaf(v[k].w, w, y.w);
-                }
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(y.x, y.y), hi = __floats2bfloat162_rn(y.z, y.w);
-              uint2 o;
-              o.x = *reinterpret_cast<const uint32_t*>(&lo);
-              o.y = *reinterpret_cast<const uint32_t*>(&hi);
-              *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + (int64_t)t * a.H + c) = o;
-            }
+            for (int t = tt >> 5; t < a.T; t += kw) few_add(a, s, t, tile * 128 + (tt & 31) * 4);
           }
         }
       }
@@ -779,6 +828,13 @@ moe_few_kernel(const MoeFewArgs a) {
   grid.sync();
   copies_wait<0>();
   run_phase(std::integral_constant<int, 1>{});
+  if (!last_adds) {
+    grid.sync();
+    for (int i = blockIdx.x + gridDim.x * warp; i < a.T * (a.H >> 7); i += gridDim.x * kWarps) {
+      const int t = quotient(i, a.H >> 7);
+      few_add(a, s, t, (i - t * (a.H >> 7)) * 128 + lane * 4);
+    }
+  }
 }
 
 template <bool FP8>
