@@ -62,6 +62,7 @@ constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
 constexpr int kCutTiles = 4;
+constexpr int kParts = 4;         // partial results in flight per lane when parts are joined
 constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
 template <int D>
@@ -189,8 +190,9 @@ __device__ __forceinline__ float ex2(float x) {
 // (one chunk where the sequence is shorter), so a CTA's share never holds a chunk strictly inside.
 struct Chunks {
   int n, nt;
-  __device__ __forceinline__ int start(int i) const { return (int)((int64_t)i * nt / n); }
-  __device__ __forceinline__ int of(int tile) const { return (int)(((int64_t)(tile + 1) * n - 1) / nt); }
+  // (n is at most the grid, and nt * n below 2^32: the host has checked the number of units)
+  __device__ __forceinline__ int start(int i) const { return n == 1 ? i * nt : (int)((uint32_t)i * (uint32_t)nt / (uint32_t)n); }
+  __device__ __forceinline__ int of(int tile) const { return (int)(((uint32_t)(tile + 1) * (uint32_t)n - 1) / (uint32_t)nt); }
 };
 
 // Per sequence, in shared memory.
@@ -894,10 +896,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   if (plan.whole) return;
   cg::this_grid().sync();
   const int nq = a.num_kv_heads * G, qrows = a.rows * G, groups = (qrows + 31) / 32;
-  const int64_t tasks = (int64_t)groups * a.num_kv_heads * (D / 16);
-  for (int64_t it = blockIdx.x + (int64_t)gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
-    const int c4 = (int)(it % (D / 16)) * 4, h = (int)(it / (D / 16) % a.num_kv_heads);
-    const int qr = (int)(it / (D / 16) / a.num_kv_heads) * 32 + lane;
+  const int tasks = groups * a.num_kv_heads * (D / 16);
+  for (int it = blockIdx.x + gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
+    const int c4 = it % (D / 16) * 4, x = it / (D / 16), h = x % a.num_kv_heads;
+    const int qr = x / a.num_kv_heads * 32 + lane;
     if (qr >= qrows) continue;
     const int row = qr / G, hg = qr % G;
     int lo = 0, up = a.batch;
@@ -923,34 +925,40 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const int u0 = unit0 + (h * nt + start) * pr + pair * clen;
       const int x0 = plan.cta(u0), x1 = plan.cta(u0 + clen - 1);
       if (c.n == 1 && x0 == x1) { whole = true; break; }
-      for (int x = x0; x <= x1; x += 2) {
-        float2 ml[2];
-        float4 v[2][4];
+      for (int x = x0; x <= x1; x += kParts) {
+        float2 ml[kParts];
+        float4 v[kParts][4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kParts; ++k) {
           ml[k] = make_float2(-INFINITY, 0.f);
           if (x + k > x1) continue;
-          const int64_t pblk = (x + k) * 2 + (plan.lo(x + k) >= u0 ? 0 : 1);
+          const int pblk = (x + k) * 2 + (plan.lo(x + k) >= u0 ? 0 : 1);
           ml[k] = __ldcg(t.part_ml + pblk * t.part_rows + prow);
-          const float4* po = reinterpret_cast<const float4*>(t.part_o) + (pblk * (D / 4) + c4) * t.part_rows + prow;
+          const float4* po = reinterpret_cast<const float4*>(t.part_o) + ((int64_t)pblk * (D / 4) + c4) * t.part_rows + prow;
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[k][e] = __ldcg(po + e * t.part_rows);
         }
+        float mt = top;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kParts; ++k) mt = fmaxf(mt, ml[k].x);
+        const float fa = top == -INFINITY ? 0.f : ex2(top - mt);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] *= fa;
+        l *= fa;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
           if (x + k > x1) continue;
-          const float mt = fmaxf(top, ml[k].x);
-          const float fa = top == -INFINITY ? 0.f : ex2(top - mt), fb = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - mt);
+          const float fb = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - mt);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            acc[4 * e] = acc[4 * e] * fa + v[k][e].x * fb;
-            acc[4 * e + 1] = acc[4 * e + 1] * fa + v[k][e].y * fb;
-            acc[4 * e + 2] = acc[4 * e + 2] * fa + v[k][e].z * fb;
-            acc[4 * e + 3] = acc[4 * e + 3] * fa + v[k][e].w * fb;
+            acc[4 * e] += v[k][e].x * fb;
+            acc[4 * e + 1] += v[k][e].y * fb;
+            acc[4 * e + 2] += v[k][e].z * fb;
+            acc[4 * e + 3] += v[k][e].w * fb;
           }
-          l = l * fa + ml[k].y * fb;
-          top = mt;
+          l += ml[k].y * fb;
         }
+        top = mt;
       }
     }
     if (whole) continue;
