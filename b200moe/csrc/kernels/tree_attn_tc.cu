@@ -2,7 +2,7 @@
 // or 128): the same function as tree_attn.cu, for the shapes a server runs.
 //
 // Rows and keys.  The n nodes of a sequence times the G query heads of one KV head are
-// packed into tiles of 128 rows (row = node * G + head), keys into tiles of 128.  A
+// packed into tiles of 128 rows (row = node * G + head), keys into tiles of 64.  A
 // unit of work is one key tile against one pair of row tiles:
 //
 //   two row tiles (n * G > 128)   softmax group w of the CTA takes row tile w,
@@ -56,22 +56,21 @@ namespace {
 namespace cg = cooperative_groups;
 using bf16 = __nv_bfloat16;
 
-constexpr int kRows = 128, kKeys = 128;   // of a tile
-constexpr int kSub = 64;                  // keys of one score buffer
+constexpr int kRows = 128, kKeys = 64;    // of a tile
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
-constexpr int kCutTiles = 4;
+constexpr int kCutTiles = 8;
 constexpr int kParts = 4;         // partial results in flight per lane when parts are joined
 constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
 template <int D>
 struct Lay {
-  static constexpr int TILE = kKeys * D * 2;       // a K, V or Q tile: D / 64 halves of [128][64]
-  static constexpr int HALF = kKeys * 64 * 2;
-  static constexpr int SLOTS = D == 128 ? 2 : 4;   // K tiles, and V tiles, in flight
+  static constexpr int QTILE = kRows * D * 2, QHALF = kRows * 64 * 2;   // D / 64 halves of [128][64]
+  static constexpr int TILE = kKeys * D * 2, HALF = kKeys * 64 * 2;     // of K or V: halves of [64][64]
+  static constexpr int SLOTS = D == 128 ? 4 : 8;   // K tiles, and V tiles, in flight (even: see the issuers)
   static constexpr int Q = 0;                      // two row tiles; the second also carries the join
-  static constexpr int K = Q + 2 * TILE;
+  static constexpr int K = Q + 2 * QTILE;
   static constexpr int V = K + SLOTS * TILE;
   static constexpr int ANC = V + SLOTS * TILE;     // [nodes][kAncWords] ancestor bits
   static constexpr int PAR = ANC + kTreeMaxNodes * kAncWords * 4;
@@ -251,17 +250,15 @@ struct Seg {
 };
 static_assert(sizeof(Seg) == 64, "segment ring");
 
-// The key tiles of a segment that softmax group w takes, in runs of 64 keys.
+// The key tiles of a segment that softmax group w takes.
 struct Own {
-  int first, step, subs;
+  int first, step, n;
   __device__ __forceinline__ Own(const Seg& g, int gt, int w) {
     step = g.two ? 1 : 2;
     first = g.two || (gt & 1) == w ? g.t0 : g.t0 + 1;
-    const int n = first < g.t1 ? (g.t1 - 1 - first) / step + 1 : 0;
-    // the sequence's last keys may not reach the second half of their tile
-    subs = 2 * n - (n > 0 && g.len - (first + (n - 1) * step) * kKeys <= kSub ? 1 : 0);
+    n = first < g.t1 ? (g.t1 - 1 - first) / step + 1 : 0;
   }
-  __device__ __forceinline__ int tile(int s) const { return first + (s >> 1) * step; }
+  __device__ __forceinline__ int tile(int s) const { return first + s * step; }
 };
 
 __device__ __forceinline__ Seg seg_at(const Plan& p, int u, int lo, int hi) {
@@ -437,60 +434,87 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
       tma_prefetch_desc(&q_map);
-      const int nsub = kKeys / t.sub_rows;
-      int gt = 0, sg = 0;   // tiles, segments
-      bool ok = true, bad = false;
-      for (int u = u_lo; ok; ++sg) {
-        Seg g{};
-        if (u < u_hi) g = seg_at(plan, u, u_lo, u_hi);
-        u += g.t1 - g.t0;
-        {
-          volatile int* dst = reinterpret_cast<volatile int*>(&segs[sg % kRing]);
-          const int* src = reinterpret_cast<const int*>(&g);
+    }
+    const int nsub = kKeys / t.sub_rows;
+    int gt = 0, sg = 0;   // tiles, segments
+    bool ok = true, bad = false;
+    // The lanes hold block ids of the table, 32 at a time and the next 32 on their way: a load per
+    // tile in front of its copies cost more than the copies.
+    const int* tab = nullptr;
+    int window = 0, ids = 0, ids_next = 0;
+    auto entry = [&](int i) { return i < a.max_blocks ? __ldg(tab + i) : -1; };
+    for (int u = u_lo; ok; ++sg) {
+      Seg g{};
+      if (u < u_hi) g = seg_at(plan, u, u_lo, u_hi);
+      u += g.t1 - g.t0;
+      if (lane == 0) {
+        volatile int* dst = reinterpret_cast<volatile int*>(&segs[sg % kRing]);
+        const int* src = reinterpret_cast<const int*>(&g);
 #pragma unroll
-          for (int i = 0; i < 11; ++i) dst[i] = src[i];
-          mbar_arrive(&seg_full[sg % kRing]);
-        }
-        if (g.t1 == 0) break;
-        if (!mbar_wait(q_empty, (sg & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag)) break;
+        for (int i = 0; i < 11; ++i) dst[i] = src[i];
+        mbar_arrive(&seg_full[sg % kRing]);
+      }
+      if (g.t1 == 0) break;
+      tab = a.block_tables + (int64_t)g.b * a.max_blocks;
+      int bi = g.t0 * kKeys / a.block_size, y = g.t0 * kKeys - bi * a.block_size;   // of the tile's first key
+      window = bi;
+      ids = entry(window + lane);
+      ids_next = entry(window + 32 + lane);
+      ok = mbar_wait(q_empty, (sg & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag);
+      // its second Q tile may still carry a join
+      if (ok && g.two && sg > 0) ok = join_over(sg - 1);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      if (lane == 0) {
         const int tiles = g.two ? 2 : 1;
-        if (g.two && sg > 0 && !join_over(sg - 1)) break;   // its second Q tile may still carry a join
         mbar_arrive_expect_tx(q_full, tiles * kHalves * per * G * 128);
         for (int i = 0; i < tiles; ++i)
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf)
-            tma_3d(smem_u32(smem + L::Q + i * L::TILE + hf * L::HALF), &q_map, q_full, hf * 64, g.h * G,
+            tma_3d(smem_u32(smem + L::Q + i * L::QTILE + hf * L::QHALF), &q_map, q_full, hf * 64, g.h * G,
                    g.q0 + (2 * g.pair + i) * per);
-        const int* tab = a.block_tables + (int64_t)g.b * a.max_blocks;
-        for (int j = g.t0; j < g.t1 && ok; ++j, ++gt) {
-          const int slot = gt % kSlots;
-          const uint32_t ph = (gt / kSlots) & 1;
+      }
+      for (int j = g.t0; j < g.t1; ++j, ++gt) {
+        const int slot = gt % kSlots;
+        const uint32_t ph = (gt / kSlots) & 1;
+        while (bi >= window + 32) {
+          window += 32;
+          ids = ids_next;
+          ids_next = entry(window + 32 + lane);
+        }
+        int bi1 = bi, y1 = y;
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            uint64_t* full = kv ? &v_full[slot] : &k_full[slot];
-            if (!mbar_wait(kv ? &v_empty[slot] : &k_empty[slot], ph ^ 1, status, kStatusTimeoutEmpty, abort_flag)) {
-              ok = false;
-              break;
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t* full = kv ? &v_full[slot] : &k_full[slot];
+          ok = mbar_wait(kv ? &v_empty[slot] : &k_empty[slot], ph ^ 1, status, kStatusTimeoutEmpty, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(full, L::TILE);
+          const uint32_t dst = smem_u32(smem + (kv ? L::V : L::K) + slot * L::TILE);
+          bi1 = bi;
+          y1 = y;
+          for (int sub = 0; sub < nsub; ++sub) {
+            // a block of the window or of the next one (a tile has at most eight)
+            const int d = bi1 - window, a0 = __shfl_sync(0xffffffffu, ids, d & 31), a1 = __shfl_sync(0xffffffffu, ids_next, d & 31);
+            const int id = d < 32 ? a0 : a1;
+            int blk = a.num_blocks;      // out of range: zero fill
+            if (j * kKeys + sub * t.sub_rows < g.len) {
+              if (id >= 0 && id < a.num_blocks) blk = id;
+              else bad = true;
             }
-            mbar_arrive_expect_tx(full, L::TILE);
-            const uint32_t dst = smem_u32(smem + (kv ? L::V : L::K) + slot * L::TILE);
-            for (int sub = 0; sub < nsub; ++sub) {
-              const int key = j * kKeys + sub * t.sub_rows;
-              int blk = a.num_blocks;      // out of range: zero fill
-              if (key < g.len) {
-                const int bi = key / a.block_size;
-                const int id = bi < a.max_blocks ? tab[bi] : -1;
-                if (id >= 0 && id < a.num_blocks) blk = id;
-                else bad = true;
-              }
+            if (lane == 0) {
 #pragma unroll
               for (int hf = 0; hf < kHalves; ++hf)
-                tma_4d(dst + hf * L::HALF + sub * t.sub_rows * 128, kv ? &v_map : &k_map, full, hf * 64,
-                       key % a.block_size, g.h, blk);
+                tma_4d(dst + hf * L::HALF + sub * t.sub_rows * 128, kv ? &v_map : &k_map, full, hf * 64, y1, g.h, blk);
             }
+            y1 += t.sub_rows;
+            if (y1 >= a.block_size) { y1 = 0; ++bi1; }
           }
         }
+        if (!ok) break;
+        bi = bi1;
+        y = y1;
       }
+    }
+    if (lane == 0) {
       if (bad) record_status(status, kStatusBadShape);
       if (*abort_flag) {
         // a wait gave up: let the copies already issued land before the CTA exits
@@ -503,53 +527,49 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // ================================================================ MMA issuer of group w
     if (lane == 0) {
       const int w = warp - 1;
-      const uint32_t idesc_s = umma_idesc_bf16(kRows, kSub);
+      const uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys);
       const uint32_t idesc_pv = umma_idesc_bf16(kRows, D) | (1u << 16);  // B (V) is MN-major
       const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
-      int gt = 0, sg = 0, mine = 0;   // tiles of the CTA, segments, runs of this group
+      int gt = 0, sg = 0, mine = 0;   // tiles of the CTA, segments, tiles of this group
       bool ok = true;
       Seg g;
       for (; ok && segment(sg, g); ++sg) {
         if (!mbar_wait(q_full, sg & 1, status, kStatusTimeoutFull, abort_flag)) break;
-        const uint32_t qa = smem_u32(smem + L::Q + (g.two ? w : 0) * L::TILE);
+        const uint32_t qa = smem_u32(smem + L::Q + (g.two ? w : 0) * L::QTILE);
         const Own own(g, gt, w);
         auto issue_s = [&](int s) {
           const int slot = (gt + own.tile(s) - g.t0) % kSlots, buf = (mine + s) & 1;
-          const uint32_t kb = smem_u32(smem + L::K + slot * L::TILE) + (s & 1) * (kSub * 128);
+          const uint32_t kb = smem_u32(smem + L::K + slot * L::TILE);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * L::HALF + (k & 3) * 32;
-            umma_f16_ss(tS + buf * kSub, umma_sdesc_sw128(qa + off), umma_sdesc_sw128(kb + off), idesc_s, k > 0 ? 1u : 0u);
+            const uint32_t qo = (k >> 2) * L::QHALF + (k & 3) * 32, ko = (k >> 2) * L::HALF + (k & 3) * 32;
+            umma_f16_ss(tS + buf * kKeys, umma_sdesc_sw128(qa + qo), umma_sdesc_sw128(kb + ko), idesc_s, k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[2 * w + buf]);
-          if ((s & 1) || s + 1 == own.subs) {
-            umma_commit(&k_empty[slot]);
-            if (!g.two) umma_commit(&k_empty[slot]);   // the other group does not read this tile
-          }
+          umma_commit(&k_empty[slot]);
+          if (!g.two) umma_commit(&k_empty[slot]);     // the other group does not read this tile
         };
         auto issue_pv = [&](int s) {
           const int slot = (gt + own.tile(s) - g.t0) % kSlots, buf = (mine + s) & 1;
-          const uint32_t vb = smem_u32(smem + L::V + slot * L::TILE) + (s & 1) * (kSub * 128);
+          const uint32_t vb = smem_u32(smem + L::V + slot * L::TILE);
 #pragma unroll
-          for (int k = 0; k < kSub / 16; ++k)
-            umma_f16_ts(tO, tS + buf * kSub + k * 8, sdesc_mn(vb + k * 16 * 128, L::HALF), idesc_pv, (s > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_f16_ts(tO, tS + buf * kKeys + k * 8, sdesc_mn(vb + k * 16 * 128, L::HALF), idesc_pv, (s > 0 || k > 0) ? 1u : 0u);
           umma_commit(&pv_done[2 * w + buf]);
-          if ((s & 1) || s + 1 == own.subs) {
-            umma_commit(&v_empty[slot]);
-            if (!g.two) umma_commit(&v_empty[slot]);
-          }
+          umma_commit(&v_empty[slot]);
+          if (!g.two) umma_commit(&v_empty[slot]);
         };
-        // Scores run up to two runs ahead; whichever product has its inputs goes first (waiting for
+        // Scores run up to two tiles ahead; whichever product has its inputs goes first (waiting for
         // the next K here would hold back the product that frees a V tile).
         int si = 0, pi = 0;
         uint64_t since = 0;
-        while (pi < own.subs) {
+        while (pi < own.n) {
           bool did = false;
-          if (si < own.subs && si < pi + 2) {
+          if (si < own.n && si < pi + 2) {
             const int at = gt + own.tile(si) - g.t0;
-            // the scores overlay the P of the run two before
+            // the scores overlay the P of the tile two before
             if ((si < 2 || mbar_test(&pv_done[2 * w + ((mine + si) & 1)], ((mine + si - 2) >> 1) & 1)) &&
-                ((si & 1) || mbar_test(&k_full[at % kSlots], (at / kSlots) & 1))) {
+                mbar_test(&k_full[at % kSlots], (at / kSlots) & 1)) {
               tc_fence_after();
               issue_s(si++);
               did = true;
@@ -557,7 +577,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           }
           if (pi < si && mbar_test(&p_full[2 * w + ((mine + pi) & 1)], ((mine + pi) >> 1) & 1)) {
             const int at = gt + own.tile(pi) - g.t0;
-            if ((pi & 1) || mbar_test(&v_ready[at % kSlots], (at / kSlots) & 1)) {
+            if (mbar_test(&v_ready[at % kSlots], (at / kSlots) & 1)) {
               tc_fence_after();
               issue_pv(pi++);
               did = true;
@@ -575,7 +595,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           }
         }
         if (!ok) break;
-        mine += own.subs;
+        mine += own.n;
         gt += g.t1 - g.t0;
         // the segment's products are done (its Q, and every K and V phase before the next)
         umma_commit(q_empty);
@@ -696,21 +716,21 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       };
       float m = -INFINITY, l = 0.f;
       const Own own(g, gt, w);
-      const int done = own.subs;
+      const int done = own.n;
 #pragma unroll 1
-      for (int i = 0; i < own.subs; ++i, ++mine) {
+      for (int i = 0; i < own.n; ++i, ++mine) {
         const int buf = mine & 1;
-        const uint32_t tb = tS + buf * kSub;
+        const uint32_t tb = tS + buf * kKeys;
         ok = mbar_wait(&s_full[2 * w + buf], (mine >> 1) & 1, status, kStatusTimeoutAccFull, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (any) {
-          const int kb = own.tile(i) * kKeys + (i & 1) * kSub;
-          float s[kSub];
+          const int kb = own.tile(i) * kKeys;
+          float s[kKeys];
           tmem_ld<32>(tb, s);
           tmem_ld<32>(tb + 32, s + 32);
           tmem_ld_wait();
-          if (kb + kSub > prefix) {
+          if (kb + kKeys > prefix) {
             const uint32_t lo = sees(kb, 0), hi = sees(kb, 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
@@ -786,7 +806,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       // Where both groups hold a part, each hands the other half of its columns, D / 4 at a time,
       // through the second Q tile (not in use by a segment with one row tile).
       constexpr int kHand = D / 4;
-      float4* stage = reinterpret_cast<float4*>(smem + L::Q + L::TILE);   // [2][kHand / 4][128]
+      float4* stage = reinterpret_cast<float4*>(smem + L::Q + L::QTILE);   // [2][kHand / 4][128]
       auto hand = [&](int round) {
 #pragma unroll
         for (int c = 0; c < kHand; c += 16) {
