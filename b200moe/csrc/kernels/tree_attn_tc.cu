@@ -20,16 +20,17 @@
 // fp32 result with its running maximum and sum; after a grid-wide barrier the warps
 // join those (softmax over the parts).
 //
-// Roles per CTA (12 warps): a TMA producer; two MMA issuers, one per softmax group
-// (S = Q K^T, then O += P V with P read from TMEM, where it overlays its S); a cleaner
-// of the last V tiles; two softmax groups of four warps, a thread per row, so the row
+// Roles per CTA (12 warps): two TMA producers, one of Q and K and one of V, because a
+// copy with its wait costs its thread about 650 cycles and one thread alone held the
+// whole kernel at 4.9 TB/s; two MMA issuers, one per softmax group (S = Q K^T, then
+// O += P V with P read from TMEM, where it overlays its S); two softmax groups of four warps, a thread per row, so the row
 // statistics need no shuffles.  The running maximum moves only when a row grows by
 // more than 2^8, so O is rarely rescaled.  P is rounded to bf16 for the MMA and the sum
 // that divides O adds the rounded values, which cancels that rounding where few keys
 // carry the weight.
 //
 // A masked place never reaches the result: scores are selected, not added to, and a V
-// row is cleaned in front of the MMA (0 * NaN is NaN) -- rows behind the sequence become
+// row is cleaned by its producer in front of the MMA (0 * NaN is NaN) -- rows behind the sequence become
 // zero, and where a node's V is not finite those elements become zero and are added back
 // for the rows that see the node.
 //
@@ -106,11 +107,12 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int half, int z,
+                                       int w) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(half), "r"(z), "r"(w)
       : "memory");
 }
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -290,6 +292,56 @@ __device__ __forceinline__ Seg seg_at(const Plan& p, int u, int lo, int hi) {
   return g;
 }
 
+// Block ids of a sequence's table by the lanes of a warp, 32 at a time and the next 32 on their way:
+// a load per tile in front of its copies cost more than the copies.  Also copies a tile of keys.
+struct Blocks {
+  const int* tab;
+  int max_blocks, num_blocks, block_size, sub_rows, len;
+  int bi, y;             // block and row of the next tile's first key
+  int window, ids, ids_next;
+  bool bad;
+  __device__ __forceinline__ int entry(int i) const { return i < max_blocks ? __ldg(tab + i) : -1; }
+  __device__ __forceinline__ void start(const TreeAttnArgs& a, int b, int key, int keys, int lane) {
+    tab = a.block_tables + (int64_t)b * a.max_blocks;
+    len = keys;
+    bi = key / block_size;
+    y = key - bi * block_size;
+    window = bi;
+    ids = entry(window + lane);
+    ids_next = entry(window + 32 + lane);
+  }
+  // keys [key, key + kKeys) of KV head h, in boxes of sub_rows; the whole warp
+  template <int D>
+  __device__ __forceinline__ void copy(const CUtensorMap* map, uint64_t* bar, uint8_t* tile, int key, int h, int lane) {
+    using L = Lay<D>;
+    while (bi >= window + 32) {
+      window += 32;
+      ids = ids_next;
+      ids_next = entry(window + 32 + lane);
+    }
+    const uint32_t dst = smem_u32(tile);
+    for (int row = 0; row < kKeys; row += sub_rows) {
+      // a block of the window or of the next one (a tile has at most eight)
+      const int d = bi - window, a0 = __shfl_sync(0xffffffffu, ids, d & 31), a1 = __shfl_sync(0xffffffffu, ids_next, d & 31);
+      const int id = d < 32 ? a0 : a1;
+      int blk = num_blocks;          // out of range: zero fill
+      if (key + row < len) {
+        if (id >= 0 && id < num_blocks) blk = id;
+        else bad = true;
+      }
+      // (a box of fewer rows than the tile has its halves that many rows apart: one copy for each)
+      if (lane == 0) {
+        if (sub_rows == kKeys) tma_5d(dst, map, bar, 0, y, 0, h, blk);
+        else
+#pragma unroll
+          for (int hf = 0; hf < D / 64; ++hf) tma_5d(dst + hf * L::HALF + row * 128, map, bar, 0, y, hf, h, blk);
+      }
+      y += sub_rows;
+      if (y >= block_size) { y = 0; ++bi; }
+    }
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -301,9 +353,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t* k_empty = k_full + kSlots;
-  uint64_t* v_full = k_empty + kSlots;    // landed
-  uint64_t* v_ready = v_full + kSlots;    // cleaned where it had to be
-  uint64_t* v_empty = v_ready + kSlots;
+  uint64_t* v_ready = k_empty + kSlots;   // landed, and cleaned where it had to be
+  uint64_t* v_full = v_ready + kSlots;    // landed, of the tiles that have to be cleaned
+  uint64_t* v_empty = v_full + kSlots;
   uint64_t* q_full = v_empty + kSlots;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;         // [2][2] per softmax group and score buffer
@@ -428,21 +480,22 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     return g.t1 > 0;
   };
 
+  auto settle = [&]() {
+    if (!*abort_flag) return;
+    // a wait gave up: let the copies already issued land before the CTA exits
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+  };
+
   if (warp == 0) {
-    // ================================================================ TMA producer
+    // ================================================================ producer of Q and K
     if (lane == 0) {
       tma_prefetch_desc(&k_map);
-      tma_prefetch_desc(&v_map);
       tma_prefetch_desc(&q_map);
     }
-    const int nsub = kKeys / t.sub_rows;
+    Blocks blocks{nullptr, a.max_blocks, a.num_blocks, a.block_size, t.sub_rows};
     int gt = 0, sg = 0;   // tiles, segments
-    bool ok = true, bad = false;
-    // The lanes hold block ids of the table, 32 at a time and the next 32 on their way: a load per
-    // tile in front of its copies cost more than the copies.
-    const int* tab = nullptr;
-    int window = 0, ids = 0, ids_next = 0;
-    auto entry = [&](int i) { return i < a.max_blocks ? __ldg(tab + i) : -1; };
+    bool ok = true;
     for (int u = u_lo; ok; ++sg) {
       Seg g{};
       if (u < u_hi) g = seg_at(plan, u, u_lo, u_hi);
@@ -455,11 +508,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         mbar_arrive(&seg_full[sg % kRing]);
       }
       if (g.t1 == 0) break;
-      tab = a.block_tables + (int64_t)g.b * a.max_blocks;
-      int bi = g.t0 * kKeys / a.block_size, y = g.t0 * kKeys - bi * a.block_size;   // of the tile's first key
-      window = bi;
-      ids = entry(window + lane);
-      ids_next = entry(window + 32 + lane);
+      blocks.start(a, g.b, g.t0 * kKeys, g.len, lane);
       ok = mbar_wait(q_empty, (sg & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag);
       // its second Q tile may still carry a join
       if (ok && g.two && sg > 0) ok = join_over(sg - 1);
@@ -475,52 +524,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
       for (int j = g.t0; j < g.t1; ++j, ++gt) {
         const int slot = gt % kSlots;
-        const uint32_t ph = (gt / kSlots) & 1;
-        while (bi >= window + 32) {
-          window += 32;
-          ids = ids_next;
-          ids_next = entry(window + 32 + lane);
-        }
-        int bi1 = bi, y1 = y;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          uint64_t* full = kv ? &v_full[slot] : &k_full[slot];
-          ok = mbar_wait(kv ? &v_empty[slot] : &k_empty[slot], ph ^ 1, status, kStatusTimeoutEmpty, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_expect_tx(full, L::TILE);
-          const uint32_t dst = smem_u32(smem + (kv ? L::V : L::K) + slot * L::TILE);
-          bi1 = bi;
-          y1 = y;
-          for (int sub = 0; sub < nsub; ++sub) {
-            // a block of the window or of the next one (a tile has at most eight)
-            const int d = bi1 - window, a0 = __shfl_sync(0xffffffffu, ids, d & 31), a1 = __shfl_sync(0xffffffffu, ids_next, d & 31);
-            const int id = d < 32 ? a0 : a1;
-            int blk = a.num_blocks;      // out of range: zero fill
-            if (j * kKeys + sub * t.sub_rows < g.len) {
-              if (id >= 0 && id < a.num_blocks) blk = id;
-              else bad = true;
-            }
-            if (lane == 0) {
-#pragma unroll
-              for (int hf = 0; hf < kHalves; ++hf)
-                tma_4d(dst + hf * L::HALF + sub * t.sub_rows * 128, kv ? &v_map : &k_map, full, hf * 64, y1, g.h, blk);
-            }
-            y1 += t.sub_rows;
-            if (y1 >= a.block_size) { y1 = 0; ++bi1; }
-          }
-        }
-        if (!ok) break;
-        bi = bi1;
-        y = y1;
+        ok = mbar_wait(&k_empty[slot], ((gt / kSlots) & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[slot], L::TILE);
+        blocks.template copy<D>(&k_map, &k_full[slot], smem + L::K + slot * L::TILE, j * kKeys, g.h, lane);
       }
     }
     if (lane == 0) {
-      if (bad) record_status(status, kStatusBadShape);
-      if (*abort_flag) {
-        // a wait gave up: let the copies already issued land before the CTA exits
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
-      }
+      if (blocks.bad) record_status(status, kStatusBadShape);
+      settle();
     }
     __syncwarp();
   } else if (warp <= 2) {
@@ -606,8 +618,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
     __syncwarp();
   } else if (warp == 3) {
-    // ================================================================ V cleaner
+    // ================================================================ producer of V
+    if (lane == 0) tma_prefetch_desc(&v_map);
+    Blocks blocks{nullptr, a.max_blocks, a.num_blocks, a.block_size, t.sub_rows};
     int gt = 0, sg = 0;
+    uint32_t cleaned = 0;      // parity of each slot's v_full: it counts the tiles that had to be cleaned
     bool ok = true;
     Seg g;
     for (; ok && __all_sync(0xffffffffu, segment(sg, g)); ++sg) {
@@ -615,42 +630,60 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       if (lane < kAncWords) dirt[lane] = 0;
       __syncwarp();
       const int prefix = g.len - g.n;
-      for (int j = g.t0; j < g.t1; ++j, ++gt) {
-        const int slot = gt % kSlots;
-        ok = mbar_wait(&v_full[slot], (gt / kSlots) & 1, status, kStatusTimeoutFull, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        if ((j + 1) * kKeys > prefix) {
-          uint8_t* vt = smem + L::V + slot * L::TILE;
-          for (int r = lane; r < kKeys; r += 32) {
-            const int node = j * kKeys + r - prefix;
-            if (node < 0) continue;
-            const bool behind = node >= g.n;
-            bool bad = false;
+      blocks.start(a, g.b, g.t0 * kKeys, g.len, lane);
+      // a tile with nodes or with rows behind the sequence, in slot `slot`
+      auto clean = [&](int j, int slot) {
+        ok = mbar_wait(&v_full[slot], (cleaned >> slot) & 1, status, kStatusTimeoutFull, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
+        cleaned ^= 1u << slot;
+        uint8_t* vt = smem + L::V + slot * L::TILE;
+        for (int r = lane; r < kKeys; r += 32) {
+          const int node = j * kKeys + r - prefix;
+          if (node < 0) continue;
+          const bool behind = node >= g.n;
+          bool bad = false;
 #pragma unroll 1
-            for (int c = 0; c < D / 8; ++c) {
-              uint4* p = reinterpret_cast<uint4*>(vt + (c >> 3) * L::HALF + sw_off(r, c & 7));
-              if (behind) {
-                *p = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              const uint4 v = *p;
-              uint32_t e[4] = {v.x, v.y, v.z, v.w};
-              bool hit = false;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {   // all exponent bits set: infinite or NaN
-                if ((e[i] & 0x7f80u) == 0x7f80u) { e[i] &= 0xffff0000u; hit = true; }
-                if ((e[i] & 0x7f800000u) == 0x7f800000u) { e[i] &= 0xffffu; hit = true; }
-              }
-              if (hit) { *p = make_uint4(e[0], e[1], e[2], e[3]); bad = true; }
+          for (int c = 0; c < D / 8; ++c) {
+            uint4* p = reinterpret_cast<uint4*>(vt + (c >> 3) * L::HALF + sw_off(r, c & 7));
+            if (behind) {
+              *p = make_uint4(0, 0, 0, 0);
+              continue;
             }
-            if (bad) atomicOr(&dirt[node >> 5], 1u << (node & 31));
+            const uint4 v = *p;
+            uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            bool hit = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {   // all exponent bits set: infinite or NaN
+              if ((e[i] & 0x7f80u) == 0x7f80u) { e[i] &= 0xffff0000u; hit = true; }
+              if ((e[i] & 0x7f800000u) == 0x7f800000u) { e[i] &= 0xffffu; hit = true; }
+            }
+            if (hit) { *p = make_uint4(e[0], e[1], e[2], e[3]); bad = true; }
           }
-          fence_proxy_async_smem();
+          if (bad) atomicOr(&dirt[node >> 5], 1u << (node & 31));
         }
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_ready[slot]);
+      };
+      int due = -1;            // the tile before this one, if it has to be cleaned
+      for (int j = g.t0; j < g.t1 && ok; ++j, ++gt) {
+        const int slot = gt % kSlots;
+        ok = mbar_wait(&v_empty[slot], ((gt / kSlots) & 1) ^ 1, status, kStatusTimeoutEmpty, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        const bool dirty_tile = (j + 1) * kKeys > prefix;
+        uint64_t* bar = dirty_tile ? &v_full[slot] : &v_ready[slot];
+        if (lane == 0) mbar_arrive_expect_tx(bar, L::TILE);
+        blocks.template copy<D>(&v_map, bar, smem + L::V + slot * L::TILE, j * kKeys, g.h, lane);
+        if (due >= 0) clean(due, (gt - 1) % kSlots);
+        due = dirty_tile ? j : -1;
       }
+      if (ok && due >= 0) clean(due, (gt - 1) % kSlots);
     }
+    if (lane == 0) {
+      if (blocks.bad) record_status(status, kStatusBadShape);
+      settle();
+    }
+    __syncwarp();
   } else {
     // ================================================================ softmax group w
     const int w = (warp - 4) >> 2;
@@ -1005,7 +1038,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 void encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
             const cuuint32_t* box) {
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box,
                                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1015,11 +1048,12 @@ void encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims
 template <int D>
 void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
   CUtensorMap km, vm, qm;
-  const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.block_size, (cuuint64_t)a.num_kv_heads, (cuuint64_t)a.num_blocks};
-  const cuuint64_t ks[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.block_size * D * 2, (cuuint64_t)a.block_stride * 2};
-  const cuuint32_t kb[4] = {64, (cuuint32_t)p.sub_rows, 1, 1};
-  encode(&km, 4, a.k_cache, kd, ks, kb);
-  encode(&vm, 4, a.v_cache, kd, ks, kb);
+  // columns as (64, D / 64): one copy brings both halves of a tile
+  const cuuint64_t kd[5] = {64, (cuuint64_t)a.block_size, D / 64, (cuuint64_t)a.num_kv_heads, (cuuint64_t)a.num_blocks};
+  const cuuint64_t ks[4] = {(cuuint64_t)D * 2, 128, (cuuint64_t)a.block_size * D * 2, (cuuint64_t)a.block_stride * 2};
+  const cuuint32_t kb[5] = {64, (cuuint32_t)p.sub_rows, (cuuint32_t)(p.sub_rows == kKeys ? D / 64 : 1), 1, 1};
+  encode(&km, 5, a.k_cache, kd, ks, kb);
+  encode(&vm, 5, a.v_cache, kd, ks, kb);
   const int nq = a.num_kv_heads * a.group;
   const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)nq, (cuuint64_t)a.rows};
   const cuuint64_t qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)nq * D * 2};
