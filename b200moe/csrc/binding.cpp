@@ -751,52 +751,75 @@ void kv_int8_stage(Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k_scale
   b200::kv_int8_stage(a, stream());
 }
 
+// The draft-tree entry points check their arguments here alone (their Python sides do not repeat it on
+// a GPU: a call's host time counts there), so a bad one is a ValueError.  Numbers enter a message by
+// to_string: a C++ library linked into this module must not format them into a stream of torch's.
+#define CHECK_VALUE(cond, ...) \
+  do { if (!(cond)) throw py::value_error(c10::str(__VA_ARGS__)); } while (0)
+
+void check_contiguous(const Tensor& t, const char* name) {
+  CHECK_VALUE(t.is_cuda() && t.is_contiguous(), name, " must be a contiguous CUDA tensor");
+}
+
+void check_bf16(const Tensor& t, const char* name) {
+  CHECK_VALUE(t.scalar_type() == torch::kBFloat16, name, " must be bf16, got ", t.scalar_type());
+}
+
+// Contiguous tensors that share bytes.
+void check_apart(const Tensor& a, const Tensor& b, const char* names) {
+  const auto lo = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  CHECK_VALUE(lo(a) + a.nbytes() <= lo(b) || lo(b) + b.nbytes() <= lo(a), names, " must not overlap");
+}
+
 void check_aligned(const Tensor& t, const char* name) {
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name, " must start on a 16-byte boundary");
+  CHECK_VALUE((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name, " must start on a 16-byte boundary");
 }
 
 // int32 metadata of a batch of drafted trees: cu [B + 1], lens [B], tables [B, max_blocks], parents [rows].
 void check_tree(const Tensor& cu, const Tensor& lens, const Tensor& tables, const Tensor& parents,
                 c10::Device dev, int64_t max_q_len) {
   for (const Tensor* t : {&cu, &lens, &tables, &parents}) {
-    TORCH_CHECK(t->device() == dev, "tree metadata must be on ", dev, ", got ", t->device());
-    TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->is_contiguous(), "tree metadata must be contiguous int32");
+    CHECK_VALUE(t->device() == dev, "tree metadata must be on ", dev, ", got ", t->device());
+    CHECK_VALUE(t->scalar_type() == torch::kInt32 && t->is_contiguous(), "tree metadata must be contiguous int32");
   }
-  TORCH_CHECK(cu.dim() == 1 && lens.dim() == 1 && cu.numel() == lens.numel() + 1,
+  CHECK_VALUE(cu.dim() == 1 && lens.dim() == 1 && cu.numel() == lens.numel() + 1,
               "cu_seqlens_q must hold one entry more than seq_lens");
-  TORCH_CHECK(tables.dim() == 2 && tables.size(0) == lens.numel() && tables.size(1) >= 1,
+  CHECK_VALUE(tables.dim() == 2 && tables.size(0) == lens.numel() && tables.size(1) >= 1,
               "block_tables must be [batch, max_blocks]");
-  TORCH_CHECK(parents.dim() == 1, "parents must be [rows]");
-  TORCH_CHECK(max_q_len >= 1 && max_q_len <= b200::kTreeMaxNodes, "max_q_len must be in [1, ", b200::kTreeMaxNodes,
-              "], got ", max_q_len);
+  CHECK_VALUE(parents.dim() == 1, "parents must be [rows]");
+  CHECK_VALUE(max_q_len >= 1 && max_q_len <= b200::kTreeMaxNodes, "max_q_len must be in [1, ",
+              std::to_string(b200::kTreeMaxNodes), "], got ", std::to_string(max_q_len));
 }
 
-void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k_scale, c10::optional<Tensor> v_scale,
-               Tensor cu, Tensor lens, Tensor tables, Tensor parents, Tensor out, int64_t max_q_len,
-               int64_t block_size, int64_t block_stride, int64_t scale_block_stride, double scale, Tensor status,
-               std::vector<int64_t> chan) {
-  CHECK_CUDA(q); CHECK_CONTIG(q); CHECK_CONTIG(out);
-  CHECK_DT(q, torch::kBFloat16); CHECK_DT(out, torch::kBFloat16);
-  TORCH_CHECK(q.dim() == 3 && out.sizes() == q.sizes() && out.device() == q.device(),
+Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k_scale,
+                 c10::optional<Tensor> v_scale, Tensor cu, Tensor lens, Tensor tables, Tensor parents,
+                 c10::optional<Tensor> out_arg, int64_t max_q_len, int64_t block_size, int64_t block_stride,
+                 int64_t scale_block_stride, double scale, Tensor status, std::vector<int64_t> chan) {
+  check_contiguous(q, "q"); check_bf16(q, "q");
+  Tensor out = out_arg.has_value() ? *out_arg : torch::empty_like(q);
+  check_contiguous(out, "out"); check_bf16(out, "out");
+  CHECK_VALUE(q.dim() == 3 && out.sizes() == q.sizes() && out.device() == q.device(),
               "q and out must be [rows, q_heads, head_dim] on one device");
-  TORCH_CHECK(k_cache.device() == q.device() && v_cache.device() == q.device() && k_cache.dim() == 4 &&
+  check_apart(q, out, "q and out");
+  CHECK_VALUE(k_cache.device() == q.device() && v_cache.device() == q.device() && k_cache.dim() == 4 &&
               k_cache.sizes() == v_cache.sizes() && k_cache.scalar_type() == v_cache.scalar_type(),
               "k and v must be [blocks, kv_heads, block_size, head_dim] of one type on q's device");
   const int64_t nkv = k_cache.size(1), D = q.size(2), nq = q.size(1);
-  TORCH_CHECK(k_cache.size(2) == block_size && k_cache.size(3) == D, "cache blocks must be [block_size, head_dim]");
+  CHECK_VALUE(k_cache.size(2) == block_size && k_cache.size(3) == D, "cache blocks must be [block_size, head_dim]");
   for (const Tensor* t : {&k_cache, &v_cache})
-    TORCH_CHECK(t->stride(0) == block_stride && t->stride(1) == block_size * D && t->stride(2) == D &&
+    CHECK_VALUE(t->stride(0) == block_stride && t->stride(1) == block_size * D && t->stride(2) == D &&
                 t->stride(3) == 1, "cache planes must be contiguous [kv_heads, block_size, head_dim]");
-  TORCH_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128, got ", D);
-  TORCH_CHECK(nq % nkv == 0, "q heads must be a multiple of kv heads");
+  CHECK_VALUE(D == 64 || D == 128, "head_dim must be 64 or 128, got ", std::to_string(D));
+  CHECK_VALUE(nkv >= 1 && nq >= 1 && nq % nkv == 0, "q heads must be a multiple of kv heads");
   const bool int8 = k_cache.scalar_type() == torch::kInt8;
-  TORCH_CHECK(int8 || k_cache.scalar_type() == torch::kBFloat16, "cache must be bf16 or int8");
+  CHECK_VALUE(int8 || k_cache.scalar_type() == torch::kBFloat16, "cache must be bf16 or int8");
   check_tree(cu, lens, tables, parents, q.device(), max_q_len);
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(out.data_ptr()) & 31) == 0, "out must start on a 32-byte boundary");
+  CHECK_VALUE((reinterpret_cast<uintptr_t>(out.data_ptr()) & 31) == 0, "out must start on a 32-byte boundary");
   check_aligned(q, "q"); check_aligned(k_cache, "k"); check_aligned(v_cache, "v");
-  TORCH_CHECK(block_stride * k_cache.element_size() % 16 == 0, "cache blocks must be multiples of 16 bytes");
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
-  TORCH_CHECK(parents.numel() == q.size(0), "parents must hold one entry per row of q");
+  CHECK_VALUE(block_stride * k_cache.element_size() % 16 == 0, "cache blocks must be multiples of 16 bytes");
+  CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale must be positive");
+  CHECK_VALUE(parents.numel() == q.size(0), "parents must hold one entry per row of q");
+  if (q.size(0) == 0 || lens.numel() == 0) return out;
   b200::TreeAttnArgs a{};
   a.q = q.data_ptr();
   a.k_cache = k_cache.data_ptr();
@@ -804,9 +827,9 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   a.kv_int8 = int8 ? 1 : 0;
   set_kv_channel(&a.kv_int8, &a.ch, chan);
   if (a.kv_int8 == 1) {
-    TORCH_CHECK(k_scale.has_value() && v_scale.has_value(), "int8 cache needs its scales");
+    CHECK_VALUE(k_scale.has_value() && v_scale.has_value(), "int8 cache needs its scales");
     for (const Tensor* t : {&*k_scale, &*v_scale})
-      TORCH_CHECK(t->device() == q.device() && t->scalar_type() == torch::kFloat32 && t->dim() == 3 &&
+      CHECK_VALUE(t->device() == q.device() && t->scalar_type() == torch::kFloat32 && t->dim() == 3 &&
                   t->size(0) == k_cache.size(0) && t->size(1) == nkv && t->size(2) == block_size &&
                   t->stride(0) == scale_block_stride && t->stride(1) == block_size && t->stride(2) == 1,
                   "scales must be fp32 [blocks, kv_heads, block_size]");
@@ -840,6 +863,7 @@ void tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k
   } else {
     b200::tree_attn(a, stream());
   }
+  return out;
 }
 
 // Accepted paths of a batch of trees; the rows of kv_data (and scales / side) move in place.
@@ -847,24 +871,24 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
                                                c10::optional<Tensor> kv_side, Tensor cu, Tensor lens, Tensor tables,
                                                Tensor parents, Tensor draft, Tensor target, int64_t max_q_len,
                                                Tensor status) {
-  CHECK_CUDA(kv_data); CHECK_CONTIG(kv_data);
-  TORCH_CHECK(kv_data.dim() == 6 && kv_data.size(2) == 2,
+  check_contiguous(kv_data, "kv_data");
+  CHECK_VALUE(kv_data.dim() == 6 && kv_data.size(2) == 2,
               "kv_data must be [blocks, layers, 2, kv_heads, block_size, head_dim]");
   check_tree(cu, lens, tables, parents, kv_data.device(), max_q_len);
   for (const Tensor* t : {&draft, &target})
-    TORCH_CHECK(t->device() == kv_data.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous() &&
+    CHECK_VALUE(t->device() == kv_data.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous() &&
                 t->sizes() == parents.sizes(), "draft_ids and target_ids must be int32 like parents");
   b200::TreeCommitArgs a{};
   a.num_blocks = (int)kv_data.size(0);
   a.planes = (int)(kv_data.size(1) * 2 * kv_data.size(3));
   a.block_size = (int)kv_data.size(4);
-  TORCH_CHECK(kv_data.size(0) * kv_data.size(4) < (1ll << 31), "the pool must have fewer than 2^31 slots");
+  CHECK_VALUE(kv_data.size(0) * kv_data.size(4) < (1ll << 31), "the pool must have fewer than 2^31 slots");
   auto add = [&](const Tensor& t, int64_t per_row, const char* name) {
-    TORCH_CHECK(t.device() == kv_data.device() && t.is_contiguous() &&
+    CHECK_VALUE(t.device() == kv_data.device() && t.is_contiguous() &&
                 t.numel() == kv_data.size(0) * a.planes * a.block_size * per_row,
                 name, " must be contiguous, [blocks, layers, 2, kv_heads, block_size] rows like kv_data");
     const int64_t bytes = per_row * t.element_size();
-    TORCH_CHECK(bytes % 4 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+    CHECK_VALUE(bytes % 4 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
                 name, " rows must be a multiple of 4 bytes on an aligned base");
     a.rows[a.kinds++] = {static_cast<uint8_t*>(t.data_ptr()), (int)bytes};
   };
@@ -894,43 +918,49 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
   return {accepted, path, tokens};
 }
 
-void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Tensor w2, c10::optional<Tensor> s2,
-             int64_t E, int64_t topk, bool renorm, Tensor out, c10::optional<Tensor> ids,
-             c10::optional<Tensor> weights, bool tiled, Tensor status) {
-  CHECK_CUDA(x); CHECK_CONTIG(x); CHECK_CONTIG(out); CHECK_DT(x, torch::kBFloat16); CHECK_DT(out, torch::kBFloat16);
-  TORCH_CHECK(x.dim() == 2 && out.sizes() == x.sizes(), "x and out must be [tokens, hidden]");
+Tensor moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Tensor w2, c10::optional<Tensor> s2,
+               int64_t E, int64_t topk, bool renorm, c10::optional<Tensor> out_arg, c10::optional<Tensor> ids,
+               c10::optional<Tensor> weights, bool tiled, Tensor status) {
+  check_contiguous(x, "x"); check_bf16(x, "x");
+  Tensor out = out_arg.has_value() ? *out_arg : torch::empty_like(x);
+  check_contiguous(out, "out"); check_bf16(out, "out");
+  CHECK_VALUE(x.dim() == 2 && out.sizes() == x.sizes(), "x and out must be [tokens, hidden]");
+  check_apart(x, out, "x and out");
   const int64_t T = x.size(0), H = x.size(1);
-  TORCH_CHECK(T <= b200::kFewMaxTokens, "at most ", b200::kFewMaxTokens, " tokens, got ", T);
-  TORCH_CHECK(E >= 1 && E <= b200::kFewMaxExperts && topk >= 1 && topk <= b200::kFewMaxTopk && topk <= E,
-              "experts must be in [1, ", b200::kFewMaxExperts, "] and topk in [1, ", b200::kFewMaxTopk, "]");
+  CHECK_VALUE(T <= b200::kFewMaxTokens, "at most ", std::to_string(b200::kFewMaxTokens), " tokens, got ",
+              std::to_string(T));
+  CHECK_VALUE(E >= 1 && E <= b200::kFewMaxExperts && topk >= 1 && topk <= b200::kFewMaxTopk && topk <= E,
+              "experts must be in [1, ", std::to_string(b200::kFewMaxExperts), "] and topk in [1, ",
+              std::to_string(b200::kFewMaxTopk), "]");
   for (const Tensor* t : {&router, &w13, &w2, &out})
-    TORCH_CHECK(t->device() == x.device() && t->is_contiguous(), "weights must be contiguous, on x's device");
+    CHECK_VALUE(t->device() == x.device() && t->is_contiguous(), "weights must be contiguous, on x's device");
   check_aligned(x, "x"); check_aligned(out, "out"); check_aligned(router, "router"); check_aligned(w13, "w13");
   check_aligned(w2, "w2");
-  CHECK_DT(router, torch::kBFloat16);
-  TORCH_CHECK(router.dim() == 2 && router.size(0) >= E && router.size(1) == H, "router must be [>= experts, hidden]");
+  check_bf16(router, "router");
+  CHECK_VALUE(router.dim() == 2 && router.size(0) >= E && router.size(1) == H, "router must be [>= experts, hidden]");
   const bool fp8 = w13.scalar_type() == torch::kFloat8_e4m3fn;
-  TORCH_CHECK((fp8 || w13.scalar_type() == torch::kBFloat16) && w2.scalar_type() == w13.scalar_type(),
+  CHECK_VALUE((fp8 || w13.scalar_type() == torch::kBFloat16) && w2.scalar_type() == w13.scalar_type(),
               "expert weights must both be e4m3 or both bf16");
-  TORCH_CHECK(w2.dim() == 3 && w13.dim() == 3 && w2.size(0) == E && w13.size(0) == E && w2.size(1) == H &&
+  CHECK_VALUE(w2.dim() == 3 && w13.dim() == 3 && w2.size(0) == E && w13.size(0) == E && w2.size(1) == H &&
               w13.size(2) == H && w13.size(1) == 2 * w2.size(2), "w13 must be [E, 2I, H] and w2 [E, H, I]");
   const int64_t I = w2.size(2);
-  TORCH_CHECK(H % 128 == 0 && I % 128 == 0 && H >= 128 && I >= 128 && H <= 8192 && I <= 8192,
+  CHECK_VALUE(H % 128 == 0 && I % 128 == 0 && H >= 128 && I >= 128 && H <= 8192 && I <= 8192,
               "hidden and intermediate sizes must be multiples of 128, at most 8192");
-  TORCH_CHECK(fp8 == s13.has_value() && fp8 == s2.has_value(), "e4m3 weights need their scales; bf16 weights take none");
-  TORCH_CHECK(fp8 || !tiled, "bf16 weights are row-major");
+  CHECK_VALUE(fp8 == s13.has_value() && fp8 == s2.has_value(), "e4m3 weights need their scales; bf16 weights take none");
+  CHECK_VALUE(fp8 || !tiled, "bf16 weights are row-major");
   if (fp8) {
     for (const Tensor* t : {&*s13, &*s2})
-      TORCH_CHECK(t->device() == x.device() && t->is_contiguous() && t->scalar_type() == torch::kFloat32,
+      CHECK_VALUE(t->device() == x.device() && t->is_contiguous() && t->scalar_type() == torch::kFloat32,
                   "scales must be contiguous fp32");
-    TORCH_CHECK(s13->numel() == E * (2 * I / 128) * (H / 128) && s2->numel() == E * (H / 128) * (I / 128),
+    CHECK_VALUE(s13->numel() == E * (2 * I / 128) * (H / 128) && s2->numel() == E * (H / 128) * (I / 128),
                 "scales must be [E, N/128, K/128]");
   }
   for (const c10::optional<Tensor>* t : {&ids, &weights})
     if (t->has_value())
-      TORCH_CHECK((*t)->device() == x.device() && (*t)->is_contiguous() && (*t)->numel() == T * topk &&
+      CHECK_VALUE((*t)->device() == x.device() && (*t)->is_contiguous() && (*t)->numel() == T * topk &&
                   (*t)->scalar_type() == (t == &ids ? torch::kInt32 : torch::kFloat32),
                   "ids (int32) and weights (fp32) must be [tokens, topk]");
+  if (T == 0) return out;
   c10::cuda::CUDAGuard guard(x.device());
   // [slots | hidden rows | their factors | x in e4m3 | logits | x factors | selection | counters], floats
   const int64_t P = T * topk, at_h = P * H, at_hf = at_h + P * I, at_x = at_hf + P * (I / 16), at_l = at_x + T * H / 2,
@@ -961,6 +991,7 @@ void moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Ten
   a.done = reinterpret_cast<int*>(w + at_done);
   a.status = status.data_ptr<int>();
   b200::moe_few(a, stream());
+  return out;
 }
 
 void argmax(Tensor logits, Tensor out) {

@@ -485,6 +485,11 @@ def moe_permute(x, ids, counts, cursor, x_perm, slot_of_row, offsets_out=None):
     count_launches()
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Contiguous tensors that share bytes."""
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
 MOE_FEW_MAX_TOKENS = 64
 
 
@@ -496,6 +501,11 @@ def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True
     (``tiled``: stored by ``tile_fp8``) or bf16 (s13 = s2 = None); every expert is on this GPU.
     ``ids`` [T, topk] int32 / ``weights`` [T, topk] fp32 receive the routing.  An e4m3 weight enters as
     q * scale in fp32, where the grouped GEMMs round that product to bf16 first."""
+    if x.is_cuda:
+        out = native().moe_few(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled,
+                               status_word(x.device))
+        count_launches(1 if x.shape[0] else 0)
+        return out
     if x.dim() != 2 or not x.is_contiguous():
         raise ValueError("x must be contiguous [tokens, hidden]")
     T, H = x.shape
@@ -512,15 +522,9 @@ def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True
         out = torch.empty_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be like x")
-    if not x.is_cuda:
-        return _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled)
-    if H % 128 or w2.shape[2] % 128:
-        raise ValueError("hidden and intermediate sizes must be multiples of 128")
-    if T:
-        native().moe_few(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled,
-                         status_word(x.device))
-        count_launches()
-    return out
+    elif _overlap(x, out):
+        raise ValueError("x and out must not overlap")
+    return _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled)
 
 
 def _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled):
@@ -696,6 +700,12 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
     table row has) is left out and a block id outside the pool is not read; both set the status word
     (``check_status``)."""
+    if q.is_cuda:
+        out = native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q, seq_lens,
+                                 block_tables, parents, out, max_q_len, kv_layer.block_size, kv_layer.block_stride,
+                                 kv_layer.scale_block_stride, scale, status_word(q.device), _chan_read(kv_layer))
+        count_launches(1 if q.shape[0] and seq_lens.shape[0] else 0)
+        return out
     if q.dim() != 3 or not q.is_contiguous():
         raise ValueError("q must be contiguous [rows, q_heads, head_dim]")
     _check_tree(q.shape[0], cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, q.device)
@@ -705,16 +715,11 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
         raise ValueError("out must be like q")
+    elif _overlap(q, out):
+        raise ValueError("q and out must not overlap")
     if q.shape[1] % kv_layer.num_kv_heads:
         raise ValueError("q heads must be a multiple of kv heads")
-    if not q.is_cuda:
-        return _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out)
-    if q.shape[0] and seq_lens.shape[0]:
-        native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q, seq_lens,
-                           block_tables, parents, out, max_q_len, kv_layer.block_size, kv_layer.block_stride,
-                           kv_layer.scale_block_stride, scale, status_word(q.device), _chan_read(kv_layer))
-        count_launches()
-    return out
+    return _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out)
 
 
 def _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out):
@@ -756,6 +761,11 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
     path, their places and the tokens to emit behind them, -1 behind the path; the committed length is
     P + accepted.  A malformed row accepts nothing, a move through a block id outside the pool is left
     out; both set the status word."""
+    if kv_data.is_cuda:
+        res = native().tree_commit(kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents,
+                                   draft_ids, target_ids, max_q_len, status_word(kv_data.device))
+        count_launches(1 if seq_lens.shape[0] else 0)
+        return res
     _check_tree(None, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, kv_data.device)
     for name, t in (("draft_ids", draft_ids), ("target_ids", target_ids)):
         if t.dtype != torch.int32 or t.shape != parents.shape or t.device != kv_data.device or not t.is_contiguous():
@@ -765,13 +775,8 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
     for name, t in (("kv_scales", kv_scales), ("kv_side", kv_side)):
         if t is not None and (t.shape[:5] != kv_data.shape[:5] or not t.is_contiguous() or t.device != kv_data.device):
             raise ValueError(f"{name} must be contiguous rows [blocks, layers, 2, kv_heads, block_size] like kv_data")
-    if not kv_data.is_cuda:
-        return _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids,
-                                max_q_len, kv_scales, kv_side)
-    res = native().tree_commit(kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids,
-                               target_ids, max_q_len, status_word(kv_data.device))
-    count_launches(1 if seq_lens.shape[0] else 0)
-    return res
+    return _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids, max_q_len,
+                            kv_scales, kv_side)
 
 
 def _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids, max_q_len,

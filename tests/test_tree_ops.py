@@ -238,8 +238,18 @@ def test_tree_refusals(dev):
     for args in bad:
         with pytest.raises(ValueError):
             ops.tree_attention(*args)
-    with pytest.raises(ValueError):
-        ops.tree_attention(*b.args(), out=torch.empty(3, 8, 128, dtype=q.dtype, device=dev))
+    for out in (torch.empty(3, 8, 128, dtype=q.dtype, device=dev), torch.empty_like(q, dtype=torch.float16), q):
+        with pytest.raises(ValueError):
+            ops.tree_attention(*b.args(), out=out)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            ops.tree_attention(q, kv, cu, lens, tab, par, n, scale)
+    if dev == "cuda":   # metadata left on the host, a head size without a kernel
+        with pytest.raises(ValueError):
+            ops.tree_attention(q, kv, cu.cpu(), lens, tab, par, n, sc)
+        c = Batch(dev, [4], [20], 8, 2, 32, 16)
+        with pytest.raises(ValueError):
+            ops.tree_attention(*c.args())
     d = torch.zeros_like(par)
     for args in [(b.pool.data[0], cu, lens, tab, par, d, d, n), (b.pool.data, cu, lens, tab, par, d[:2], d, n),
                  (b.pool.data, cu, lens, tab, par, d, d.long(), n), (b.pool.data, cu, lens, tab, par, d, d, 0)]:
@@ -444,6 +454,7 @@ def test_moe_few_refusals(dev):
                      (x[:4], (router, w13, s13, w2.transpose(1, 2), s2, E, k))]:
         with pytest.raises(ValueError):
             ops.moe_few_tokens(xx, *args)
-    with pytest.raises(ValueError):
-        ops.moe_few_tokens(x[:4], *ok, out=x[:3])
+    for out in (x[:3], x[:4], x[2:6]):
+        with pytest.raises(ValueError):
+            ops.moe_few_tokens(x[:4], *ok, out=out)
     assert ops.moe_few_tokens(x[:0], *ok).shape == (0, H)
