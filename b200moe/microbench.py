@@ -8,6 +8,9 @@ cases:
   dense      QKV (5120x2048) and O-proj (2048x4096) block-scaled GEMMs, LM head
   decode     paged decode attention, T sequences of --ctx tokens
   prefill    paged prefill attention, T/--ctx sequences of --ctx tokens
+  tree       attention of drafted trees (--nodes each), T / --nodes sequences of --ctx tokens, and the
+             commit of their accepted paths over --pool-layers layers
+  few        one MoE layer (with its combine and norm) for T <= 64 tokens: one launch and the launches it replaces
   step       whole-model forward (eager) of T decode rows at --ctx context
   ep         one expert-parallel MoE layer per rank under torchrun (fused peer-memory path)
   tp         tensor-parallel O projection + rank sum + RMSNorm under torchrun, fused vs NCCL
@@ -310,6 +313,52 @@ def case_ops(T, iters, H=2048, nq=32, nkv=4, D=128, V=151936, topk=8):
     report("sample_topp", ms, T * V * 4, 0, rows=T, vocab=V)
 
 
+def case_tree(T, ctx, nodes, iters, nq=32, nkv=4, D=128, pool_layers=2, kv="bf16"):
+    """Random trees whose node i hangs on one of the nodes before it; every third draft is right, so
+    the commit moves short paths."""
+    B = max(1, T // nodes)
+    pool, tables = _kv(B, ctx + nodes, layers=pool_layers, kv=kv)
+    rows = B * nodes
+    q = torch.randn(rows, nq, D, device="cuda").to(torch.bfloat16)
+    cu = torch.arange(0, rows + 1, nodes, dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), ctx + nodes, dtype=torch.int32, device="cuda")
+    at = torch.arange(nodes, device="cuda")
+    par = ((torch.rand(B, nodes, device="cuda") * at).long() - (at == 0).long()).to(torch.int32).flatten()
+    draft, target = (torch.randint(0, 3, (rows,), device="cuda", dtype=torch.int32) for _ in range(2))
+    out = torch.empty_like(q)
+    ms = timeit(lambda: ops.tree_attention(q, pool.layer(0), cu, lens, tables, par, nodes, D ** -0.5, out), iters)
+    size = 2 if kv == "bf16" else 1
+    report("tree_attn", ms, B * (ctx + nodes) * nkv * D * 2 * size + 2 * rows * nq * D * 2,
+           4 * rows * ctx * nq * D, seqs=B, ctx=ctx, nodes=nodes, kv=kv)
+    fn = lambda: ops.tree_commit(pool.data, cu, lens, tables, par, draft, target, nodes, kv_scales=pool.scales,
+                                 kv_side=pool.side)
+    acc, path, _ = fn()
+    moved = int(((path != torch.arange(nodes, device="cuda")) & (path >= 0)).sum())
+    ms = timeit(fn, iters)
+    report("tree_commit", ms, 2 * moved * pool_layers * 2 * nkv * D * size, 0, seqs=B, nodes=nodes,
+           layers=pool_layers, moved=moved, kv=kv)
+
+
+def case_few(T, iters):
+    from b200moe.config import ModelArgs
+    from b200moe.models.qwen3_moe import Qwen3MoeForCausalLM
+    from b200moe.utils.weights import random_init_
+    args = ModelArgs(num_hidden_layers=1)
+    model = Qwen3MoeForCausalLM(args, "cuda")
+    random_init_(model, seed=7)
+    if TILED:
+        model.tile_weights_()
+    layer = model.layers[0]
+    x = torch.randn(T, args.hidden_size, device="cuda").to(torch.bfloat16)
+    res = torch.randn(T, args.hidden_size, device="cuda").to(torch.bfloat16)
+    used = int(torch.unique(model.route(layer, x)[0]).numel())
+    H, I, k = args.hidden_size, args.moe_intermediate_size, args.num_experts_per_tok
+    for name, rows in (("moe_layer_launches", 0), ("moe_layer_few", ops.MOE_FEW_MAX_TOKENS)):
+        model.MOE_FEW_ROWS = rows
+        ms = timeit(lambda: model._mlp(layer, x, res, model.norm, T), iters)
+        report(name, ms, used * 3 * H * I, 6 * T * k * H * I, tokens=T, experts=used)
+
+
 NVLINK_GBS = 770.0  # measured peer copy per direction on this pool's NVSwitch systems
 
 
@@ -557,15 +606,17 @@ def case_trace(T):
 
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("case", choices=["moe", "dense", "decode", "prefill", "step", "trace", "ep", "tp", "ops", "all"])
+    p.add_argument("case", choices=["moe", "dense", "decode", "prefill", "step", "trace", "ep", "tp", "ops", "tree", "few",
+                                    "all"])
     p.add_argument("--tokens", type=int, default=256)
     p.add_argument("--ctx", type=int, default=1152)
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--layers", type=int, default=48)
     p.add_argument("--splits", type=int, default=0, help="decode: force this many KV splits (0 = heuristic)")
-    p.add_argument("--pool-layers", type=int, default=2, help="decode: layers per KV block slab")
+    p.add_argument("--pool-layers", type=int, default=2, help="decode / tree: layers per KV block slab")
+    p.add_argument("--nodes", type=int, default=16, help="tree: nodes of a drafted tree")
     p.add_argument("--only", choices=["", "gate_up", "down"], default="", help="moe: time one of the two GEMMs")
-    p.add_argument("--kv", choices=["bf16", "int8", "int8-channel"], default="bf16", help="decode / prefill: pool type")
+    p.add_argument("--kv", choices=["bf16", "int8", "int8-channel"], default="bf16", help="decode / prefill / tree: pool type")
     a = p.parse_args()
     if a.case == "ep":
         return case_ep(a.tokens, a.iters)
@@ -580,6 +631,10 @@ def main():
         case_decode(a.tokens, a.ctx, a.iters, splits=a.splits, pool_layers=a.pool_layers, kv=a.kv)
     if a.case in ("prefill", "all"):
         case_prefill(max(a.tokens, a.ctx), a.ctx, a.iters, kv=a.kv)
+    if a.case in ("tree", "all"):
+        case_tree(a.tokens, a.ctx, a.nodes, a.iters, pool_layers=a.pool_layers, kv=a.kv)
+    if a.case in ("few", "all"):
+        case_few(min(a.tokens, ops.MOE_FEW_MAX_TOKENS), a.iters)
     if a.case == "trace":
         case_trace(a.tokens)
     if a.case == "step":

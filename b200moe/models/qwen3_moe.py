@@ -39,7 +39,10 @@ from b200moe.engine.kv_cache import KVPool
 class StepInputs:
     """Device-side description of one forward step (rows = sequences).
 
-    Decode rows (one query token) come first, then prefill rows.
+    Decode rows (one query token) come first, then prefill rows.  With ``tree_parents`` the prefill
+    rows are drafted trees: token i of a row is a node whose key is stored at slot P + i behind the
+    row's committed prefix P, whose position is P + its depth, and which sees the prefix, its ancestors
+    and itself (``ops.tree_attention``).
     """
     input_ids: torch.Tensor        # int32 [T]
     positions: torch.Tensor        # int32 [T]
@@ -55,6 +58,7 @@ class StepInputs:
     prefill_cu: torch.Tensor | None = None  # cu_seqlens of the prefill rows, rebased to 0
     feed_src: torch.Tensor | None = None    # int32 [T]: >= 0 -> the id is feed_tokens[feed_src[t]]
     feed_tokens: torch.Tensor | None = None  # previous step's sampled tokens (device)
+    tree_parents: torch.Tensor | None = None  # int32, one per token of the prefill rows: a node's parent in its tree
 
     @property
     def num_tokens(self) -> int:
@@ -263,6 +267,8 @@ class Qwen3MoeForCausalLM(nn.Module):
             self._buf("slot_of_row", (rows,), torch.int32)
             self._buf("ids", (max_tokens * k,), torch.int32)
             self._buf("topw", (max_tokens * k,), torch.float32)
+            if self.MOE_FEW_ROWS > 0:
+                self._buf("moe_few", (min(max_tokens, ops.MOE_FEW_MAX_TOKENS), H), self.dtype)
         self._buf("h_perm", (max(rows, max_tokens), I), self.dtype)
         if self._bf16_experts(rows) and self.layers and getattr(self.layers[0], "w13_bf16", None) is None:
             l0 = self.layers[0]
@@ -282,6 +288,17 @@ class Qwen3MoeForCausalLM(nn.Module):
 
     def _range(self, name: str):
         return nullcontext() if self.profiler is None else self.profiler.range(name)
+
+    # Tokens of a step up to which an MoE layer runs as one launch (ops.moe_few_tokens, at most
+    # ops.MOE_FEW_MAX_TOKENS) instead of router, permute, two grouped GEMMs and combine.  0: never.
+    MOE_FEW_ROWS = int(os.environ.get("B200MOE_MOE_FEW_ROWS", "0"))
+
+    def _moe_few(self, layer, T: int) -> bool:
+        a = self.args
+        return (T <= min(self.MOE_FEW_ROWS, ops.MOE_FEW_MAX_TOKENS) and self.ep is None
+                and layer.router.dtype == torch.bfloat16 and a.num_experts <= ops.MOE_FEW_MAX_EXPERTS
+                and a.num_experts_per_tok <= ops.MOE_FEW_MAX_TOPK
+                and all(n % 128 == 0 and n <= ops.MOE_FEW_MAX_HIDDEN for n in (a.hidden_size, layer.w2.shape[-1])))
 
     # -------------------------------------------------------------- forward
     @torch.inference_mode()
@@ -324,6 +341,20 @@ class Qwen3MoeForCausalLM(nn.Module):
             x = self._mlp(layer, x, residual, nxt, T)
         return x.index_select(0, inp.logits_indices.long())
 
+    @torch.inference_mode()
+    def verify_trees(self, inp: StepInputs, kv: KVPool):
+        """One greedy verification step of drafted trees (``inp.tree_parents``, no decode rows, every
+        token's logits wanted): the forward pass over all nodes, the token the model picks behind each,
+        and the accepted path of every tree, whose cache rows move behind the prefix.  Returns what
+        ``ops.tree_commit`` returns: (accepted [B], path, tokens [B, max_q_len])."""
+        if inp.tree_parents is None or inp.num_decode or inp.feed_src is not None:
+            raise ValueError("verify_trees takes tree rows only, with their drafted tokens in input_ids")
+        if inp.logits_indices.shape[0] != inp.num_tokens:
+            raise ValueError("verify_trees needs the logits of every node, in order")
+        picked = ops.argmax(self.compute_logits(self(inp, kv)))
+        return ops.tree_commit(kv.data, inp.cu_seqlens_q, inp.seq_lens, inp.block_tables, inp.tree_parents,
+                               inp.input_ids, picked, inp.max_q_len, kv_scales=kv.scales, kv_side=kv.side)
+
     def compute_logits(self, h: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """fp32 logits [rows, vocab] (LM head on the tcgen05 GEMM, bf16 weights)."""
         return ops.linear(h, self.lm_head, None, out_dtype=torch.float32, out=out)
@@ -348,7 +379,10 @@ class Qwen3MoeForCausalLM(nn.Module):
                 if nd:
                     ops._attention_ref(q[:nd], kvl, inp.block_tables[:nd], inp.seq_lens[:nd],
                                        torch.arange(nd + 1, dtype=torch.int32), self.scale, out[:nd])
-                if inp.num_rows > nd:
+                if inp.num_rows > nd and inp.tree_parents is not None:
+                    ops._tree_attention_ref(q[nd:], kvl, cu, inp.seq_lens[nd:], inp.block_tables[nd:],
+                                            inp.tree_parents, self.scale, out[nd:])
+                elif inp.num_rows > nd:
                     ops._attention_ref(q[nd:], kvl, inp.block_tables[nd:], inp.seq_lens[nd:], cu, self.scale,
                                        out[nd:])
             else:
@@ -361,7 +395,10 @@ class Qwen3MoeForCausalLM(nn.Module):
                               self._buf("part_l", (nd * nq * nsplit,), torch.float32))
                     ops.decode_attention(q[:nd], kvl, inp.block_tables[:nd], inp.seq_lens[:nd], self.scale,
                                          out[:nd], split_len, nsplit, ws)
-                if inp.num_rows > nd:
+                if inp.num_rows > nd and inp.tree_parents is not None:
+                    ops.tree_attention(q[nd:], kvl, cu, inp.seq_lens[nd:], inp.block_tables[nd:], inp.tree_parents,
+                                       inp.max_q_len, self.scale, out[nd:])
+                elif inp.num_rows > nd:
                     ops.prefill_attention(q[nd:], kvl, cu, inp.seq_lens[nd:], inp.block_tables[nd:],
                                           inp.max_q_len, self.scale, out[nd:])
         return out.view(T, nq * D)  # the O projection is applied by the caller
@@ -387,6 +424,14 @@ class Qwen3MoeForCausalLM(nn.Module):
             moe_out = self._moe_reference(layer, x)
             return ops.rmsnorm(moe_out, next_norm, eps, residual=residual,
                                out=self._buf("x", (T, a.hidden_size), self.dtype) if self.cuda else None)
+        if self._moe_few(layer, T):
+            with self._range("moe.few_tokens"):
+                y = ops.moe_few_tokens(x, layer.router, layer.w13, layer.s13, layer.w2, layer.s2, a.num_experts,
+                                       a.num_experts_per_tok, a.norm_topk_prob,
+                                       out=self._buf("moe_few", (T, a.hidden_size), self.dtype),
+                                       tiled=self.weights_tiled)
+            return ops.rmsnorm(y, next_norm, eps, residual=residual,
+                               out=self._buf("x", (T, a.hidden_size), self.dtype))
         slots = self._moe_fused(layer, x, T)
         with self._range("moe.combine_norm"):
             # the combine kernel also clears the routing counters for the next layer

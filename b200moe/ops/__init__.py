@@ -490,7 +490,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
 
 
-MOE_FEW_MAX_TOKENS = 64
+MOE_FEW_MAX_TOKENS, MOE_FEW_MAX_EXPERTS, MOE_FEW_MAX_TOPK, MOE_FEW_MAX_HIDDEN = 64, 256, 8, 8192
 
 
 def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True, out=None, ids=None, weights=None,
@@ -514,8 +514,8 @@ def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True
     if w13.dim() != 3 or w2.dim() != 3 or w13.shape != (num_experts, 2 * w2.shape[2], H) or w2.shape[:2] != (
             num_experts, H):
         raise ValueError("w13 must be [E, 2I, H] and w2 [E, H, I]")
-    if not 1 <= topk <= min(8, num_experts) or num_experts > 256:
-        raise ValueError("topk must be in [1, min(8, num_experts)] and num_experts at most 256")
+    if not 1 <= topk <= min(MOE_FEW_MAX_TOPK, num_experts) or num_experts > MOE_FEW_MAX_EXPERTS:
+        raise ValueError(f"topk must be in [1, min({MOE_FEW_MAX_TOPK}, experts)], experts at most {MOE_FEW_MAX_EXPERTS}")
     if (s13 is None) != (s2 is None) or (s13 is None) == (w13.dtype == torch.float8_e4m3fn) or w2.dtype != w13.dtype:
         raise ValueError("expert weights are both e4m3 with scales or both unquantised without")
     if out is None:

@@ -6,8 +6,10 @@ import pytest
 import torch
 
 from b200moe import ops
+from b200moe.config import preset_args
 from b200moe.engine.kv_cache import KVPool
-from b200moe.utils.weights import quantize_block_fp8
+from b200moe.models.qwen3_moe import Qwen3MoeForCausalLM, StepInputs
+from b200moe.utils.weights import quantize_block_fp8, random_init_
 
 HALF = torch.finfo(torch.bfloat16).eps / 2   # a bf16 rounding is off by at most this, relative to the value
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -458,3 +460,239 @@ def test_moe_few_refusals(dev):
         with pytest.raises(ValueError):
             ops.moe_few_tokens(x[:4], *ok, out=out)
     assert ops.moe_few_tokens(x[:0], *ok).shape == (0, H)
+
+
+# ------------------------------------------------------------------ together, in the model
+class Decoder:
+    """Sequences with a block table each, stepped through a tiny model."""
+
+    def __init__(self, dev, prompts, preset="tiny-moe", int8=False, blocks=12, bs=16):
+        self.args = preset_args(preset)
+        self.dev, self.bs = dev, bs
+        self.model = Qwen3MoeForCausalLM(self.args, dev)
+        random_init_(self.model, seed=5, std=0.1)
+        self.model.reserve_workspace(256, 16, 8)
+        a = self.args
+        self.pool = KVPool(len(prompts) * blocks + 1, a.num_hidden_layers, a.num_key_value_heads, bs, a.head_dim,
+                           self.model.dtype, dev, int8=int8)
+        g = torch.Generator().manual_seed(1)
+        self.tables = torch.randperm(len(prompts) * blocks, generator=g).view(len(prompts), blocks).tolist()
+        self.seqs = [list(p) for p in prompts]      # the last token's key is not stored yet
+
+    def inputs(self, rows, ids, parents=None, num_decode=0):
+        """rows: (sequence, keys already stored, tokens); parents per row: trees."""
+        i32 = dict(dtype=torch.int32, device=self.dev)
+        pos, slots, cu = [], [], [0]
+        for j, (s, p, n) in enumerate(rows):
+            depth = list(range(n))
+            if parents is not None:
+                for i, up in enumerate(parents[j]):
+                    depth[i] = 0 if up < 0 else depth[up] + 1
+            pos += [p + d for d in depth]
+            slots += [self.tables[s][(p + i) // self.bs] * self.bs + (p + i) % self.bs for i in range(n)]
+            cu.append(cu[-1] + n)
+        lens = [p + n for _, p, n in rows]
+        want = list(range(cu[-1])) if parents is not None else [c - 1 for c in cu[1:]]
+        return StepInputs(torch.tensor(ids, **i32), torch.tensor(pos, **i32), torch.tensor(slots, **i32),
+                          torch.tensor(cu, **i32), torch.tensor(lens, **i32),
+                          torch.tensor([self.tables[s] for s, _, _ in rows], **i32), torch.tensor(want, **i32),
+                          num_decode, max(n for _, _, n in rows), max(lens), len(rows),
+                          tree_parents=None if parents is None else
+                          torch.tensor([p for t in parents for p in t], **i32))
+
+    def prefill(self):
+        rows = [(s, 0, len(t) - 1) for s, t in enumerate(self.seqs)]
+        self.model(self.inputs(rows, [i for t in self.seqs for i in t[:-1]]), self.pool)
+
+    def greedy(self, steps):
+        for _ in range(steps):
+            rows = [(s, len(t) - 1, 1) for s, t in enumerate(self.seqs)]
+            h = self.model(self.inputs(rows, [t[-1] for t in self.seqs], num_decode=len(rows)), self.pool)
+            for t, n in zip(self.seqs, ops.argmax(self.model.compute_logits(h)).tolist()):
+                t.append(n)
+
+    def drafts(self, truth, right, g):
+        """A random tree per sequence; along one of its paths ``right`` drafts are what comes next."""
+        parents, ids = [], []
+        for s, t in enumerate(self.seqs):
+            n = int(torch.randint(2, 10, (1,), generator=g))
+            par = _tree(n, "random", g)
+            tok = [t[-1]] + torch.randint(0, self.args.vocab_size, (n - 1,), generator=g).tolist()
+            at, deep = 0, 0
+            for i in range(1, n):
+                if par[i] == at and deep < right:
+                    tok[i] = truth[s][len(t) + deep]
+                    at, deep = i, deep + 1
+            parents.append(par)
+            ids.append(tok)
+        return parents, ids
+
+    def verify(self, parents, ids):
+        rows = [(s, len(t) - 1, len(p)) for s, (t, p) in enumerate(zip(self.seqs, parents))]
+        inp = self.inputs(rows, [i for t in ids for i in t], parents)
+        acc, path, tokens = self.model.verify_trees(inp, self.pool)
+        for t, a, tok in zip(self.seqs, acc.tolist(), tokens.tolist()):
+            t += tok[:a]
+        return acc.tolist()
+
+
+PROMPTS = [[5, 900, 33, 7], [1, 2], list(range(40, 75)), [8] * 17]
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_verified_trees_emit_the_greedy_tokens(int8):
+    """Steps that verify trees emit what one decode step per token emits (fp32 model on the CPU)."""
+    ref, got = Decoder("cpu", PROMPTS, int8=int8), Decoder("cpu", PROMPTS, int8=int8)
+    ref.prefill()
+    ref.greedy(40)
+    got.prefill()
+    g = torch.Generator().manual_seed(2)
+    steps = []
+    for _ in range(5):
+        steps += got.verify(*got.drafts(ref.seqs, 4, g))
+    for a, b, p in zip(got.seqs, ref.seqs, PROMPTS):
+        assert a == b[:len(a)] and len(a) >= len(p) + 5
+    assert max(steps) > 2                            # paths were accepted
+    # The rows kept are those of the sequences.  A layer-0 row depends on its token and position alone: it is
+    # rounded to bf16, where the fp32 noise of another batch size (2^-20) may fall on the other side of a
+    # border (one step, 2 HALF of the value); the int8 pool adds one step of the row's scale, amax / 127.
+    for s, t in enumerate(got.seqs):
+        for x, y in zip(*(d.pool.layer(0).gather(torch.tensor(d.tables[s]), len(t) - 1) for d in (got, ref))):
+            lim = 2 * HALF * x.abs() + 2 ** -20
+            if int8:
+                lim = x.abs().amax(-1, keepdim=True) * (1.01 / 127 + 2 * HALF)
+            assert bool(((x - y).abs() <= lim).all())
+
+
+def test_verify_refuses_other_steps():
+    d = Decoder("cpu", PROMPTS)
+    rows = [(s, len(t) - 1, 1) for s, t in enumerate(d.seqs)]
+    with pytest.raises(ValueError):
+        d.model.verify_trees(d.inputs(rows, [t[-1] for t in d.seqs], num_decode=len(rows)), d.pool)
+    inp = d.inputs(rows, [t[-1] for t in d.seqs], [[-1]] * len(rows))
+    inp.logits_indices = inp.logits_indices[:2]
+    with pytest.raises(ValueError):
+        d.model.verify_trees(inp, d.pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("preset,int8,few", [("tiny-moe-fp8", False, 0), ("tiny-moe-fp8", False, 64),
+                                             ("tiny-moe", False, 64), ("tiny-moe-fp8", True, 64)])
+def test_verified_trees_in_the_model_gpu(monkeypatch, preset, int8, few):
+    """Every operator call inside a verification step, on what the model hands it, against the exact values."""
+    d = Decoder("cuda", PROMPTS, preset, int8=int8)
+    d.model.MOE_FEW_ROWS = few
+    d.prefill()
+    seen = {"attn": 0, "moe": 0, "commit": 0}
+    attn, moe, commit = ops.tree_attention, ops.moe_few_tokens, ops.tree_commit
+    g = torch.Generator().manual_seed(2)
+
+    def check_attn(q, layer, cu, lens, tables, parents, max_q, scale, out):
+        got = attn(q, layer, cu, lens, tables, parents, max_q, scale, out)
+        b = Batch.__new__(Batch)
+        b.q, b.layer, b.scale, b.tables, b.nq = q, layer, scale, tables, q.shape[1]
+        b.cu_list, b.nkv = cu.tolist(), layer.num_kv_heads
+        b.nodes = [y - x for x, y in zip(b.cu_list, b.cu_list[1:])]
+        b.ctx = [n - k for n, k in zip(lens.tolist(), b.nodes)]
+        b.trees = [parents.tolist()[x:y] for x, y in zip(b.cu_list, b.cu_list[1:])]
+        b.check(got)
+        seen["attn"] += 1
+        return got
+
+    def check_moe(x, router, w13, s13, w2, s2, E, k, renorm, out, tiled):
+        ids = torch.empty(x.shape[0], k, dtype=torch.int32, device=x.device)
+        wts = torch.empty(x.shape[0], k, device=x.device)
+        moe(x, router, w13, s13, w2, s2, E, k, renorm, out=out, ids=ids, weights=wts, tiled=tiled)
+        _moe_check(x, router, w13, s13, w2, s2, E, k, renorm, out, ids, wts)
+        seen["moe"] += 1
+        return out
+
+    def check_commit(data, cu, lens, tables, parents, draft, target, max_q, kv_scales=None, kv_side=None):
+        b = Batch.__new__(Batch)
+        b.cu_list, b.tables, b.pool = cu.tolist(), tables, d.pool
+        b.nodes = [y - x for x, y in zip(b.cu_list, b.cu_list[1:])]
+        b.ctx = [n - k for n, k in zip(lens.tolist(), b.nodes)]
+        b.trees = [parents.tolist()[x:y] for x, y in zip(b.cu_list, b.cu_list[1:])]
+        paths, toks = _commit_expect(b, draft, target)
+        kept = [t for t in (data, kv_scales, kv_side) if t is not None]
+        want = [_commit_moved(b, paths, t) for t in kept]
+        res = commit(data, cu, lens, tables, parents, draft, target, max_q, kv_scales=kv_scales, kv_side=kv_side)
+        assert res[0].tolist() == [len(p) for p in paths]
+        assert [t[:len(p)] for t, p in zip(res[2].tolist(), paths)] == toks
+        for t, w in zip(kept, want):
+            assert torch.equal(t, w)
+        seen["commit"] += 1
+        return res
+
+    monkeypatch.setattr(ops, "tree_attention", check_attn)
+    monkeypatch.setattr(ops, "moe_few_tokens", check_moe)
+    monkeypatch.setattr(ops, "tree_commit", check_commit)
+    truth = [t + list(range(1, 99)) for t in d.seqs]
+    for _ in range(3):
+        d.verify(*d.drafts(truth, 4, g))
+    layers = d.args.num_hidden_layers
+    assert seen == {"attn": 3 * layers, "moe": 3 * layers if few else 0, "commit": 3}
+    ops.check_status(d.pool.data.device)
+
+
+@pytest.mark.gpu
+def test_verify_step_replays_from_a_graph():
+    """A captured step (three operators on their workspaces) run over new inputs in its buffers gives what
+    the eager step gives."""
+    g = torch.Generator().manual_seed(4)
+    eager, graph = Decoder("cuda", PROMPTS, "tiny-moe-fp8"), Decoder("cuda", PROMPTS, "tiny-moe-fp8")
+    n = 6
+    for d in (eager, graph):
+        d.model.MOE_FEW_ROWS = 64
+        d.prefill()
+
+    def step_inputs(d, trees, ids):
+        return d.inputs([(s, len(t) - 1, n) for s, t in enumerate(d.seqs)], [i for t in ids for i in t], trees)
+
+    batches = [([_tree(n, "random", g) for _ in PROMPTS],
+                [torch.randint(0, 1000, (n,), generator=g).tolist() for _ in PROMPTS]) for _ in range(3)]
+    static = step_inputs(graph, *batches[0])
+    start = graph.pool.data.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.model.verify_trees(static, graph.pool)     # warm-up
+    torch.cuda.current_stream().wait_stream(side)
+    cg = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(cg):
+        res = graph.model.verify_trees(static, graph.pool)
+    graph.pool.data.copy_(start)
+    for trees, ids in batches:
+        want = eager.model.verify_trees(step_inputs(eager, trees, ids), eager.pool)
+        new = step_inputs(graph, trees, ids)
+        for name in ("input_ids", "positions", "slot_mapping", "seq_lens", "tree_parents"):
+            getattr(static, name).copy_(getattr(new, name))
+        cg.replay()
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+        assert torch.equal(eager.pool.data, graph.pool.data)
+        for d in (eager, graph):
+            for t, a, tok in zip(d.seqs, want[0].tolist(), want[2].tolist()):
+                t += tok[:a]
+    ops.check_status(static.input_ids.device)
+
+
+@pytest.mark.gpu
+def test_operators_on_two_streams():
+    """Calls in flight on two streams at once keep their results: each has its own workspace."""
+    b = [Batch("cuda", [64, 3], [3000, 200], 32, 4, 128, 64, seed=s) for s in range(2)]
+    m = [_moe_weights("cuda", 24, 256, 128, True, seed=s) for s in range(2)]
+    x = [torch.randn(32, 256, generator=torch.Generator().manual_seed(s)).to("cuda", torch.bfloat16) for s in range(2)]
+    want = [(ops.tree_attention(*b[i].args()), ops.moe_few_tokens(x[i], *m[i], 24, 4)) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((ops.tree_attention(*b[i].args()), ops.moe_few_tokens(x[i], *m[i], 24, 4)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, y in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(y, want[i][1])
+    ops.check_status(x[0].device)
