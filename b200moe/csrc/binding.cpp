@@ -6,6 +6,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <tuple>
@@ -794,7 +795,8 @@ void check_tree(const Tensor& cu, const Tensor& lens, const Tensor& tables, cons
 Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k_scale,
                  c10::optional<Tensor> v_scale, Tensor cu, Tensor lens, Tensor tables, Tensor parents,
                  c10::optional<Tensor> out_arg, int64_t max_q_len, int64_t block_size, int64_t block_stride,
-                 int64_t scale_block_stride, double scale, Tensor status, std::vector<int64_t> chan) {
+                 int64_t scale_block_stride, double scale, Tensor status, std::vector<int64_t> chan,
+                 int64_t stage_limit) {
   check_contiguous(q, "q"); check_bf16(q, "q");
   Tensor out = out_arg.has_value() ? *out_arg : torch::empty_like(q);
   check_contiguous(out, "out"); check_bf16(out, "out");
@@ -859,7 +861,16 @@ Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor>
   if (b200::tree_attn_tc_plan(a, (int)max_q_len, &plan)) {
     Tensor ws = torch::empty({plan.workspace_bytes}, q.options().dtype(torch::kUInt8));
     plan.workspace = ws.data_ptr();
-    b200::tree_attn_tc(a, plan, stream());
+    if (a.kv_int8) {
+      // as many sequences at a time as the stage may hold, at least one
+      const int most = std::min(a.batch, b200::kTreeTcBatch);
+      const int64_t one = b200::tree_stage_bytes(a, 1);
+      const int seqs = (int)std::min<int64_t>(most, std::max<int64_t>(1, stage_limit / one));
+      Tensor stage = torch::empty({b200::tree_stage_bytes(a, seqs)}, q.options().dtype(torch::kUInt8));
+      b200::tree_attn_staged(a, plan, seqs, stage.data_ptr(), stream());
+    } else {
+      b200::tree_attn_tc(a, plan, stream());
+    }
   } else {
     b200::tree_attn(a, stream());
   }

@@ -40,8 +40,8 @@ struct TreeAttnArgs {
 };
 void tree_attn(const TreeAttnArgs& a, cudaStream_t s);
 
-// Tensor-core form (kernels/tree_attn_tc.cu): bf16 pool, head_dim 64 or 128, blocks that
-// hold whole tiles of 128 keys or divide one in multiples of 8 rows.
+// Tensor-core form (kernels/tree_attn_tc.cu): head_dim 64 or 128, blocks that hold whole
+// tiles of 64 keys or divide one in multiples of 8 rows.
 constexpr int kTreeTcBatch = 1024;   // sequences of one launch
 struct TreeAttnTcPlan {
   int sub_rows;              // key rows of one TMA box
@@ -49,10 +49,17 @@ struct TreeAttnTcPlan {
   int grid;
   int64_t workspace_bytes;
   void* workspace;           // 16-byte aligned
+  const float* key_scales;   // staged int8 values: [batch][kv_heads][k | v][key_stride], else null
+  int key_stride;            // a multiple of 64
 };
 // False where the shape is not the tensor-core kernel's.
 bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p);
 void tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s);
+
+// int8 pools (kernels/tree_stage.cu): the keys and values of up to `seqs` sequences at a time go
+// to a bf16 stage that the tensor-core form reads.
+int64_t tree_stage_bytes(const TreeAttnArgs& a, int seqs);
+void tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, void* stage, cudaStream_t s);
 
 // One kind of rows the commit moves: [blocks, planes, block_size, row_bytes], contiguous.
 struct TreeRows {

@@ -90,6 +90,8 @@ struct TcArgs {
   float2* part_ml;   // [grid][2][part_rows]
   int part_rows;     // 128 or 256
   int sub_rows;
+  const float* key_scales;   // SCALED: [batch][kv_heads][k | v][key_stride]
+  int key_stride;
 };
 
 __device__ __forceinline__ uint32_t sw_off(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
@@ -342,7 +344,9 @@ struct Blocks {
   }
 };
 
-template <int D>
+// SCALED: K and V hold int8 values (exact in bf16), one factor for each key and one for each value row
+// apply to the scores and to P.
+template <int D, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                     const __grid_constant__ CUtensorMap q_map, const TcArgs t) {
@@ -750,6 +754,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       float m = -INFINITY, l = 0.f;
       const Own own(g, gt, w);
       const int done = own.n;
+      const float* factors = SCALED ? t.key_scales + ((int64_t)g.b * a.num_kv_heads + g.h) * 2 * t.key_stride : nullptr;
 #pragma unroll 1
       for (int i = 0; i < own.n; ++i, ++mine) {
         const int buf = mine & 1;
@@ -763,6 +768,16 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           tmem_ld<32>(tb, s);
           tmem_ld<32>(tb + 32, s + 32);
           tmem_ld_wait();
+          if constexpr (SCALED) {
+#pragma unroll
+            for (int e = 0; e < kKeys; e += 4) {
+              const float4 f = __ldg(reinterpret_cast<const float4*>(factors + kb + e));
+              s[e] *= f.x;
+              s[e + 1] *= f.y;
+              s[e + 2] *= f.z;
+              s[e + 3] *= f.w;
+            }
+          }
           if (kb + kKeys > prefix) {
             const uint32_t lo = sees(kb, 0), hi = sees(kb, 32);
 #pragma unroll
@@ -814,9 +829,17 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const float2 z = fma2(make_float2(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), k2, mu2);
-              p[e] = pack2(ex2(z.x), ex2(z.y));
-              const float2 back = make_float2(__uint_as_float(p[e] << 16), __uint_as_float(p[e] & 0xffff0000u));
-              if (e & 1) sum1 = add2(sum1, back); else sum0 = add2(sum0, back);
+              if constexpr (SCALED) {
+                // (the sum takes P as it is; a place without weight takes no part, whatever its factor)
+                const float2 x = make_float2(ex2(z.x), ex2(z.y));
+                const float2 f = __ldg(reinterpret_cast<const float2*>(factors + t.key_stride + kb + q * 32 + 2 * e));
+                p[e] = pack2(x.x == 0.f ? 0.f : x.x * f.x, x.y == 0.f ? 0.f : x.y * f.y);
+                if (e & 1) sum1 = add2(sum1, x); else sum0 = add2(sum0, x);
+              } else {
+                p[e] = pack2(ex2(z.x), ex2(z.y));
+                const float2 back = make_float2(__uint_as_float(p[e] << 16), __uint_as_float(p[e] & 0xffff0000u));
+                if (e & 1) sum1 = add2(sum1, back); else sum0 = add2(sum0, back);
+              }
             }
             tmem_st16(tb + q * 16, p);           // P overlays its scores, which this thread has read
           }
@@ -1045,7 +1068,7 @@ void encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims
   if (r != CUDA_SUCCESS) throw std::runtime_error("tree attention tensor map: encode failed " + std::to_string((int)r));
 }
 
-template <int D>
+template <int D, bool SCALED>
 void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
   CUtensorMap km, vm, qm;
   // columns as (64, D / 64): one copy brings both halves of a tile
@@ -1063,6 +1086,8 @@ void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
   t.a = a;
   t.part_rows = p.part_rows;
   t.sub_rows = p.sub_rows;
+  t.key_scales = p.key_scales;
+  t.key_stride = p.key_stride;
   t.part_o = static_cast<float*>(p.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + (int64_t)p.grid * 2 * p.part_rows * D);
   // slices of the batch that fit the shared table of units (one launch for up to kTreeTcBatch sequences)
@@ -1072,10 +1097,10 @@ void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
     t.a.seq_lens = a.seq_lens + b0;
     t.a.block_tables = a.block_tables + (int64_t)b0 * a.max_blocks;
     const int smem = Lay<D>::smem(kTreeTcBatch);
-    smem_opt_in(tree_attn_tc_kernel<D>, smem);
+    smem_opt_in(tree_attn_tc_kernel<D, SCALED>, smem);
     void* params[] = {&km, &vm, &qm, &t};
-    const cudaError_t e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(tree_attn_tc_kernel<D>), dim3(p.grid),
-                                                      dim3(kThreads), params, smem, s);
+    const cudaError_t e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(tree_attn_tc_kernel<D, SCALED>),
+                                                      dim3(p.grid), dim3(kThreads), params, smem, s);
     if (e != cudaSuccess) throw std::runtime_error(std::string("tree_attn: ") + cudaGetErrorString(e));
   }
 }
@@ -1083,7 +1108,7 @@ void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
 }  // namespace
 
 bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p) {
-  if (a.kv_int8 || (a.head_dim != 64 && a.head_dim != 128) || a.group > kRows || a.num_blocks <= 0) return false;
+  if ((a.head_dim != 64 && a.head_dim != 128) || a.group > kRows || a.num_blocks <= 0) return false;
   if (a.block_size % kKeys == 0) p->sub_rows = kKeys;
   else if (kKeys % a.block_size == 0 && a.block_size % 8 == 0) p->sub_rows = a.block_size;
   else return false;
@@ -1098,8 +1123,13 @@ bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p) 
 }
 
 void tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
-  if (a.head_dim == 128) launch<128>(a, p, s);
-  else launch<64>(a, p, s);
+  if (p.key_scales != nullptr) {
+    if (a.head_dim == 128) launch<128, true>(a, p, s);
+    else launch<64, true>(a, p, s);
+  } else {
+    if (a.head_dim == 128) launch<128, false>(a, p, s);
+    else launch<64, false>(a, p, s);
+  }
 }
 
 }  // namespace b200

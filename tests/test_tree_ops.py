@@ -168,6 +168,51 @@ def test_tree_attention_int8(dev, mode, D, bs):
     b.check(ops.tree_attention(*b.args()))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["token", "channel"])
+@pytest.mark.parametrize("limit", [None, 1, 3 << 20])
+@pytest.mark.parametrize("nodes,ctx,nq,nkv,D,bs", [
+    ([64], [9000], 32, 4, 128, 256), ([5, 0, 17, 1, 40], [0, 7, 130, 1500, 255], 8, 2, 64, 8),
+    ([3, 90, 31], [5000, 777, 1290], 16, 2, 128, 32), ([4, 3, 2], [50, 77, 9], 4, 2, 64, 24),
+])
+def test_tree_attention_int8_large(monkeypatch, mode, limit, nodes, ctx, nq, nkv, D, bs):
+    """The whole batch, one sequence, or some of them at a time in the bf16 stage; a block size without one."""
+    if limit is not None:
+        monkeypatch.setattr(ops, "INT8_STAGE_MAX_BYTES", limit)
+    b = Batch("cuda", nodes, ctx, nq, nkv, D, bs, int8=True, mode=mode, pad=2)
+    out = torch.full_like(b.q, 7.0)
+    b.check(ops.tree_attention(*b.args(), out=out))
+    assert bool((out[-2:] == 7.0).all())
+    ops.check_status(out.device)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_attention_int8_ignores_what_it_does_not_see(dev):
+    """NaN factors behind the sequence and in other branches change nothing."""
+    b = Batch(dev, [6], [25], 8, 2, 128, 16, "star", int8=True)
+    want = ops.tree_attention(*b.args()).clone()
+    last, node = b.tables[0, 30 // 16].item(), 25 + 4
+    for sc in (b.layer.k_scale, b.layer.v_scale):
+        sc[last, :, 15:] = math.nan
+        sc[b.tables[0, node // 16].item(), :, node % 16] = math.nan
+    got = ops.tree_attention(*b.args())
+    keep = [i for i in range(6) if i != 4]
+    assert torch.equal(got[keep], want[keep])
+    assert bool(torch.isnan(got[4].float()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["token", "channel"])
+def test_tree_int8_bad_block_sets_status(mode):
+    b = Batch("cuda", [4, 3], [40, 20], 8, 2, 128, 16, int8=True, mode=mode)
+    want = ops.tree_attention(*b.args()).clone()
+    b.tables[0, 0], b.tables[0, 1] = 1 << 20, -5
+    got = ops.tree_attention(*b.args())
+    assert torch.equal(got[4:], want[4:])
+    with pytest.raises(RuntimeError):
+        ops.check_status(got.device)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_tree_attention_chain_is_prefill(dev):
     """A chain sees what causal prefill sees."""
