@@ -217,8 +217,8 @@ __device__ __forceinline__ void few_topk(const MoeFewArgs& a, int t, int lane, i
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = j * 32 + lane;
-    // (logit, lowest id first) as one unsigned key: bf16 bits in order, then 0xffff - id
-    uint32_t u = __float_as_uint(v[j]) >> 16;
+    // (logit, lowest id first) as one unsigned key: bf16 bits in order (-0 as 0), then 0xffff - id
+    uint32_t u = __float_as_uint(v[j] + 0.f) >> 16;
     u = (u & 0x8000u) ? (0xffffu ^ u) : (u | 0x8000u);
     key[j] = e < a.E ? (u << 16) | (0xffffu - e) : 0u;
   }
