@@ -26,7 +26,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256, kPer = 4;               // chunks of 16 values a thread has in flight
 constexpr int kPiece = kThreads * kPer;               // chunks of one piece of work
-constexpr int kCtasPerSm = 8;
+constexpr int kCtasPerSm = 32;                       // launched, about five of them resident: shares of a block each
 
 struct Stage {
   bf16* kv;          // [seqs * max_blocks][k | v][kv_heads][block_size][D]
@@ -38,6 +38,13 @@ struct Stage {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// 32 bytes in one store: two of 16 would each write half of every sector
+__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // Four int8 values as fp32: a biased byte in the low mantissa bits of 2^23, minus 2^23 + 128.
@@ -109,8 +116,7 @@ __global__ void __launch_bounds__(kThreads) tree_stage_kernel(const TreeAttnArgs
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[e] = __byte_perm(__float_as_uint(f[2 * e]), __float_as_uint(f[2 * e + 1]), 0x7632);
       }
-      dst[2 * c] = make_uint4(out[0], out[1], out[2], out[3]);
-      dst[2 * c + 1] = make_uint4(out[4], out[5], out[6], out[7]);
+      st32(dst + 2 * c, out);
     }
     if (piece > 0) continue;
     if (threadIdx.x == 0 && kv == 0) {
