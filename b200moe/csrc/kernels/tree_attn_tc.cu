@@ -61,7 +61,7 @@ constexpr int kRows = 128, kKeys = 64;    // of a tile
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
-constexpr int kCutTiles = 8;
+constexpr int kCutBytes = 128 << 10;   // of K that cutting an item is worth
 constexpr int kParts = 4;         // partial results in flight per lane when parts are joined
 constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
@@ -210,7 +210,7 @@ struct Plan {
   int batch, kvh, per; // sequences, KV heads, nodes per row tile
   int W, items;        // units and items in all
   int grid, share;     // CTAs with work, units of the largest share
-  int whole;           // shares end at items: nothing is cut
+  int whole;           // shares end at items: nothing is cut (a rule of the kernel's, below)
   int base, rem;       // quotient and remainder of W (items) by the CTAs
 
   __device__ __forceinline__ int nodes(int b) const { return rows[b + 1].q0 - rows[b].q0; }
@@ -322,24 +322,31 @@ struct Blocks {
       ids_next = entry(window + 32 + lane);
     }
     const uint32_t dst = smem_u32(tile);
-    for (int row = 0; row < kKeys; row += sub_rows) {
-      // a block of the window or of the next one (a tile has at most eight)
-      const int d = bi - window, a0 = __shfl_sync(0xffffffffu, ids, d & 31), a1 = __shfl_sync(0xffffffffu, ids_next, d & 31);
-      const int id = d < 32 ? a0 : a1;
-      int blk = num_blocks;          // out of range: zero fill
-      if (key + row < len) {
-        if (id >= 0 && id < num_blocks) blk = id;
-        else bad = true;
-      }
-      // (a box of fewer rows than the tile has its halves that many rows apart: one copy for each)
-      if (lane == 0) {
-        if (sub_rows == kKeys) tma_5d(dst, map, bar, 0, y, 0, h, blk);
-        else
-#pragma unroll
-          for (int hf = 0; hf < D / 64; ++hf) tma_5d(dst + hf * L::HALF + row * 128, map, bar, 0, y, hf, h, blk);
-      }
-      y += sub_rows;
+    if (sub_rows == kKeys) {
+      // a box of the whole tile
+      const int id = __shfl_sync(0xffffffffu, ids, bi - window);
+      const bool in = id >= 0 && id < num_blocks;
+      if (!in) bad = true;
+      if (lane == 0) tma_5d(dst, map, bar, 0, y, 0, h, in ? id : num_blocks);   // out of range: zero fill
+      y += kKeys;
       if (y >= block_size) { y = 0; ++bi; }
+    } else {
+      // whole blocks, at most eight, each half of the columns by a lane of its own: one lane's copies
+      // one after the other held pages of 16 keys at 4.1 TB/s
+      const int row = lane / (D / 64) * sub_rows, hf = lane % (D / 64);
+      const int d = bi - window + lane / (D / 64);
+      const int a0 = __shfl_sync(0xffffffffu, ids, d & 31), a1 = __shfl_sync(0xffffffffu, ids_next, d & 31);
+      if (row < kKeys) {
+        const int id = d < 32 ? a0 : a1;
+        int blk = num_blocks;
+        if (key + row < len) {
+          if (id >= 0 && id < num_blocks) blk = id;
+          else bad = true;
+        }
+        tma_5d(dst + hf * L::HALF + row * 128, map, bar, 0, 0, hf, h, blk);
+      }
+      __syncwarp();
+      bi += kKeys / sub_rows;
     }
   }
 };
@@ -462,9 +469,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   Plan plan{rows, a.batch, a.num_kv_heads, per, rows[a.batch].unit, rows[a.batch].item};
   const int max_nt = *s_max_nt;
   plan.share = (plan.W + (int)gridDim.x - 1) / (int)gridDim.x;
-  // Cutting items costs their partial results, a grid barrier and the join, worth about kCutTiles
-  // key tiles; whole items cost the rounding up of their number.
-  plan.whole = (plan.items + (int)gridDim.x - 1) / (int)gridDim.x * max_nt <= plan.share + kCutTiles;
+  // Cutting items costs their partial results, a grid barrier and the join, worth about kCutBytes of
+  // K (8 tiles at D = 128, 16 at 64); whole items cost the rounding up of their number.  4 items of 12
+  // tiles at D = 128: 15.2 us cut, 17.2 whole; 26 items of 11 tiles at D = 64: 17.3 cut, 13.8 whole.
+  plan.whole = (plan.items + (int)gridDim.x - 1) / (int)gridDim.x * max_nt <= plan.share + kCutBytes / L::TILE;
   const int spread = plan.whole ? plan.items : plan.W;
   plan.grid = min((int)gridDim.x, spread);
   plan.base = plan.grid ? spread / plan.grid : 0;
@@ -534,10 +542,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         blocks.template copy<D>(&k_map, &k_full[slot], smem + L::K + slot * L::TILE, j * kKeys, g.h, lane);
       }
     }
-    if (lane == 0) {
-      if (blocks.bad) record_status(status, kStatusBadShape);
-      settle();
-    }
+    if (blocks.bad) record_status(status, kStatusBadShape);
+    if (lane == 0) settle();
     __syncwarp();
   } else if (warp <= 2) {
     // ================================================================ MMA issuer of group w
@@ -683,10 +689,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
       if (ok && due >= 0) clean(due, (gt - 1) % kSlots);
     }
-    if (lane == 0) {
-      if (blocks.bad) record_status(status, kStatusBadShape);
-      settle();
-    }
+    if (blocks.bad) record_status(status, kStatusBadShape);
+    if (lane == 0) settle();
     __syncwarp();
   } else {
     // ================================================================ softmax group w
