@@ -61,7 +61,12 @@ constexpr int kRows = 128, kKeys = 64;    // of a tile
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
-constexpr int kCutBytes = 128 << 10;   // of K that cutting an item is worth
+// Cutting items costs their partial results, a grid barrier and the join, worth about kCutBytes of K;
+// whole items cost the rounding up of their number.
+constexpr int kCutBytes = 128 << 10;
+// Shares that end inside an item give some CTAs two segments, worth about kShareBytes of K; parts cost
+// the rounding up of their number.
+constexpr int kShareBytes = 96 << 10;
 constexpr int kParts = 4;         // partial results in flight per lane when parts are joined
 constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
@@ -148,6 +153,18 @@ __device__ __forceinline__ void tmem_ld<32>(uint32_t addr, float* v) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+template <>
+__device__ __forceinline__ void tmem_ld<16>(uint32_t addr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -201,21 +218,26 @@ struct Chunks {
 // Per sequence, in shared memory.
 struct Row {
   int q0, len;         // first row, keys
-  int unit, item;      // units and items in front of it
+  int unit, item;      // units (parts, see Plan) and items in front of it
 };
 
-// The grid's work: equal shares of the units, or whole items where that costs hardly more.
+// The grid's work, in one of three ways:
+//   whole items    nothing is cut, several items to a CTA;
+//   parts          every item in equal parts of at most `parts` tiles, one part to a CTA (fewer items than CTAs);
+//   equal shares   of the units, a share may begin and end inside an item.
 struct Plan {
   const Row* rows;     // [batch + 1]
   int batch, kvh, per; // sequences, KV heads, nodes per row tile
   int W, items;        // units and items in all
   int grid, share;     // CTAs with work, units of the largest share
-  int whole;           // shares end at items: nothing is cut (a rule of the kernel's, below)
+  int whole;           // whole items
+  int parts;           // tiles of a part, 0: not in parts
   int base, rem;       // quotient and remainder of W (items) by the CTAs
 
   __device__ __forceinline__ int nodes(int b) const { return rows[b + 1].q0 - rows[b].q0; }
   __device__ __forceinline__ int tiles(int b) const { return (rows[b].len + kKeys - 1) / kKeys; }
   __device__ __forceinline__ int pairs(int b) const { return ((nodes(b) + per - 1) / per + 1) >> 1; }
+  __device__ __forceinline__ int cuts(int nt) const { return (nt + parts - 1) / parts; }
   __device__ __forceinline__ Chunks chunks(int nt, int pr) const {
     return {whole || pr == 1 || nt <= share ? 1 : nt / share, nt};
   }
@@ -230,6 +252,7 @@ struct Plan {
   }
   // first unit of CTA c
   __device__ __forceinline__ int lo(int c) const {
+    if (parts) return min(c, grid);
     if (c >= grid) return W;
     const int x = c * base + min(c, rem);
     if (!whole || x >= items) return whole ? W : x;
@@ -274,20 +297,29 @@ __device__ __forceinline__ Seg seg_at(const Plan& p, int u, int lo, int hi) {
   g.n = p.nodes(g.b);
   const int nt = p.tiles(g.b), pr = p.pairs(g.b);
   int r = u - row.unit;
-  const int per_head = nt * pr;
-  g.h = r / per_head;
-  r -= g.h * per_head;
-  const Chunks c = p.chunks(nt, pr);
-  int start = 0, end = nt;
-  if (c.n > 1) {
-    const int ci = c.of(r / pr);
-    start = c.start(ci);
-    end = c.start(ci + 1);
+  if (p.parts) {
+    const int cuts = p.cuts(nt), item = r / cuts;
+    r -= item * cuts;
+    g.h = item / pr;
+    g.pair = item - g.h * pr;
+    g.t0 = (r * nt) / cuts;
+    g.t1 = ((r + 1) * nt) / cuts;
+  } else {
+    const int per_head = nt * pr;
+    g.h = r / per_head;
+    r -= g.h * per_head;
+    const Chunks c = p.chunks(nt, pr);
+    int start = 0, end = nt;
+    if (c.n > 1) {
+      const int ci = c.of(r / pr);
+      start = c.start(ci);
+      end = c.start(ci + 1);
+    }
+    r -= start * pr;
+    g.pair = pr == 1 ? 0 : r / (end - start);
+    g.t0 = start + r - g.pair * (end - start);
+    g.t1 = min(end, g.t0 + (hi - u));
   }
-  r -= start * pr;
-  g.pair = pr == 1 ? 0 : r / (end - start);
-  g.t0 = start + r - g.pair * (end - start);
-  g.t1 = min(end, g.t0 + (hi - u));
   g.whole = g.t0 == 0 && g.t1 == nt;
   g.two = g.n > (2 * g.pair + 1) * p.per;
   g.slot = u == lo ? 0 : 1;
@@ -379,6 +411,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_full + kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_max_nt = reinterpret_cast<int*>(tmem_slot + 2);
+  int* s_parts = s_max_nt + 1;
   Row* rows = reinterpret_cast<Row*>(smem + L::TAB);
   volatile Seg* segs = reinterpret_cast<volatile Seg*>(smem + L::SEG);
   uint32_t* anc = reinterpret_cast<uint32_t*>(smem + L::ANC);
@@ -390,6 +423,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   const int G = a.group, per = kRows / G;   // nodes per row tile
   int* status = a.status;
 
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+    tma_prefetch_desc(&q_map);
+  }
   // ---- the work of every sequence; a tree that does not fit has none
   if (threadIdx.x == 0) *s_max_nt = 0;
   __syncthreads();
@@ -468,16 +506,52 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   const uint32_t tmem = *tmem_slot;   // S0 | S1 | O0 | O1, 128 columns each
   Plan plan{rows, a.batch, a.num_kv_heads, per, rows[a.batch].unit, rows[a.batch].item};
   const int max_nt = *s_max_nt;
-  plan.share = (plan.W + (int)gridDim.x - 1) / (int)gridDim.x;
-  // Cutting items costs their partial results, a grid barrier and the join, worth about kCutBytes of
-  // K (8 tiles at D = 128, 16 at 64); whole items cost the rounding up of their number.  4 items of 12
-  // tiles at D = 128: 15.2 us cut, 17.2 whole; 26 items of 11 tiles at D = 64: 17.3 cut, 13.8 whole.
-  plan.whole = (plan.items + (int)gridDim.x - 1) / (int)gridDim.x * max_nt <= plan.share + kCutBytes / L::TILE;
-  const int spread = plan.whole ? plan.items : plan.W;
-  plan.grid = min((int)gridDim.x, spread);
-  plan.base = plan.grid ? spread / plan.grid : 0;
-  plan.rem = plan.grid ? spread % plan.grid : 0;
-  const int u_lo = plan.lo(blockIdx.x), u_hi = plan.lo(blockIdx.x + 1);
+  const int ctas = (int)gridDim.x;
+  // (the integer divisions are the longest part of this, so the small batches leave before them)
+  const int rounds = plan.items <= ctas ? 1 : (plan.items + ctas - 1) / ctas;
+  plan.share = max_nt;
+  plan.whole = rounds * max_nt <= kCutBytes / L::TILE;
+  if (!plan.whole) {
+    plan.share = (plan.W + ctas - 1) / ctas;
+    int cut = plan.share;
+    if (plan.items < ctas && max_nt < 1 << 23) {
+      // Parts of S tiles are at most W / S + items, and S (ctas - items) >= W makes that at most the CTAs.
+      // (Two tiles take the two groups as long as one.)
+      const int parts = max(2, (plan.W + ctas - plan.items - 1) / (ctas - plan.items));
+      if (parts <= plan.share + kShareBytes / L::TILE) cut = plan.parts = parts;
+    }
+    plan.whole = rounds * max_nt <= cut + kCutBytes / L::TILE;
+    if (plan.whole) plan.parts = 0;
+  }
+  if (plan.parts) {
+    // parts in front of every sequence, in the place of its units
+    if (warp == 0) {
+      int sum = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        const int mine = b < a.batch ? (rows[b + 1].item - rows[b].item) * plan.cuts(plan.tiles(b)) : 0;
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int px = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += px;
+        }
+        if (b < a.batch) rows[b].unit = sum + x - mine;
+        sum += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) *s_parts = sum;
+    }
+    __syncthreads();          // (every thread has read the number of units)
+    plan.grid = *s_parts;
+    if (threadIdx.x == 0) rows[a.batch].unit = plan.grid;
+  } else {
+    const int spread = plan.whole ? plan.items : plan.W;
+    plan.grid = min(ctas, spread);
+    plan.base = spread <= ctas ? 1 : spread / ctas;
+    plan.rem = spread <= ctas ? 0 : spread - plan.base * ctas;
+  }
+  int edge[2] = {plan.lo(blockIdx.x), plan.lo(blockIdx.x + 1)};
+  const int u_lo = edge[0], u_hi = edge[1];
   // No role is kRing segments ahead of another, so a ring of barriers tells segments apart.
   auto join_over = [&](int sg) {
     return mbar_wait(&joined[sg % kRing], (sg / kRing) & 1, status, kStatusTimeoutEmpty, abort_flag);
@@ -501,17 +575,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
   if (warp == 0) {
     // ================================================================ producer of Q and K
-    if (lane == 0) {
-      tma_prefetch_desc(&k_map);
-      tma_prefetch_desc(&q_map);
-    }
     Blocks blocks{nullptr, a.max_blocks, a.num_blocks, a.block_size, t.sub_rows};
     int gt = 0, sg = 0;   // tiles, segments
     bool ok = true;
     for (int u = u_lo; ok; ++sg) {
       Seg g{};
       if (u < u_hi) g = seg_at(plan, u, u_lo, u_hi);
-      u += g.t1 - g.t0;
+      u = plan.parts ? u_hi : u + g.t1 - g.t0;
       if (lane == 0) {
         volatile int* dst = reinterpret_cast<volatile int*>(&segs[sg % kRing]);
         const int* src = reinterpret_cast<const int*>(&g);
@@ -629,7 +699,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     __syncwarp();
   } else if (warp == 3) {
     // ================================================================ producer of V
-    if (lane == 0) tma_prefetch_desc(&v_map);
     Blocks blocks{nullptr, a.max_blocks, a.num_blocks, a.block_size, t.sub_rows};
     int gt = 0, sg = 0;
     uint32_t cleaned = 0;      // parity of each slot's v_full: it counts the tiles that had to be cleaned
@@ -814,7 +883,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 float o[16];
-                tmem_ld16(tO + c * 16, o);
+                tmem_ld<16>(tO + c * 16, o);
                 tmem_ld_wait();
                 uint32_t ou[16];
 #pragma unroll
@@ -868,15 +937,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       constexpr int kHand = D / 4;
       float4* stage = reinterpret_cast<float4*>(smem + L::Q + L::QTILE);   // [2][kHand / 4][128]
       auto hand = [&](int round) {
+        float o[kHand];
+        tmem_ld<kHand>(tO + ((w ^ 1) * 2 + round) * kHand, o);
+        tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < kHand; c += 16) {
-          float o[16];
-          tmem_ld16(tO + ((w ^ 1) * 2 + round) * kHand + c, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            stage[(w * (kHand / 4) + c / 4 + e) * kRows + r] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
+        for (int e = 0; e < kHand / 4; ++e)
+          stage[(w * (kHand / 4) + e) * kRows + r] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
       };
       float fac = 1.f, ofac = 0.f;
       if (join) {
@@ -905,21 +971,20 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       // columns this thread writes: all of its row, or its half of a joined row
       const int c_end = join ? (w + 1) * (D / 2) : done > 0 ? D : 0;
 #pragma unroll 1
-      for (int c = join ? w * (D / 2) : 0; c < c_end; c += 16) {
-        const int in = c - w * (D / 2);                        // place in this group's half
-        if (join && in == kHand) {
+      for (int c = join ? w * (D / 2) : 0; c < c_end; c += kHand) {
+        if (join && c != w * (D / 2)) {
           if (!(ok = meet())) break;
           hand(1);
           if (!(ok = meet())) break;
         }
-        float o[16];
+        float o[kHand];
         __syncwarp();
-        tmem_ld16(tO + c, o);
+        tmem_ld<kHand>(tO + c, o);
         tmem_ld_wait();
         if (join) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 v = stage[((w ^ 1) * (kHand / 4) + (in % kHand) / 4 + e) * kRows + r];
+          for (int e = 0; e < kHand / 4; ++e) {
+            const float4 v = stage[((w ^ 1) * (kHand / 4) + e) * kRows + r];
             o[4 * e] = o[4 * e] * fac + v.x * ofac;
             o[4 * e + 1] = o[4 * e + 1] * fac + v.y * ofac;
             o[4 * e + 2] = o[4 * e + 2] * fac + v.z * ofac;
@@ -935,24 +1000,27 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
               const bf16* v = static_cast<const bf16*>(a.v_cache) + (int64_t)id * a.block_stride +
                               ((int64_t)g.h * a.block_size + key % a.block_size) * D + c;
 #pragma unroll 1
-              for (int e = 0; e < 16; ++e) {
+              for (int e = 0; e < kHand; ++e) {
                 const float x = __bfloat162float(v[e]);
 #pragma unroll
-                for (int f = 0; f < 16; ++f)
+                for (int f = 0; f < kHand; ++f)
                   if (f == e && !isfinite(x)) o[f] += x;
               }
             }
           }
           if (g.whole) {
-            uint32_t v[8];
+            uint32_t v[kHand / 2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = pack2(o[2 * e] * inv, o[2 * e + 1] * inv);
-            st32(static_cast<bf16*>(a.out) + ((int64_t)(g.q0 + node) * nq + head) * D + c, v);
+            for (int e = 0; e < kHand / 2; ++e) v[e] = pack2(o[2 * e] * inv, o[2 * e + 1] * inv);
+#pragma unroll
+            for (int e = 0; e < kHand; e += 16)
+              st32(static_cast<bf16*>(a.out) + ((int64_t)(g.q0 + node) * nq + head) * D + c + e, v + e / 2);
           } else {
             // columns by fours, rows inside: a warp's stores are contiguous
             float4* dst = reinterpret_cast<float4*>(t.part_o) + (pblk * (D / 4) + c / 4) * t.part_rows + prow;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e * t.part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < kHand / 4; ++e)
+              dst[e * t.part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
       }
@@ -978,10 +1046,10 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   const int nq = a.num_kv_heads * G, qrows = a.rows * G, groups = (qrows + 31) / 32;
   const int tasks = groups * a.num_kv_heads * (D / 16);
   for (int it = blockIdx.x + gridDim.x * warp; it < tasks; it += gridDim.x * (kThreads / 32)) {
-    const int c4 = it % (D / 16) * 4, x = it / (D / 16), h = x % a.num_kv_heads;
+    const int c4 = it % (D / 16) * 4, x = it / (D / 16), h = x - x / a.num_kv_heads * a.num_kv_heads;
     const int qr = x / a.num_kv_heads * 32 + lane;
     if (qr >= qrows) continue;
-    const int row = qr / G, hg = qr % G;
+    const int row = qr / G, hg = qr - row * G;
     int lo = 0, up = a.batch;
     while (up - lo > 1) {
       const int mid = (lo + up) >> 1;
@@ -994,16 +1062,25 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     const int nt = plan.tiles(b), pr = plan.pairs(b);
     const int rt = node / per, pair = rt / 2;
     const bool two = plan.nodes(b) > (2 * pair + 1) * per;
-    const int prow = (two ? rt & 1 : 0) * kRows + (node % per) * G + hg;
-    const Chunks c = plan.chunks(nt, pr);
+    const int prow = (two ? rt & 1 : 0) * kRows + (node - rt * per) * G + hg;
+    const Chunks c = plan.parts ? Chunks{1, nt} : plan.chunks(nt, pr);
     float acc[16], top = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool whole = false;
     for (int ci = 0; ci < c.n && !whole; ++ci) {
       const int start = c.start(ci), clen = c.start(ci + 1) - start;
-      const int u0 = unit0 + (h * nt + start) * pr + pair * clen;
-      const int x0 = plan.cta(u0), x1 = plan.cta(u0 + clen - 1);
+      int x0, x1, begun = 0;      // CTAs; whether the first one's share begins in front of this chunk
+      if (plan.parts) {
+        const int cuts = plan.cuts(nt);
+        x0 = unit0 + (h * pr + pair) * cuts;
+        x1 = x0 + cuts - 1;
+      } else {
+        const int u0 = unit0 + (h * nt + start) * pr + pair * clen;
+        x0 = plan.cta(u0);
+        x1 = plan.cta(u0 + clen - 1);
+        begun = x0 * plan.base + min(x0, plan.rem) < u0;
+      }
       if (c.n == 1 && x0 == x1) { whole = true; break; }
       for (int x = x0; x <= x1; x += kParts) {
         float2 ml[kParts];
@@ -1012,7 +1089,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int k = 0; k < kParts; ++k) {
           ml[k] = make_float2(-INFINITY, 0.f);
           if (x + k > x1) continue;
-          const int pblk = (x + k) * 2 + (plan.lo(x + k) >= u0 ? 0 : 1);
+          const int pblk = (x + k) * 2 + (x + k == x0 ? begun : 0);
           ml[k] = __ldcg(t.part_ml + pblk * t.part_rows + prow);
           const float4* po = reinterpret_cast<const float4*>(t.part_o) + ((int64_t)pblk * (D / 4) + c4) * t.part_rows + prow;
 #pragma unroll
