@@ -5,8 +5,10 @@
 // where j runs over the committed prefix [0, P) of node i's sequence and over node i
 // and its ancestors, whose keys sit at positions P + node.
 //
-// One warp per (node, query head): a lane scores one key of 32, the warp keeps the
-// running maximum and sum in fp32, and each lane accumulates D / 32 columns of o.
+// The general form, for the block sizes that the tensor-core form (tree_attn_tc.cu) does not
+// take: one warp per (node, query head), a lane scores one key of 32, the warp keeps the
+// running maximum and sum in fp32, and each lane accumulates D / 32 columns of o.  It is bound
+// by instructions (16 trees of 16 nodes at 1152 context: 5 ms against 27 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

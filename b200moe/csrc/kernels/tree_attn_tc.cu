@@ -1,5 +1,6 @@
-// Attention of drafted trees on the 5th-generation tensor cores (bf16 pool, head_dim 64
-// or 128): the same function as tree_attn.cu, for the shapes a server runs.
+// Attention of drafted trees on the 5th-generation tensor cores (head_dim 64 or 128; bf16
+// pool, or the stage of an int8 one): the same function as tree_attn.cu, for the shapes a
+// server runs.
 //
 // Rows and keys.  The n nodes of a sequence times the G query heads of one KV head are
 // packed into tiles of 128 rows (row = node * G + head), keys into tiles of 64.  A
@@ -11,23 +12,30 @@
 //
 // so both groups work on either shape and a K/V tile is read once for up to 256 rows.
 //
-// Split.  Units are ordered (sequence, KV head, key chunk, row pair, key tile), and
-// CTA c of the persistent grid takes the c-th of equal shares of that order: long
-// contexts, few requests and ragged batches all fill every SM, without the host
-// knowing a length.  A chunk is at least a share long and is the same for all row pairs
+// Split, without the host knowing a length.  An item is the keys of one (sequence, KV head,
+// row pair).  Small batches give every CTA whole items; batches with fewer items than SMs
+// cut each item in equal parts, one to a CTA; larger ones order the units (sequence, KV
+// head, key chunk, row pair, key tile), and CTA c of the persistent grid takes the c-th of
+// equal shares of that order.  A chunk is at least a share long and is the same for all row pairs
 // of a KV head, so the CTAs that read the same keys do so at about the same time and
-// the L2 serves all but the first.  A share that cuts an item leaves an unnormalised
+// the L2 serves all but the first.  A cut item leaves an unnormalised
 // fp32 result with its running maximum and sum; after a grid-wide barrier the warps
 // join those (softmax over the parts).
 //
 // Roles per CTA (12 warps): two TMA producers, one of Q and K and one of V, because a
 // copy with its wait costs its thread about 650 cycles and one thread alone held the
 // whole kernel at 4.9 TB/s; two MMA issuers, one per softmax group (S = Q K^T, then
-// O += P V with P read from TMEM, where it overlays its S); two softmax groups of four warps, a thread per row, so the row
-// statistics need no shuffles.  The running maximum moves only when a row grows by
+// O += P V with P read from TMEM, where it overlays its S); two softmax groups of four
+// warps, a thread per row, so the row statistics need no shuffles.  The running maximum moves only when a row grows by
 // more than 2^8, so O is rarely rescaled.  P is rounded to bf16 for the MMA and the sum
 // that divides O adds the rounded values, which cancels that rounding where few keys
 // carry the weight.
+//
+// What bounds it.  64 chains of 4 nodes at 4k context: the cache, 542 MB in 96.6 us (5.6 TB/s).
+// 4 trees of 64 nodes at 32k, 16 query heads on a KV head: 272 GFLOP in 287 us, 0.58 of the bf16 peak; a
+// tile's chain S, softmax, P V, next S is as long as the softmax of a tile (about 2,100 cycles), and TMEM
+// has no room for a third S.  Smaller calls: setup, first loads, epilogue, barrier and join, 10 to 12 us
+// (one request at 500 context 12.4 us, 32 at 1.1k 26.7 us).
 //
 // A masked place never reaches the result: scores are selected, not added to, and a V
 // row is cleaned by its producer in front of the MMA (0 * NaN is NaN) -- rows behind the sequence become
@@ -61,12 +69,12 @@ constexpr int kRows = 128, kKeys = 64;    // of a tile
 constexpr int kThreads = 384;
 constexpr float kLazyLog2 = 8.f;
 constexpr int kAncWords = kTreeMaxNodes / 32;
-// Cutting items costs their partial results, a grid barrier and the join, worth about kCutBytes of K;
-// whole items cost the rounding up of their number.
-constexpr int kCutBytes = 128 << 10;
-// Shares that end inside an item give some CTAs two segments, worth about kShareBytes of K; parts cost
-// the rounding up of their number.
-constexpr int kShareBytes = 96 << 10;
+// What a way of splitting costs beside its longest run of tiles, in bytes of K.  Cut items: partial results, a
+// grid barrier and the join (4 items of 12 tiles at D = 128: 15.2 us cut, 17.2 whole; 26 of 11 tiles at
+// D = 64: 17.3 cut, 13.8 whole).  Shares that end inside items: a second segment for some CTAs (48 items of
+// 51 tiles at D = 128: 28.4 us in parts, 31.5 in shares; with 256 KB 160 items of 24 tiles would go whole,
+// 50.7 us instead of 45.7).
+constexpr int kCutBytes = 128 << 10, kShareBytes = 192 << 10;
 constexpr int kParts = 4;         // partial results in flight per lane when parts are joined
 constexpr int kRing = 4;          // segments known ahead, and their dirty bits
 
@@ -513,12 +521,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   plan.whole = rounds * max_nt <= kCutBytes / L::TILE;
   if (!plan.whole) {
     plan.share = (plan.W + ctas - 1) / ctas;
-    int cut = plan.share;
+    int cut = plan.share + kShareBytes / L::TILE;
     if (plan.items < ctas && max_nt < 1 << 23) {
       // Parts of S tiles are at most W / S + items, and S (ctas - items) >= W makes that at most the CTAs.
       // (Two tiles take the two groups as long as one.)
       const int parts = max(2, (plan.W + ctas - plan.items - 1) / (ctas - plan.items));
-      if (parts <= plan.share + kShareBytes / L::TILE) cut = plan.parts = parts;
+      if (parts <= cut) cut = plan.parts = parts;
     }
     plan.whole = rounds * max_nt <= cut + kCutBytes / L::TILE;
     if (plan.whole) plan.parts = 0;

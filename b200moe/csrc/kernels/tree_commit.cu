@@ -17,6 +17,11 @@
 // fixed 16-byte (scales: 4-byte) columns of its planes and takes the path in ascending
 // order.  path[j] >= j and path ascends, so a row is read before the step that writes
 // its place (j' = path[j] > j), and moving in place is safe without a copy.
+//
+// Bound by latency: table, tree, walk and rows are four dependent reads.  One request of 8 nodes over 48
+// layers takes 4.1 us, 32 requests of up to 32 nodes (22 MB read and written) 8.9 us, 24 requests on an int8
+// pool with its scales 7.0 us.  A CTA takes 8 planes: with 4 the walks of twice the CTAs cost more than the
+// copies gain (10.9 us for the 32 requests), with 16 the one request takes 5.0 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const TreeCommitA
 
 void tree_commit(const TreeCommitArgs& a, cudaStream_t s) {
   if (a.batch == 0) return;
-  const int per = 8;
+  const int per = 8;   // planes of a CTA
   pdl_launch(tree_commit_kernel, dim3((a.planes + per - 1) / per, a.batch), kThreads, 0, s, a, per);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("tree_commit: ") + cudaGetErrorString(e));

@@ -6,7 +6,8 @@
 // rounded that the pool does not round.  Channel mode: the stage holds bf16(q8 * dscale), or
 // the side value at an outlier dimension, which is what that mode's values are.
 //
-// Bound by memory: 1 byte read and 2 written per value.
+// Bound by memory: 1 byte read and 2 written per value.  16 sequences of 8208 keys (134 MB of int8) take
+// about 100 us, and the attention of the stage 70 us; at 1168 keys 17 + 28 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -26,7 +27,9 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256, kPer = 4;               // chunks of 16 values a thread has in flight
 constexpr int kPiece = kThreads * kPer;               // chunks of one piece of work
-constexpr int kCtasPerSm = 32;                       // launched, about five of them resident: shares of a block each
+// CTAs launched for each SM.  A CTA has a piece of a block (16 KB) at a time; with 8, sequences that hold a few
+// pieces more than they have CTAs take twice as long (1168 keys 45.7 us instead of 44.9, 8208 keys 176 instead of 170).
+constexpr int kCtasPerSm = 32;
 
 struct Stage {
   bf16* kv;          // [seqs * max_blocks][k | v][kv_heads][block_size][D]
