@@ -931,7 +931,7 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
 
 Tensor moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Tensor w2, c10::optional<Tensor> s2,
                int64_t E, int64_t topk, bool renorm, c10::optional<Tensor> out_arg, c10::optional<Tensor> ids,
-               c10::optional<Tensor> weights, bool tiled, Tensor status) {
+               c10::optional<Tensor> weights, bool tiled) {
   check_contiguous(x, "x"); check_bf16(x, "x");
   Tensor out = out_arg.has_value() ? *out_arg : torch::empty_like(x);
   check_contiguous(out, "out"); check_bf16(out, "out");
@@ -1000,7 +1000,6 @@ Tensor moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, T
   a.x_factor = w + at_xf;
   a.sel = reinterpret_cast<int2*>(w + at_sel);
   a.done = reinterpret_cast<int*>(w + at_done);
-  a.status = status.data_ptr<int>();
   b200::moe_few(a, stream());
   return out;
 }

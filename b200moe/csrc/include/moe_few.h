@@ -31,7 +31,6 @@ struct MoeFewArgs {
   float* slots;              // [T * topk, H]
   int2* sel;                 // [T * topk] chosen experts and weights
   int* done;                 // [H / 128]
-  int* status;
 };
 void moe_few(const MoeFewArgs& a, cudaStream_t s);
 

@@ -502,8 +502,7 @@ def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True
     ``ids`` [T, topk] int32 / ``weights`` [T, topk] fp32 receive the routing.  An e4m3 weight enters as
     q * scale in fp32, where the grouped GEMMs round that product to bf16 first."""
     if x.is_cuda:
-        out = native().moe_few(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled,
-                               status_word(x.device))
+        out = native().moe_few(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled)
         count_launches(1 if x.shape[0] else 0)
         return out
     if x.dim() != 2 or not x.is_contiguous():
@@ -696,7 +695,8 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     stored before the call, as for ``prefill_attention``).  parents [rows]: place of a node's parent in
     its tree, below the node's own; -1 for a node that follows the prefix directly.  max_q_len: no tree
     has more nodes (at most ``TREE_MAX_NODES``).  Chains (parents i - 1) give causal attention.  Rows
-    behind the last sequence are left as they are.  bf16 and int8 pools, head_dim 64 or 128.  A tree
+    behind the last sequence are left as they are.  bf16 and int8 pools (int8 through a bf16 stage of at
+    most ``INT8_STAGE_MAX_BYTES``, or of one sequence), head_dim 64 or 128; out must not overlap q.  A tree
     that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
     table row has) is left out and a block id outside the pool is not read; both set the status word
     (``check_status``)."""
@@ -761,7 +761,7 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
     sequence.  Returns int32 (accepted [B], path [B, max_q_len], tokens [B, max_q_len]): nodes on the
     path, their places and the tokens to emit behind them, -1 behind the path; the committed length is
     P + accepted.  A malformed row accepts nothing, a move through a block id outside the pool is left
-    out; both set the status word."""
+    out; both set the status word (the CPU path raises)."""
     if kv_data.is_cuda:
         res = native().tree_commit(kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents,
                                    draft_ids, target_ids, max_q_len, status_word(kv_data.device))
