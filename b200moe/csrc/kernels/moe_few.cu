@@ -6,7 +6,7 @@
 //   out = sum_k w_k Wd_e ( silu(Wg_e x) * (Wu_e x) ),   e = the token's k-th expert
 //
 // The grid is launched cooperatively, one CTA per SM, and synchronises after the logits and
-// after the experts' hidden rows, above 16 tokens also between top-k and its tables, above 2
+// after the experts' hidden rows, above 16 tokens also between top-k and its tables, above 4
 // tokens in front of the last sums.
 //
 // Nearly all the time goes into reading the touched experts' weights once, so the
@@ -31,7 +31,7 @@
 // value as two bf16, value and rest.
 //
 // The parts of K are added in order through shared memory.  The rows of Wd write fp32 (token, k) slots.
-// A token's slots are added in the order of the top-k: with up to 2 tokens by the team that finishes the
+// A token's slots are added in the order of the top-k: with up to 4 tokens by the team that finishes the
 // last expert of a tile of 128 columns, above by the whole grid behind one more barrier (at 64 tokens one
 // warp per tile needed 47 us for them).
 //
@@ -67,7 +67,9 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRingBytes = 12832;        // of a warp
 constexpr int kCols = 8;                 // tokens of one pass
-constexpr int kLastAdds = 2;             // tokens up to which the last team of a tile adds the slots
+// Tokens up to which the last team of a tile adds the slots, a warp each (3 tokens: 44.7 us, by the grid
+// behind a barrier 45.8; at 8 the grid is as fast, at 64 far faster).
+constexpr int kLastAdds = 4;
 
 // fp64 -> bf16 in one rounding: fp32 with round-to-odd keeps the bit that decides a tie.
 __device__ __forceinline__ float bf16_of(double v) {

@@ -840,3 +840,35 @@ def test_operators_on_two_streams():
         for a, y in got[i]:
             assert torch.equal(a, want[i][0]) and torch.equal(y, want[i][1])
     ops.check_status(x[0].device)
+
+
+@pytest.mark.gpu
+def test_operators_in_two_graphs_of_one_pool():
+    """Two captured graphs that share a memory pool, replayed in turn over new inputs: a workspace holds nothing
+    from one call to the next."""
+    def case(seed):
+        b = Batch("cuda", [30, 7], [2500, 300], 32, 4, 128, 32, seed=seed)
+        w = _moe_weights("cuda", 24, 256, 128, True, seed=seed)
+        x = torch.randn(20, 256, generator=torch.Generator().manual_seed(seed)).to("cuda", torch.bfloat16)
+        return b, w, x
+
+    def run(b, w, x):
+        return ops.tree_attention(*b.args()), ops.moe_few_tokens(x, *w, 24, 4)
+
+    cases, graphs, outs = [case(s) for s in range(2)], [], []
+    run(*cases[0])                                   # warm-up
+    torch.cuda.synchronize()
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(run(*c))
+        graphs.append(g)
+    for r in range(3):
+        for c in cases:
+            c[0].q.copy_(torch.randn(c[0].q.shape, generator=torch.Generator().manual_seed(r)))
+            c[2].mul_(1.25)
+        for g in graphs:
+            g.replay()
+        for c, got in zip(cases, outs):
+            assert all(torch.equal(a, b) for a, b in zip(got, run(*c)))
+    ops.check_status("cuda:0")
