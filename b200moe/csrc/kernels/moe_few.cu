@@ -414,6 +414,7 @@ struct Few {
   __device__ __forceinline__ int tiles(int phase) const { return (phase ? a.H : a.I) >> 7; }
   __device__ __forceinline__ static constexpr int subs(int phase) { return phase ? 4 : 8; }
   // warps of a team (4, 2 or 1): the least rounds of items, each its runs and about one run's time more
+  // (with 8 among them at most 1 % is gained, and 10 tokens take 80 us instead of 73)
   __device__ __forceinline__ int team_warps(int phase) const {
     const int n = s.passes * tiles(phase) * subs(phase), runs = (phase ? a.I : a.H) / 64;
     int best = 4, cost = 1 << 30;
