@@ -105,10 +105,13 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
           s = fmaf(s_q[warp][d], kv_value<MODE>(a, a.k_cache, a.ch.side_k, 0, blk, h, y, d, ks), s);
         s *= sl2;
       }
+      if (!__any_sync(0xffffffffu, see)) continue;
+      // The maximum passes over NaN.  While no score is above -inf, 0 stands for it: a -inf weighs
+      // nothing, a NaN makes the sum NaN.
       const float mn = fmaxf(m, warp_max(s));
-      if (mn == -INFINITY) continue;
-      const float alpha = exp2f(m - mn);  // m = -inf: 0
-      const float p = see ? exp2f(s - mn) : 0.f;
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float alpha = exp2f(m - base);  // m = -inf: 0
+      const float p = see ? exp2f(s - base) : 0.f;
       m = mn;
       l = l * alpha + warp_sum(p);
 #pragma unroll

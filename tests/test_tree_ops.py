@@ -872,3 +872,36 @@ def test_operators_in_two_graphs_of_one_pool():
         for c, got in zip(cases, outs):
             assert all(torch.equal(a, b) for a, b in zip(got, run(*c)))
     ops.check_status("cuda:0")
+
+
+# ------------------------------------------------------------------ what the cases above do not reach
+FORMS = [(16, False, "token"), (64, False, "token"), (24, False, "token"), (48, False, "token"), (96, False, "token"),
+         (16, True, "token"), (48, True, "token"), (16, True, "channel"), (48, True, "channel")]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bs,int8,mode", FORMS)
+def test_tree_attention_nan_query(dev, bs, int8, mode):
+    """A NaN in one head of one query makes that head of that node NaN and changes nothing else."""
+    b = Batch(dev, [7, 1, 12], [50, 0, 170], 8, 2, 64, bs, int8=int8, mode=mode)
+    want = ops.tree_attention(*b.args()).clone()
+    b.q[9, 3, 5] = b.q[7, 0, 0] = math.nan       # a node of the third tree, the only one of the second
+    got = ops.tree_attention(*b.args())
+    hit = torch.zeros(20, 8, dtype=torch.bool, device=dev)
+    hit[9, 3] = hit[7, 0] = True
+    assert bool(torch.isnan(got[hit].float()).all())
+    assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bs", [16, 64, 24, 48, 96])
+@pytest.mark.parametrize("keys", [1, 32, 75])
+def test_tree_attention_nan_keys_in_front(dev, bs, keys):
+    """The first keys of a prefix are NaN: so is every node of that sequence, and no other."""
+    b = Batch(dev, [7, 5], [120, 60], 8, 2, 64, bs)
+    want = ops.tree_attention(*b.args()).clone()
+    for y in range(keys):
+        b.layer.k[b.tables[0, y // bs].item(), :, y % bs] = math.nan
+    got = ops.tree_attention(*b.args())
+    assert bool(torch.isnan(got[:7].float()).all())
+    assert torch.equal(got[7:], want[7:])
