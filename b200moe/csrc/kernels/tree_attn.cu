@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
     float m = -INFINITY, l = 0.f, o[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+    bool any = false;    // a key has been read
     for (int k0 = 0; k0 < len; k0 += 32) {
       const int key = k0 + lane;
       bool see = key < prefix;
@@ -106,6 +107,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
         s *= sl2;
       }
       if (!__any_sync(0xffffffffu, see)) continue;
+      any = true;
       // The maximum passes over NaN.  While no score is above -inf, 0 stands for it: a -inf weighs
       // nothing, a NaN makes the sum NaN.
       const float mn = fmaxf(m, warp_max(s));
@@ -128,7 +130,8 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
           o[i] = fmaf(pj, kv_value<MODE>(a, a.v_cache, a.ch.side_v, 1, bj, h, yj, i * 32 + lane, vj), o[i]);
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    // every score -inf: no softmax, NaN; every block id outside the pool: zeros
+    const float inv = any ? 1.f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
       static_cast<bf16*>(a.out)[qrow + i * 32 + lane] = __float2bfloat16(o[i] * inv);

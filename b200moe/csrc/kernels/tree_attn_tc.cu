@@ -968,7 +968,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         l = l * fac + other.y * ofac;
         m = top;
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = 1.f / l;   // every score -inf: l and O are 0, the row NaN
       const int64_t pblk = blockIdx.x * 2 + g.slot;
       const int prow = (g.two ? w : 0) * kRows + r;
       if (!g.whole && valid && done > 0 && (!join || w == 0)) t.part_ml[pblk * t.part_rows + prow] = make_float2(m, l);
@@ -1127,7 +1127,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
     }
     if (whole) continue;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = 1.f / l;
     uint32_t v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);

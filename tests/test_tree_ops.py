@@ -905,3 +905,22 @@ def test_tree_attention_nan_keys_in_front(dev, bs, keys):
     got = ops.tree_attention(*b.args())
     assert bool(torch.isnan(got[:7].float()).all())
     assert torch.equal(got[7:], want[7:])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bs,ctx", [(16, 60), (64, 60), (64, 9000), (48, 60)])
+def test_tree_attention_infinite_keys(dev, bs, ctx):
+    """Keys that score -inf weigh nothing; a node that sees no other has no softmax and is NaN."""
+    b = Batch(dev, [4, 1], [ctx, 200], 8, 2, 64, bs, "star")
+    b.q.copy_(b.q.abs() + 1)
+    some = {y for y in range(ctx) if y % 3 == 0}
+    for y in some:
+        b.layer.k[b.tables[0, y // bs].item(), :, y % bs] = -math.inf
+    got = ops.tree_attention(*b.args())
+    b.check(got)
+    for y in set(range(ctx + 2)) - some:         # all that node 1 sees: the prefix, node 0 and itself
+        b.layer.k[b.tables[0, y // bs].item(), :, y % bs] = -math.inf
+    last = ops.tree_attention(*b.args())
+    assert bool(torch.isnan(last[:2].float()).all())
+    assert torch.equal(last[4], got[4])          # the other sequence
+    assert bool(torch.isfinite(last[2:4].float()).all())   # nodes 2 and 3 see themselves
