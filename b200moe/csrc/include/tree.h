@@ -11,6 +11,14 @@ namespace b200 {
 
 constexpr int kTreeMaxNodes = 256;   // nodes of one tree
 
+#ifdef __CUDACC__
+// Whether a sequence's nodes [q0, q1) lie in the rows and its keys hold them.  Compared, not subtracted,
+// until the offsets are known to be in range: a difference of two of them may wrap to a small number.
+__device__ __forceinline__ bool tree_fits(int q0, int q1, int rows, int max_q_len, int len) {
+  return q0 >= 0 && q0 <= q1 && q1 <= rows && q1 - q0 <= max_q_len && (q0 == q1 || len >= q1 - q0);
+}
+#endif
+
 struct TreeAttnArgs {
   const void* q;             // [rows, q_heads, D] bf16
   const void* k_cache;       // layer base of the pool, [blocks, kv_heads, block_size, D]

@@ -57,13 +57,13 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
     const int mid = (lo + hi) >> 1;
     if (a.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid;
   }
-  const int b = lo, q0 = a.cu_seqlens_q[b], n = a.cu_seqlens_q[b + 1] - q0, node = row - q0;
-  if (node < 0 || node >= n) return;  // rows behind the last sequence
-  const int len = a.seq_lens[b], prefix = len - n;
-  if (n > a.max_q_len || prefix < 0 || q0 < 0 || q0 + n > a.rows || len > (int64_t)a.max_blocks * a.block_size) {
+  const int b = lo, q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
+  if (row < q0 || row >= q1) return;  // rows behind the last sequence
+  if (!tree_fits(q0, q1, a.rows, a.max_q_len, len) || len > (int64_t)a.max_blocks * a.block_size) {
     if (threadIdx.x == 0) record_status(a.status, kStatusBadShape);
     return;
   }
+  const int n = q1 - q0, node = row - q0, prefix = len - n;
   for (int i = threadIdx.x; i < n; i += kWarps * 32) s_par[i] = a.parents[q0 + i];
   __syncthreads();
   const int* tab = a.block_tables + (int64_t)b * a.max_blocks;

@@ -440,19 +440,19 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   if (threadIdx.x == 0) *s_max_nt = 0;
   __syncthreads();
   for (int b = threadIdx.x; b < a.batch; b += kThreads) {
-    const int q0 = a.cu_seqlens_q[b], n = a.cu_seqlens_q[b + 1] - q0, len = a.seq_lens[b];
-    const bool bad = n < 0 || n > a.max_q_len || q0 < 0 || q0 + n > a.rows ||
-                     (n > 0 && (len < n || len > (int64_t)a.max_blocks * a.block_size));
+    const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
+    const bool bad = !tree_fits(q0, q1, a.rows, a.max_q_len, len) ||
+                     (q0 < q1 && len > (int64_t)a.max_blocks * a.block_size);
     if (bad && blockIdx.x == 0) record_status(status, kStatusBadShape);
     Row r{q0, len, 0, 0};
-    if (!bad && n > 0) {
+    if (!bad && q0 < q1) {
       const int nt = (len + kKeys - 1) / kKeys;
-      r.item = ((n + per - 1) / per + 1) / 2 * a.num_kv_heads;
+      r.item = ((q1 - q0 + per - 1) / per + 1) / 2 * a.num_kv_heads;
       r.unit = r.item * nt;
       atomicMax(s_max_nt, nt);
     }
     rows[b] = r;
-    if (b == a.batch - 1) rows[b + 1].q0 = q0 + n;
+    if (b == a.batch - 1) rows[b + 1].q0 = q1;
   }
   if (threadIdx.x == 32) {
     for (int i = 0; i < kSlots; ++i) {

@@ -71,15 +71,11 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const TreeCommitA
   __shared__ int2 s_moves[kTreeMaxNodes];  // (source, destination) slots of the pool
   __shared__ int s_len, s_moves_n;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-  const int q0 = a.cu_seqlens_q[b];
-  int n = a.cu_seqlens_q[b + 1] - q0;
-  const int prefix = a.seq_lens[b] - n;
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], keys = a.seq_lens[b];
   // a malformed row (offsets outside the arrays, more nodes than keys) commits nothing
-  const bool bad = n < 0 || n > a.max_q_len || q0 < 0 || q0 + n > a.nodes || (n > 0 && prefix < 0);
-  if (bad) {
-    if (tid == 0) record_status(a.status, kStatusBadShape);
-    n = 0;
-  }
+  const bool bad = !tree_fits(q0, q1, a.nodes, a.max_q_len, keys);
+  const int n = bad ? 0 : q1 - q0, prefix = keys - n;
+  if (bad && tid == 0) record_status(a.status, kStatusBadShape);
   for (int i = tid; i < n; i += kThreads) {
     s_par[i] = a.parents[q0 + i];
     s_draft[i] = a.draft[q0 + i];

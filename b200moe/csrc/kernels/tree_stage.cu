@@ -60,9 +60,9 @@ __device__ __forceinline__ void four(uint32_t w, float* f) {
 template <int D, bool CHAN>
 __global__ void __launch_bounds__(kThreads) tree_stage_kernel(const TreeAttnArgs a, const Stage o) {
   const int b = blockIdx.y, bs = a.block_size, nkv = a.num_kv_heads;
-  const int n = a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b], len = a.seq_lens[b];
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
   // (a tree that does not fit is left out and reported by the attention)
-  if (n <= 0 || len < n || len > (int64_t)a.max_blocks * bs) return;
+  if (q0 == q1 || !tree_fits(q0, q1, a.rows, a.max_q_len, len) || len > (int64_t)a.max_blocks * bs) return;
   const int nb = (len + bs - 1) / bs;
   const int64_t plane = (int64_t)nkv * bs * D;
   const int chunks = (int)(plane / 16), pieces = (chunks + kPiece - 1) / kPiece;

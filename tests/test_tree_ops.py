@@ -924,3 +924,23 @@ def test_tree_attention_infinite_keys(dev, bs, ctx):
     assert bool(torch.isnan(last[:2].float()).all())
     assert torch.equal(last[4], got[4])          # the other sequence
     assert bool(torch.isfinite(last[2:4].float()).all())   # nodes 2 and 3 see themselves
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,int8", [(16, False), (48, False), (16, True)])
+def test_tree_offsets_whose_difference_wraps(bs, int8):
+    """Offsets 2^31 - 1 and -2^31 + 3: their difference, 4 in 32 bits, is not a tree of 4 nodes."""
+    b = Batch("cuda", [3, 5, 4, 6, 2], [40, 9, 40, 43, 70], 8, 2, 64, bs, int8=int8)
+    want = ops.tree_attention(*b.args()).clone()
+    b.cu[2], b.cu[3] = (1 << 31) - 1, -(1 << 31) + 3
+    out = torch.full_like(b.q, 7.0)
+    ops.tree_attention(*b.args(), out=out)
+    assert torch.equal(out[:3], want[:3]) and bool((out[3:18] == 7.0).all())
+    with pytest.raises(RuntimeError):
+        ops.check_status(out.device)
+    draft = torch.zeros_like(b.parents)
+    acc = ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, draft, draft, b.max_nodes,
+                          kv_scales=b.pool.scales)[0]
+    assert [int(n) > 0 for n in acc.tolist()] == [True, False, False, False, True]
+    with pytest.raises(RuntimeError):
+        ops.check_status(out.device)
