@@ -44,25 +44,43 @@ __device__ __forceinline__ float kv_value(const TreeAttnArgs& a, const void* poo
   return __bfloat162float(__float2bfloat16(q * a.ch.dscale[((int64_t)kv * a.num_kv_heads + h) * a.head_dim + d]));
 }
 
+__device__ __forceinline__ bool usable(const TreeAttnArgs& a, int b) {
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
+  return tree_fits(q0, q1, a.rows, a.max_q_len, len) && (q0 == q1 || len <= (int64_t)a.max_blocks * a.block_size);
+}
+
+// Whether row is a node of sequence b.
+__device__ __forceinline__ bool holds(const TreeAttnArgs& a, int b, int row) {
+  return a.cu_seqlens_q[b] <= row && row < a.cu_seqlens_q[b + 1] && usable(a, b);
+}
+
 template <int D, int MODE>
 __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnArgs a) {
   pdl_enter();
   __shared__ int s_par[kTreeMaxNodes];
   __shared__ float s_q[kWarps][D];
+  __shared__ int s_found;
   const int row = blockIdx.x, h = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (row == 0 && h == 0)      // report the trees that do not fit
+    for (int i = threadIdx.x; i < a.batch; i += kWarps * 32)
+      if (!usable(a, i)) record_status(a.status, kStatusBadShape);
   // the sequence that holds this row: last b with cu[b] <= row
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid;
+  int b = 0, hi = a.batch;
+  while (hi - b > 1) {
+    const int mid = (b + hi) >> 1;
+    if (a.cu_seqlens_q[mid] <= row) b = mid; else hi = mid;
   }
-  const int b = lo, q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
-  if (row < q0 || row >= q1) return;  // rows behind the last sequence
-  if (!tree_fits(q0, q1, a.rows, a.max_q_len, len) || len > (int64_t)a.max_blocks * a.block_size) {
-    if (threadIdx.x == 0) record_status(a.status, kStatusBadShape);
-    return;
+  if (!holds(a, b, row)) {     // none, or offsets of a bad tree led the search astray
+    if (threadIdx.x == 0) s_found = a.batch;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.batch; i += kWarps * 32)
+      if (holds(a, i, row)) atomicMin(&s_found, i);
+    __syncthreads();
+    b = s_found;
+    if (b == a.batch) return;  // rows of bad trees and behind the last sequence
   }
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
   const int n = q1 - q0, node = row - q0, prefix = len - n;
   for (int i = threadIdx.x; i < n; i += kWarps * 32) s_par[i] = a.parents[q0 + i];
   __syncthreads();

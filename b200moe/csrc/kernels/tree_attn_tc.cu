@@ -439,6 +439,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   // ---- the work of every sequence; a tree that does not fit has none
   if (threadIdx.x == 0) *s_max_nt = 0;
   __syncthreads();
+  bool any_bad = false;
   for (int b = threadIdx.x; b < a.batch; b += kThreads) {
     const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
     const bool bad = !tree_fits(q0, q1, a.rows, a.max_q_len, len) ||
@@ -451,6 +452,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       r.unit = r.item * nt;
       atomicMax(s_max_nt, nt);
     }
+    if (bad) r.item = -1;
+    any_bad |= bad;
     rows[b] = r;
     if (b == a.batch - 1) rows[b + 1].q0 = q1;
   }
@@ -480,7 +483,25 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     fence_barrier_init();
     *abort_flag = 0;
   }
-  __syncthreads();
+  if (__syncthreads_or(any_bad)) {
+    // The join looks rows up by their sequence's first one.  A bad tree in front of which another is bad
+    // has no offset to go by: it takes the end of the last good one, so that the offsets still ascend.
+    if (threadIdx.x == 0) {
+      int end = 0;
+      bool after_bad = true;
+      for (int b = 0; b < a.batch; ++b) {
+        const bool bad = rows[b].item < 0;
+        if (bad) {
+          rows[b].item = 0;
+          if (after_bad) rows[b].q0 = end;
+        } else {
+          end = rows[b + 1].q0;
+        }
+        after_bad = bad;
+      }
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
     int units = 0, items = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {

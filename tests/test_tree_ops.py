@@ -944,3 +944,37 @@ def test_tree_offsets_whose_difference_wraps(bs, int8):
     assert [int(n) > 0 for n in acc.tolist()] == [True, False, False, False, True]
     with pytest.raises(RuntimeError):
         ops.check_status(out.device)
+
+
+# offsets past the rows, below zero, that descend
+BAD_CU = [(1, 1 << 20), (2, 1 << 20), (1, -7), (2, 0), (2, -(1 << 31))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,int8", [(16, False), (128, False), (48, False), (16, True)])
+@pytest.mark.parametrize("ctx", [40, 5000])
+@pytest.mark.parametrize("at,value", BAD_CU)
+def test_tree_bad_offset_leaves_the_other_trees(bs, int8, ctx, at, value):
+    """An offset outside the rows spoils the two trees that it bounds; the others are right."""
+    if bs == 48 and ctx > 1000:
+        ctx = 300                                # the form without tensor cores
+    b = Batch("cuda", [3, 5, 4, 6, 2], [ctx, 9, ctx, ctx + 3, 70], 8, 2, 64, bs, int8=int8)
+    want = ops.tree_attention(*b.args()).clone()
+    b.cu[at] = value
+    out = torch.full_like(b.q, 7.0)
+    ops.tree_attention(*b.args(), out=out)
+    rows = torch.zeros(20, dtype=torch.bool, device="cuda")   # of the trees between at - 1 and at + 1
+    rows[b.cu_list[at - 1]:b.cu_list[at + 1]] = True
+    kept = out.clone()
+    kept[rows] = want[rows]
+    b.check(kept)
+    with pytest.raises(RuntimeError):
+        ops.check_status(out.device)
+    # the commit too accepts nothing of the two
+    draft = torch.zeros_like(b.parents)
+    acc, path, _ = ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, draft, draft, b.max_nodes,
+                                   kv_scales=b.pool.scales)
+    bad = [i for i in range(5) if i in (at - 1, at)]
+    assert [i for i, n in enumerate(acc.tolist()) if n == 0] == bad and bool((path[bad] == -1).all())
+    with pytest.raises(RuntimeError):
+        ops.check_status(out.device)
