@@ -95,45 +95,81 @@ struct Shared {
   float sel_w[kPairs];
 };
 
-// Logits of experts blockIdx.x, blockIdx.x + gridDim.x, ...: a product of two bf16 is exact in
-// fp32 and the sum of four stays so for nearly all of them; beyond that the sum runs in fp64,
-// because a logit is rounded to bf16 and a wrong last bit there can change the experts.
-// Exact products of eight bf16 pairs, summed by fours in fp32, the rest in fp64.
-__device__ __forceinline__ double dot8(const uint4& w, const uint4& x) {
+// The sum of eight products of bf16 pairs: exact in fp32 each (above its smallest normal number), and added
+// in fp64.  (Sums of four in fp32 dropped a bit in 1 of 50, and with it the side of a bf16 border on
+// which a logit lies.)
+__device__ __forceinline__ double dot8(const uint4& w, const uint4& x, double acc) {
   const uint32_t wu[4] = {w.x, w.y, w.z, w.w}, xu[4] = {x.x, x.y, x.z, x.w};
-  float p[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    p[2 * i] = __uint_as_float(wu[i] << 16) * __uint_as_float(xu[i] << 16);
-    p[2 * i + 1] = __uint_as_float(wu[i] & 0xffff0000u) * __uint_as_float(xu[i] & 0xffff0000u);
+    acc += (double)(__uint_as_float(wu[i] << 16) * __uint_as_float(xu[i] << 16));
+    acc += (double)(__uint_as_float(wu[i] & 0xffff0000u) * __uint_as_float(xu[i] & 0xffff0000u));
   }
-  return (double)((p[0] + p[1]) + (p[2] + p[3])) + (double)((p[4] + p[5]) + (p[6] + p[7]));
+  return acc;
 }
 
+// Values 2 q and 2 q + 1 of eight bf16.
+__device__ __forceinline__ void two_of(const uint4& v, int q, double (&d)[2]) {
+  const uint32_t u = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
+  d[0] = (double)__uint_as_float(u << 16);
+  d[1] = (double)__uint_as_float(u & 0xffff0000u);
+}
+
+// Logits of experts blockIdx.x + gridDim.x, ..., summed in fp64: a logit is rounded to bf16, and
+// a wrong last bit there can change the experts.
 __device__ void few_logits(const MoeFewArgs& a, double* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (a.T > kWarps) {
-    // many tokens: tiles of 16 tokens (a warp each) x 4 experts, so x is not read once per expert
+    // many tokens: tiles of 16 tokens x 4 experts, so x is not read once per expert; a warp takes 4 tokens and
+    // a quarter of K, which converts half a value per product (1 with a token per warp: 2.5 us more at 64 tokens)
     const int groups = (a.T + kWarps - 1) / kWarps, tiles = groups * ((a.E + 3) / 4);
     for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const int t = i % groups * kWarps + warp, e0 = i / groups * 4;
-      if (t >= a.T) continue;
-      const bf16* xr = static_cast<const bf16*>(a.x) + t * a.H;
-      const bf16* wr = static_cast<const bf16*>(a.router) + e0 * a.H;   // the last rows are repeated below
-      double acc[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-      for (int c = lane * 8; c < a.H; c += 256) {
-        const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
+      const int t0 = i % groups * kWarps + (warp & 3) * 4, e0 = i / groups * 4;
+      double acc[16] = {};                       // [token][expert]; the last rows are repeated
+      if (t0 < a.T) {
+        for (int c = (warp >> 2) * 256 + lane * 8; c < a.H; c += 1024) {
+          uint4 xv[4], wv[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[j] += dot8(__ldg(reinterpret_cast<const uint4*>(wr + min(j, a.E - 1 - e0) * a.H + c)), xv);
+          for (int j = 0; j < 4; ++j) {
+            xv[j] = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.x) + min(t0 + j, a.T - 1) * a.H + c);
+            wv[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.router) + min(e0 + j, a.E - 1) * a.H + c));
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            double xd[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) two_of(xv[j], q, xd[j]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              double wd[2];
+              two_of(wv[k], q, wd);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[j * 4 + k] = fma(xd[j][1], wd[1], fma(xd[j][0], wd[0], acc[j * 4 + k]));
+            }
+          }
+        }
+        // lane l < 16 gets sum l of the warp: halves of the sums are exchanged
+#pragma unroll
+        for (int n = 8; n > 0; n >>= 1) {
+          const bool up = lane & n;
+#pragma unroll
+          for (int j = 0; j < n; ++j) {
+            const double give = up ? acc[j] : acc[j + n];
+            acc[j] = (up ? acc[j + n] : acc[j]) + __shfl_xor_sync(0xffffffffu, give, n);
+          }
+        }
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 16);
+        if (lane < 16) red[warp * 16 + lane] = acc[0];
       }
+      __syncthreads();
+      if (threadIdx.x < 64) {                    // 16 tokens x 4 experts, the quarters of K in order
+        const int t = i % groups * kWarps + (threadIdx.x >> 2), e = e0 + (threadIdx.x & 3);
+        double sum = 0.0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-        if (lane == j && e0 + j < a.E) a.logits[t * a.E + e0 + j] = bf16_of(acc[j]);
+        for (int q = 0; q < 4; ++q) sum += red[(q * 4 + (threadIdx.x >> 4)) * 16 + (threadIdx.x & 15)];
+        if (t < a.T && e < a.E) a.logits[t * a.E + e] = bf16_of(sum);
       }
+      __syncthreads();
     }
     return;
   }
@@ -147,7 +183,7 @@ __device__ void few_logits(const MoeFewArgs& a, double* red) {
       double acc = 0.0;
 #pragma unroll 8
       for (int c = (sub * 32 + lane) * 8; c < a.H; c += share * 256) {
-        acc += dot8(*reinterpret_cast<const uint4*>(wr + c), *reinterpret_cast<const uint4*>(xr + c));
+        acc = dot8(*reinterpret_cast<const uint4*>(wr + c), *reinterpret_cast<const uint4*>(xr + c), acc);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);

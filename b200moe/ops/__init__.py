@@ -526,9 +526,17 @@ def moe_few_tokens(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm=True
     return _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled)
 
 
+def _bf16_of_double(v: torch.Tensor) -> torch.Tensor:
+    """float64 -> bf16 in one rounding: fp32 rounded to odd on the way keeps the bit that decides a tie."""
+    f = v.float()
+    f = torch.where(f.double().abs() > v.abs(), torch.nextafter(f, torch.zeros_like(f)), f)
+    odd = (f.view(torch.int32) | 1).view(torch.float32)
+    return torch.where((f.double() != v) & ~v.isnan(), odd, f).to(torch.bfloat16)
+
+
 def _moe_few_ref(x, router_w, w13, s13, w2, s2, num_experts, topk, renorm, out, ids, weights, tiled):
     T = x.shape[0]
-    logits = (x.double() @ router_w[:num_experts].double().t()).to(torch.bfloat16).float()
+    logits = _bf16_of_double(x.double() @ router_w[:num_experts].double().t()).float()
     p = torch.softmax(logits, dim=-1)
     e = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :topk]
     w = p.gather(1, e)

@@ -978,3 +978,29 @@ def test_tree_bad_offset_leaves_the_other_trees(bs, int8, ctx, at, value):
     assert [i for i, n in enumerate(acc.tolist()) if n == 0] == bad and bool((path[bad] == -1).all())
     with pytest.raises(RuntimeError):
         ops.check_status(out.device)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T", [1, 2, 5, 16, 17, 64])
+@pytest.mark.parametrize("at", [0, 1, 6])
+def test_moe_few_tokens_logit_beside_a_tie(dev, T, at):
+    """Logits 1 + 2^-8 + 2^-30 and 1 + 2^-8 - 2^-30 lie beside a border of two bf16 values, 1 and 1 + 2^-7:
+    the bit far below decides, and with it the expert."""
+    E, H, I = 8, 256, 128
+    _, w13, s13, w2, s2 = _moe_weights(dev, E, H, I, True, seed=5)
+    router = torch.zeros(128, H)
+    router[:E, 3] = -4.0
+    x = torch.zeros(T, H)
+    x[:, [at, 7, 200]] = 1.0
+    lo, up = 2, 5
+    router[lo, :] = 0
+    router[up, :] = 0
+    router[lo, [at, 7, 200]] = torch.tensor([1.0, 2.0 ** -8, -2.0 ** -30])
+    router[up, [at, 7, 200]] = torch.tensor([1.0, 2.0 ** -30, 2.0 ** -8])
+    router[:2, [at]] = -1.0
+    x, router = x.to(dev, torch.bfloat16), router.to(dev, torch.bfloat16)
+    ids = torch.empty(T, 2, dtype=torch.int32, device=dev)
+    wts = torch.empty(T, 2, dtype=torch.float32, device=dev)
+    out = ops.moe_few_tokens(x, router, w13, s13, w2, s2, E, 2, ids=ids, weights=wts)
+    assert ids.tolist() == [[up, lo]] * T
+    _moe_check(x, router, w13, s13, w2, s2, E, 2, True, out, ids, wts)
