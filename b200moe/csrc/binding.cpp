@@ -792,11 +792,13 @@ void check_tree(const Tensor& cu, const Tensor& lens, const Tensor& tables, cons
               std::to_string(b200::kTreeMaxNodes), "], got ", std::to_string(max_q_len));
 }
 
-Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor> k_scale,
-                 c10::optional<Tensor> v_scale, Tensor cu, Tensor lens, Tensor tables, Tensor parents,
-                 c10::optional<Tensor> out_arg, int64_t max_q_len, int64_t block_size, int64_t block_stride,
-                 int64_t scale_block_stride, double scale, Tensor status, std::vector<int64_t> chan,
-                 int64_t stage_limit) {
+// Returns out and the number of kernels launched.
+std::tuple<Tensor, int> tree_attn(Tensor q, Tensor k_cache, Tensor v_cache,
+                                  c10::optional<Tensor> k_scale, c10::optional<Tensor> v_scale, Tensor cu,
+                                  Tensor lens, Tensor tables, Tensor parents, c10::optional<Tensor> out_arg,
+                                  int64_t max_q_len, int64_t block_size, int64_t block_stride,
+                                  int64_t scale_block_stride, double scale, Tensor status,
+                                  std::vector<int64_t> chan, int64_t stage_limit) {
   check_contiguous(q, "q"); check_bf16(q, "q");
   Tensor out = out_arg.has_value() ? *out_arg : torch::empty_like(q);
   check_contiguous(out, "out"); check_bf16(out, "out");
@@ -821,7 +823,7 @@ Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor>
   CHECK_VALUE(block_stride * k_cache.element_size() % 16 == 0, "cache blocks must be multiples of 16 bytes");
   CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale must be positive");
   CHECK_VALUE(parents.numel() == q.size(0), "parents must hold one entry per row of q");
-  if (q.size(0) == 0 || lens.numel() == 0) return out;
+  if (q.size(0) == 0 || lens.numel() == 0) return {out, 0};
   b200::TreeAttnArgs a{};
   a.q = q.data_ptr();
   a.k_cache = k_cache.data_ptr();
@@ -867,14 +869,11 @@ Tensor tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, c10::optional<Tensor>
       const int64_t one = b200::tree_stage_bytes(a, 1);
       const int seqs = (int)std::min<int64_t>(most, std::max<int64_t>(1, stage_limit / one));
       Tensor stage = torch::empty({b200::tree_stage_bytes(a, seqs)}, q.options().dtype(torch::kUInt8));
-      b200::tree_attn_staged(a, plan, seqs, stage.data_ptr(), stream());
-    } else {
-      b200::tree_attn_tc(a, plan, stream());
+      return {out, b200::tree_attn_staged(a, plan, seqs, stage.data_ptr(), stream())};
     }
-  } else {
-    b200::tree_attn(a, stream());
+    return {out, b200::tree_attn_tc(a, plan, stream())};
   }
-  return out;
+  return {out, b200::tree_attn(a, stream())};
 }
 
 // Accepted paths of a batch of trees; the rows of kv_data (and scales / side) move in place.

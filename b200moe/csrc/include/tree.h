@@ -46,7 +46,8 @@ struct TreeAttnArgs {
   void* out;                 // [rows, q_heads, D] bf16
   int* status;               // device status word
 };
-void tree_attn(const TreeAttnArgs& a, cudaStream_t s);
+// The forms return the number of kernels that they launched.
+int tree_attn(const TreeAttnArgs& a, cudaStream_t s);
 
 // Tensor-core form (kernels/tree_attn_tc.cu): head_dim 64 or 128, blocks that hold whole
 // tiles of 64 keys or divide one in multiples of 8 rows.
@@ -62,12 +63,12 @@ struct TreeAttnTcPlan {
 };
 // False where the shape is not the tensor-core kernel's.
 bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p);
-void tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s);
+int tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s);
 
 // int8 pools (kernels/tree_stage.cu): the keys and values of up to `seqs` sequences at a time go
 // to a bf16 stage that the tensor-core form reads.
 int64_t tree_stage_bytes(const TreeAttnArgs& a, int seqs);
-void tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, void* stage, cudaStream_t s);
+int tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, void* stage, cudaStream_t s);
 
 // One kind of rows the commit moves: [blocks, planes, block_size, row_bytes], contiguous.
 struct TreeRows {

@@ -169,12 +169,13 @@ void launch(const TreeAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-void tree_attn(const TreeAttnArgs& a, cudaStream_t s) {
-  if (a.rows == 0 || a.batch == 0) return;
+int tree_attn(const TreeAttnArgs& a, cudaStream_t s) {
+  if (a.rows == 0 || a.batch == 0) return 0;
   if (a.head_dim == 128) launch<128>(a, s);
   else launch<64>(a, s);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("tree_attn: ") + cudaGetErrorString(e));
+  return 1;
 }
 
 }  // namespace b200

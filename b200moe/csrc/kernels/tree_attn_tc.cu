@@ -1179,7 +1179,7 @@ void encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims
 }
 
 template <int D, bool SCALED>
-void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
+int launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
   CUtensorMap km, vm, qm;
   // columns as (64, D / 64): one copy brings both halves of a tile
   const cuuint64_t kd[5] = {64, (cuuint64_t)a.block_size, D / 64, (cuuint64_t)a.num_kv_heads, (cuuint64_t)a.num_blocks};
@@ -1201,7 +1201,8 @@ void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
   t.part_o = static_cast<float*>(p.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + (int64_t)p.grid * 2 * p.part_rows * D);
   // slices of the batch that fit the shared table of units (one launch for up to kTreeTcBatch sequences)
-  for (int b0 = 0; b0 < a.batch; b0 += kTreeTcBatch) {
+  int launches = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kTreeTcBatch, ++launches) {
     t.a.batch = std::min(kTreeTcBatch, a.batch - b0);
     t.a.cu_seqlens_q = a.cu_seqlens_q + b0;
     t.a.seq_lens = a.seq_lens + b0;
@@ -1213,6 +1214,7 @@ void launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
                                                       dim3(p.grid), dim3(kThreads), params, smem, s);
     if (e != cudaSuccess) throw std::runtime_error(std::string("tree_attn: ") + cudaGetErrorString(e));
   }
+  return launches;
 }
 
 }  // namespace
@@ -1232,14 +1234,9 @@ bool tree_attn_tc_plan(const TreeAttnArgs& a, int max_q_len, TreeAttnTcPlan* p) 
   return true;
 }
 
-void tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
-  if (p.key_scales != nullptr) {
-    if (a.head_dim == 128) launch<128, true>(a, p, s);
-    else launch<64, true>(a, p, s);
-  } else {
-    if (a.head_dim == 128) launch<128, false>(a, p, s);
-    else launch<64, false>(a, p, s);
-  }
+int tree_attn_tc(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
+  if (p.key_scales != nullptr) return a.head_dim == 128 ? launch<128, true>(a, p, s) : launch<64, true>(a, p, s);
+  return a.head_dim == 128 ? launch<128, false>(a, p, s) : launch<64, false>(a, p, s);
 }
 
 }  // namespace b200

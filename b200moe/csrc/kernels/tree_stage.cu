@@ -150,8 +150,9 @@ int64_t tree_stage_bytes(const TreeAttnArgs& a, int seqs) {
          (int64_t)seqs * a.num_kv_heads * 2 * key_stride(a) * 4 + round16(blocks * 4);
 }
 
-void tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, void* stage, cudaStream_t s) {
+int tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, void* stage, cudaStream_t s) {
   const int64_t plane = (int64_t)a.num_kv_heads * a.block_size * a.head_dim;
+  int launches = 0;
   for (int b0 = 0; b0 < a.batch; b0 += seqs) {
     TreeAttnArgs x = a;
     x.batch = std::min(seqs, a.batch - b0);
@@ -187,8 +188,9 @@ void tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, 
     x.block_tables = o.tables;
     x.block_stride = 2 * plane;
     x.num_blocks = (int)blocks;
-    tree_attn_tc(x, q, s);
+    launches += 1 + tree_attn_tc(x, q, s);
   }
+  return launches;
 }
 
 }  // namespace b200

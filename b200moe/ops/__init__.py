@@ -709,11 +709,11 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     table row has) is left out and a block id outside the pool is not read; both set the status word
     (``check_status``)."""
     if q.is_cuda:
-        out = native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q, seq_lens,
-                                 block_tables, parents, out, max_q_len, kv_layer.block_size, kv_layer.block_stride,
-                                 kv_layer.scale_block_stride, scale, status_word(q.device), _chan_read(kv_layer),
-                                 INT8_STAGE_MAX_BYTES)
-        count_launches(1 if q.shape[0] and seq_lens.shape[0] else 0)
+        out, launches = native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q,
+                                           seq_lens, block_tables, parents, out, max_q_len, kv_layer.block_size,
+                                           kv_layer.block_stride, kv_layer.scale_block_stride, scale,
+                                           status_word(q.device), _chan_read(kv_layer), INT8_STAGE_MAX_BYTES)
+        count_launches(launches)
         return out
     if q.dim() != 3 or not q.is_contiguous():
         raise ValueError("q must be contiguous [rows, q_heads, head_dim]")

@@ -1004,3 +1004,22 @@ def test_moe_few_tokens_logit_beside_a_tie(dev, T, at):
     out = ops.moe_few_tokens(x, router, w13, s13, w2, s2, E, 2, ids=ids, weights=wts)
     assert ids.tolist() == [[up, lo]] * T
     _moe_check(x, router, w13, s13, w2, s2, E, 2, True, out, ids, wts)
+
+
+@pytest.mark.gpu
+def test_tree_operators_count_their_launches(monkeypatch):
+    def launches(b, limit=None):
+        if limit is not None:
+            monkeypatch.setattr(ops, "INT8_STAGE_MAX_BYTES", limit)
+        before = ops.launch_count()
+        ops.tree_attention(*b.args())
+        return ops.launch_count() - before
+
+    assert launches(Batch("cuda", [4, 3], [40, 20], 8, 2, 64, 16)) == 1
+    assert launches(Batch("cuda", [4, 3], [40, 20], 8, 2, 64, 48)) == 1
+    assert launches(Batch("cuda", [1] * 1025, [2] * 1025, 4, 2, 64, 8)) == 2     # 1024 sequences at a time
+    b = Batch("cuda", [4, 3, 2], [40, 20, 9], 8, 2, 64, 16, int8=True)
+    assert launches(b) == 2                      # the stage and the attention that reads it
+    assert launches(b, limit=1) == 6             # one sequence at a time
+    assert launches(Batch("cuda", [4, 3], [40, 20], 8, 2, 64, 24, int8=True)) == 1
+    assert launches(Batch("cuda", [0, 0], [5, 0], 8, 2, 64, 16)) == 0
