@@ -776,17 +776,20 @@ void check_aligned(const Tensor& t, const char* name) {
   CHECK_VALUE((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name, " must start on a 16-byte boundary");
 }
 
-// int32 metadata of a batch of drafted trees: cu [B + 1], lens [B], tables [B, max_blocks], parents [rows].
+// int32 metadata of a batch of drafted trees: cu [B + 1], lens [B], tables [B, max_blocks] (rows may lie apart),
+// parents [rows].
 void check_tree(const Tensor& cu, const Tensor& lens, const Tensor& tables, const Tensor& parents,
                 c10::Device dev, int64_t max_q_len) {
   for (const Tensor* t : {&cu, &lens, &tables, &parents}) {
     CHECK_VALUE(t->device() == dev, "tree metadata must be on ", dev, ", got ", t->device());
-    CHECK_VALUE(t->scalar_type() == torch::kInt32 && t->is_contiguous(), "tree metadata must be contiguous int32");
+    CHECK_VALUE(t->scalar_type() == torch::kInt32 && (t == &tables || t->is_contiguous()),
+                "tree metadata must be contiguous int32");
   }
   CHECK_VALUE(cu.dim() == 1 && lens.dim() == 1 && cu.numel() == lens.numel() + 1,
               "cu_seqlens_q must hold one entry more than seq_lens");
   CHECK_VALUE(tables.dim() == 2 && tables.size(0) == lens.numel() && tables.size(1) >= 1,
               "block_tables must be [batch, max_blocks]");
+  CHECK_VALUE(tables.stride(1) == 1 || tables.size(1) == 1, "rows of block_tables must be contiguous");
   CHECK_VALUE(parents.dim() == 1, "parents must be [rows]");
   CHECK_VALUE(max_q_len >= 1 && max_q_len <= b200::kTreeMaxNodes, "max_q_len must be in [1, ",
               std::to_string(b200::kTreeMaxNodes), "], got ", std::to_string(max_q_len));
@@ -843,6 +846,7 @@ std::tuple<Tensor, int> tree_attn(Tensor q, Tensor k_cache, Tensor v_cache,
   a.cu_seqlens_q = cu.data_ptr<int>();
   a.seq_lens = lens.data_ptr<int>();
   a.block_tables = tables.data_ptr<int>();
+  a.table_stride = tables.stride(0);
   a.parents = parents.data_ptr<int>();
   a.batch = (int)lens.numel();
   a.rows = (int)q.size(0);
@@ -864,10 +868,10 @@ std::tuple<Tensor, int> tree_attn(Tensor q, Tensor k_cache, Tensor v_cache,
     Tensor ws = torch::empty({plan.workspace_bytes}, q.options().dtype(torch::kUInt8));
     plan.workspace = ws.data_ptr();
     if (a.kv_int8) {
-      // as many sequences at a time as the stage may hold, at least one
-      const int most = std::min(a.batch, b200::kTreeTcBatch);
+      // as many sequences at a time as the stage may hold, at least one, in slices of one size
       const int64_t one = b200::tree_stage_bytes(a, 1);
-      const int seqs = (int)std::min<int64_t>(most, std::max<int64_t>(1, stage_limit / one));
+      const int most = (int)std::min<int64_t>(std::min(a.batch, b200::kTreeTcBatch), std::max<int64_t>(1, stage_limit / one));
+      const int slices = (a.batch + most - 1) / most, seqs = (a.batch + slices - 1) / slices;
       Tensor stage = torch::empty({b200::tree_stage_bytes(a, seqs)}, q.options().dtype(torch::kUInt8));
       return {out, b200::tree_attn_staged(a, plan, seqs, stage.data_ptr(), stream())};
     }
@@ -912,6 +916,7 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
   a.cu_seqlens_q = cu.data_ptr<int>();
   a.seq_lens = lens.data_ptr<int>();
   a.block_tables = tables.data_ptr<int>();
+  a.table_stride = tables.stride(0);
   a.parents = parents.data_ptr<int>();
   a.draft = draft.data_ptr<int>();
   a.target = target.data_ptr<int>();

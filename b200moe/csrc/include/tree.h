@@ -29,7 +29,8 @@ struct TreeAttnArgs {
   KvChannel ch;
   const int* cu_seqlens_q;   // [batch + 1] first node of each sequence
   const int* seq_lens;       // [batch] keys: committed prefix + nodes
-  const int* block_tables;   // [batch, max_blocks]
+  const int* block_tables;   // [batch, max_blocks], rows table_stride apart
+  int64_t table_stride;
   const int* parents;        // [rows] place of a node's parent in its tree, -1: none
   int batch;
   int rows;
@@ -83,7 +84,8 @@ struct TreeCommitArgs {
   int num_blocks;
   const int* cu_seqlens_q;   // [batch + 1]
   const int* seq_lens;       // [batch] committed prefix + nodes
-  const int* block_tables;   // [batch, max_blocks]
+  const int* block_tables;   // [batch, max_blocks], rows table_stride apart
+  int64_t table_stride;
   const int* parents;        // [nodes]
   const int* draft;          // [nodes] drafted token of each node
   const int* target;         // [nodes] token the model picks behind each node

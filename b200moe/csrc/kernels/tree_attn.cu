@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeAttnAr
   const int n = q1 - q0, node = row - q0, prefix = len - n;
   for (int i = threadIdx.x; i < n; i += kWarps * 32) s_par[i] = a.parents[q0 + i];
   __syncthreads();
-  const int* tab = a.block_tables + (int64_t)b * a.max_blocks;
+  const int* tab = a.block_tables + b * a.table_stride;
   const float sl2 = a.scale * 1.4426950408889634f;
   bool bad = false;
   for (int g = warp; g < a.group; g += kWarps) {

@@ -344,7 +344,7 @@ struct Blocks {
   bool bad;
   __device__ __forceinline__ int entry(int i) const { return i < max_blocks ? __ldg(tab + i) : -1; }
   __device__ __forceinline__ void start(const TreeAttnArgs& a, int b, int key, int keys, int lane) {
-    tab = a.block_tables + (int64_t)b * a.max_blocks;
+    tab = a.block_tables + b * a.table_stride;
     len = keys;
     bi = key / block_size;
     y = key - bi * block_size;
@@ -1025,7 +1025,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             // V elements that were not finite count for the rows that see their node
             for (int d = 0; d < g.n; ++d) {
               if (!((dirt[d >> 5] & anc[node * kAncWords + (d >> 5)]) >> (d & 31) & 1u)) continue;
-              const int key = prefix + d, id = a.block_tables[(int64_t)g.b * a.max_blocks + key / a.block_size];
+              const int key = prefix + d, id = a.block_tables[g.b * a.table_stride + key / a.block_size];
               const bf16* v = static_cast<const bf16*>(a.v_cache) + (int64_t)id * a.block_stride +
                               ((int64_t)g.h * a.block_size + key % a.block_size) * D + c;
 #pragma unroll 1
@@ -1206,7 +1206,7 @@ int launch(const TreeAttnArgs& a, const TreeAttnTcPlan& p, cudaStream_t s) {
     t.a.batch = std::min(kTreeTcBatch, a.batch - b0);
     t.a.cu_seqlens_q = a.cu_seqlens_q + b0;
     t.a.seq_lens = a.seq_lens + b0;
-    t.a.block_tables = a.block_tables + (int64_t)b0 * a.max_blocks;
+    t.a.block_tables = a.block_tables + b0 * a.table_stride;
     const int smem = Lay<D>::smem(kTreeTcBatch);
     smem_opt_in(tree_attn_tc_kernel<D, SCALED>, smem);
     void* params[] = {&km, &vm, &qm, &t};

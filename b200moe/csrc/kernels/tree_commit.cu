@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const TreeCommitA
     }
     __syncwarp();
     // the path's rows that change places, as pool slots
-    const int* tab = a.block_tables + (int64_t)b * a.max_blocks;
+    const int* tab = a.block_tables + b * a.table_stride;
     int moved = 0;
     bool out_of_range = false;
     for (int j0 = 0; j0 < len; j0 += 32) {

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads) tree_stage_kernel(const TreeAttnArgs
   const int64_t items = (int64_t)nb * 2 * pieces;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int piece = (int)(it % pieces), kv = (int)(it / pieces) & 1, j = (int)(it / pieces / 2);
-    const int id = a.block_tables[(int64_t)b * a.max_blocks + j];
+    const int id = a.block_tables[b * a.table_stride + j];
     const bool ok = id >= 0 && id < a.num_blocks;
     const int64_t slot = (int64_t)b * a.max_blocks + j;
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const int8_t*>(kv ? a.v_cache : a.k_cache) +
@@ -158,7 +158,7 @@ int tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, v
     x.batch = std::min(seqs, a.batch - b0);
     x.cu_seqlens_q += b0;
     x.seq_lens += b0;
-    x.block_tables += (int64_t)b0 * a.max_blocks;
+    x.block_tables += b0 * a.table_stride;
     const int64_t blocks = (int64_t)x.batch * a.max_blocks;
     Stage o;
     o.kv = static_cast<bf16*>(stage);
@@ -186,6 +186,7 @@ int tree_attn_staged(const TreeAttnArgs& a, const TreeAttnTcPlan& p, int seqs, v
     x.k_cache = o.kv;
     x.v_cache = o.kv + plane;
     x.block_tables = o.tables;
+    x.table_stride = a.max_blocks;
     x.block_stride = 2 * plane;
     x.num_blocks = (int)blocks;
     launches += 1 + tree_attn_tc(x, q, s);

@@ -53,7 +53,7 @@ class StepInputs:
     logits_indices: torch.Tensor   # int32 [B] token index whose logits are sampled
     num_decode: int                # rows [0, num_decode) are single-token decode rows
     max_q_len: int                 # over prefill rows
-    max_seq_len: int               # over all rows (decode split sizing)
+    max_seq_len: int               # over all rows (decode split sizing; table columns of tree rows, int8 pool)
     num_rows: int
     prefill_cu: torch.Tensor | None = None  # cu_seqlens of the prefill rows, rebased to 0
     feed_src: torch.Tensor | None = None    # int32 [T]: >= 0 -> the id is feed_tokens[feed_src[t]]
@@ -396,12 +396,21 @@ class Qwen3MoeForCausalLM(nn.Module):
                     ops.decode_attention(q[:nd], kvl, inp.block_tables[:nd], inp.seq_lens[:nd], self.scale,
                                          out[:nd], split_len, nsplit, ws)
                 if inp.num_rows > nd and inp.tree_parents is not None:
-                    ops.tree_attention(q[nd:], kvl, cu, inp.seq_lens[nd:], inp.block_tables[nd:], inp.tree_parents,
+                    ops.tree_attention(q[nd:], kvl, cu, inp.seq_lens[nd:], self._tree_tables(inp, kvl), inp.tree_parents,
                                        inp.max_q_len, self.scale, out[nd:])
                 elif inp.num_rows > nd:
                     ops.prefill_attention(q[nd:], kvl, cu, inp.seq_lens[nd:], inp.block_tables[nd:],
                                           inp.max_q_len, self.scale, out[nd:])
         return out.view(T, nq * D)  # the O projection is applied by the caller
+
+    @staticmethod
+    def _tree_tables(inp: StepInputs, kvl):
+        """Block tables of the tree rows; for an int8 pool no wider than the step's longest row needs, because
+        the operator's stage is as wide (a captured step may be replayed on longer rows: all columns)."""
+        tables = inp.block_tables[inp.num_decode:]
+        if kvl.k.dtype == torch.int8 and not (tables.is_cuda and torch.cuda.is_current_stream_capturing()):
+            tables = tables[:, :max(1, -(-inp.max_seq_len // kvl.block_size))]
+        return tables
 
     def decode_splits(self, rows: int, max_len: int) -> tuple[int, int]:
         """Keys per split and split count for flash-decoding: enough CTAs to

@@ -677,17 +677,24 @@ def _attention_ref(q, kv_layer, block_tables, seq_lens, cu_seqlens_q, scale, out
 
 # ------------------------------------------------------------- drafted trees
 TREE_MAX_NODES = 256   # nodes of one drafted tree
+# The bf16 stage of an int8 pool in tree attention: allocated for the call, so it comes out of what the KV budget
+# leaves for transient tensors (3 GiB), where INT8_STAGE_MAX_BYTES is reserved and held by the prefill stage.
+# 64 sequences of 4112 keys (0.56 GB): 338 us in two slices, 329 in one; with 256 MB 385, and 16 of 8208 keys 199
+# instead of 173.
+TREE_STAGE_MAX_BYTES = int(os.environ.get("B200MOE_TREE_STAGE_MB", "512")) << 20
 
 
 def _check_tree(rows, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, device):
     for name, t in (("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens), ("block_tables", block_tables),
                     ("parents", parents)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+        if t.dtype != torch.int32 or not (t.is_contiguous() or t is block_tables) or t.device != device:
             raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
     if cu_seqlens_q.dim() != 1 or seq_lens.dim() != 1 or cu_seqlens_q.shape[0] != seq_lens.shape[0] + 1:
         raise ValueError("cu_seqlens_q must hold one entry more than seq_lens")
     if block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0] or block_tables.shape[1] < 1:
         raise ValueError("block_tables must be [batch, max_blocks]")
+    if block_tables.stride(1) != 1 and block_tables.shape[1] > 1:
+        raise ValueError("rows of block_tables must be contiguous")
     if parents.dim() != 1 or (rows is not None and parents.shape[0] != rows):
         raise ValueError("parents must hold one entry per row")
     if not 1 <= max_q_len <= TREE_MAX_NODES:
@@ -703,8 +710,10 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     stored before the call, as for ``prefill_attention``).  parents [rows]: place of a node's parent in
     its tree, below the node's own; -1 for a node that follows the prefix directly.  max_q_len: no tree
     has more nodes (at most ``TREE_MAX_NODES``).  Chains (parents i - 1) give causal attention.  Rows
-    behind the last sequence are left as they are.  bf16 and int8 pools (int8 through a bf16 stage of at
-    most ``INT8_STAGE_MAX_BYTES``, or of one sequence), head_dim 64 or 128; out must not overlap q.  A tree
+    behind the last sequence are left as they are.  bf16 and int8 pools, head_dim 64 or 128; out must
+    not overlap q.  int8 pools go through a bf16 stage of as many sequences at a time as ``TREE_STAGE_MAX_BYTES`` and
+    ``INT8_STAGE_MAX_BYTES`` hold, at least one, each as long as its table row; a graph keeps the stage of a captured
+    call.  block_tables may be a view of the first columns of a wider table, which makes it shorter.  A tree
     that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
     table row has) is left out and a block id outside the pool is not read; both set the status word
     (``check_status``)."""
@@ -712,7 +721,8 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
         out, launches = native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q,
                                            seq_lens, block_tables, parents, out, max_q_len, kv_layer.block_size,
                                            kv_layer.block_stride, kv_layer.scale_block_stride, scale,
-                                           status_word(q.device), _chan_read(kv_layer), INT8_STAGE_MAX_BYTES)
+                                           status_word(q.device), _chan_read(kv_layer),
+                                           min(INT8_STAGE_MAX_BYTES, TREE_STAGE_MAX_BYTES))
         count_launches(launches)
         return out
     if q.dim() != 3 or not q.is_contiguous():

@@ -1023,3 +1023,72 @@ def test_tree_operators_count_their_launches(monkeypatch):
     assert launches(b, limit=1) == 6             # one sequence at a time
     assert launches(Batch("cuda", [4, 3], [40, 20], 8, 2, 64, 24, int8=True)) == 1
     assert launches(Batch("cuda", [0, 0], [5, 0], 8, 2, 64, 16)) == 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bs,int8", [(16, False), (48, False), (16, True), (48, True)])
+def test_tree_operators_take_a_view_of_a_wider_table(dev, bs, int8):
+    b = Batch(dev, [5, 1, 9], [70, 0, 130], 8, 2, 64, bs, int8=int8)
+    wide = torch.full((3, 40), -1, dtype=torch.int32, device=dev)
+    wide[:, :b.tables.shape[1]] = b.tables
+    view = wide[:, :b.tables.shape[1]]
+    assert not view.is_contiguous()
+    want = ops.tree_attention(*b.args())
+    got = ops.tree_attention(b.q, b.layer, b.cu, b.lens, view, b.parents, b.max_nodes, b.scale)
+    assert torch.equal(got, want)
+    data, scales = b.pool.data.clone(), None if b.pool.scales is None else b.pool.scales.clone()
+    draft = torch.ones_like(b.parents)
+    args = (draft, draft, b.max_nodes)
+    x = ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, *args, kv_scales=b.pool.scales)
+    y = ops.tree_commit(data, b.cu, b.lens, view, b.parents, *args, kv_scales=scales)
+    assert all(torch.equal(s, t) for s, t in zip(x, y)) and torch.equal(data, b.pool.data)
+    with pytest.raises(ValueError):              # rows that are not contiguous
+        ops.tree_attention(b.q, b.layer, b.cu, b.lens, wide.t().contiguous().t(), b.parents, b.max_nodes, b.scale)
+
+
+def test_verify_step_narrows_the_tables_of_an_int8_pool(monkeypatch):
+    """The stage of an int8 pool is as wide as the tables: the model hands over the columns that the step uses."""
+    attn, widths = ops.tree_attention, []
+
+    def spy(q, layer, cu, lens, tables, *rest):
+        widths.append(tables.shape[1])
+        return attn(q, layer, cu, lens, tables, *rest)
+
+    monkeypatch.setattr(ops, "tree_attention", spy)
+    for int8 in (False, True):
+        d = Decoder("cpu", PROMPTS, int8=int8)
+        d.prefill()
+        truth = [t + list(range(1, 99)) for t in d.seqs]
+        parents, ids = d.drafts(truth, 2, torch.Generator().manual_seed(3))
+        longest = max(len(t) - 1 + len(p) for t, p in zip(d.seqs, parents))
+        widths.clear()
+        d.verify(parents, ids)
+        assert set(widths) == {-(-longest // d.bs) if int8 else 12}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["token", "channel"])
+def test_tree_int8_stage_stays_within_its_limit(mode):
+    """64 short sequences in tables of 200 blocks would fill a stage of 1.7 GB: the call allocates no more than the
+    limit, and with the columns in use alone a small stage and two launches."""
+    b = Batch("cuda", [8] * 64, [300] * 64, 32, 4, 128, 64, int8=True, mode=mode)
+    wide = torch.zeros(64, 200, dtype=torch.int32, device="cuda")
+    wide[:, :b.tables.shape[1]] = b.tables
+    want = ops.tree_attention(*b.args())
+
+    def call(tables):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        mem, before = torch.cuda.memory_allocated(), ops.launch_count()
+        out = ops.tree_attention(b.q, b.layer, b.cu, b.lens, tables, b.parents, b.max_nodes, b.scale)
+        torch.cuda.synchronize()
+        return out, torch.cuda.max_memory_allocated() - mem, ops.launch_count() - before
+
+    rest = 148 * 2 * 128 * (128 * 4 + 8) + want.nbytes + (4 << 20)   # partial results, the output, rounding
+    out, used, _ = call(wide)
+    b.check(out)
+    assert used <= (512 << 20) + rest
+    out, used, launches = call(wide[:, :b.tables.shape[1]])
+    assert torch.equal(out, want) and launches == 2
+    assert used <= 64 * b.tables.shape[1] * 64 * 4 * (128 * 4 + 8) + rest
