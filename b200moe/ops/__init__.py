@@ -701,6 +701,20 @@ def _check_tree(rows, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, 
         raise ValueError(f"max_q_len must be in [1, {TREE_MAX_NODES}], got {max_q_len}")
 
 
+def _check_tree_row(b, q0, q1, keys, rows, max_q_len):
+    if not 0 <= q0 <= q1 <= rows or q1 - q0 > max_q_len or (q0 < q1 and keys < q1 - q0):
+        raise ValueError(f"sequence {b}: {q1 - q0} nodes at row {q0} do not fit its {keys} keys, the {rows} rows or "
+                         f"max_q_len {max_q_len}")
+
+
+def _check_tree_block(b, block_tables, i, num_blocks):
+    """Block i of sequence b, a block of the pool."""
+    at = int(block_tables[b, i]) if i < block_tables.shape[1] else -1
+    if not 0 <= at < num_blocks:
+        raise ValueError(f"sequence {b}: its block {i} is not in the table or not in the pool")
+    return at
+
+
 def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, scale, out=None):
     """Attention of drafted trees over the paged pool: each node sees its sequence's
     committed prefix, its ancestors and itself.
@@ -716,7 +730,7 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     call.  block_tables may be a view of the first columns of a wider table, which makes it shorter.  A tree
     that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
     table row has) is left out and a block id outside the pool is not read; both set the status word
-    (``check_status``)."""
+    (``check_status``; the CPU path raises)."""
     if q.is_cuda:
         out, launches = native().tree_attn(q, kv_layer.k, kv_layer.v, kv_layer.k_scale, kv_layer.v_scale, cu_seqlens_q,
                                            seq_lens, block_tables, parents, out, max_q_len, kv_layer.block_size,
@@ -738,6 +752,11 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
         raise ValueError("q and out must not overlap")
     if q.shape[1] % kv_layer.num_kv_heads:
         raise ValueError("q heads must be a multiple of kv heads")
+    cu = cu_seqlens_q.tolist()
+    for b, keys in enumerate(seq_lens.tolist()):
+        _check_tree_row(b, cu[b], cu[b + 1], keys, q.shape[0], max_q_len)
+        for i in range(-(-keys // kv_layer.block_size) if cu[b] < cu[b + 1] else 0):
+            _check_tree_block(b, block_tables, i, kv_layer.k.shape[0])
     return _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, scale, out)
 
 
@@ -748,10 +767,9 @@ def _tree_attention_ref(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, paren
     cu, lens, par = cu_seqlens_q.tolist(), seq_lens.tolist(), parents.tolist()
     for b, L in enumerate(lens):
         q0, n = cu[b], cu[b + 1] - cu[b]
-        if n <= 0:
+        _check_tree_row(b, q0, q0 + n, L, q.shape[0], TREE_MAX_NODES)
+        if n == 0:
             continue
-        if L < n or q0 < 0 or q0 + n > q.shape[0]:
-            raise ValueError(f"sequence {b}: {n} nodes at row {q0} do not fit its {L} keys or the {q.shape[0]} rows")
         k, v = (t.float() for t in kv_layer.gather(block_tables[b], L))
         for i in range(n):   # one node's keys at a time: what it does not see is not touched, NaN or not
             seen, at = [], i
@@ -805,12 +823,12 @@ def _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, dra
     path = torch.full((B, max_q_len), -1, dtype=torch.int32)
     tokens = torch.full((B, max_q_len), -1, dtype=torch.int32)
     cu, lens = cu_seqlens_q.tolist(), seq_lens.tolist()
+    moves = []   # (block, row) pairs, carried out once every row has been checked
     for b in range(B):
         q0, n = cu[b], cu[b + 1] - cu[b]
+        _check_tree_row(b, q0, q0 + n, lens[b], parents.shape[0], max_q_len)
         if n == 0:
             continue
-        if n < 0 or n > max_q_len or q0 < 0 or q0 + n > parents.shape[0] or lens[b] < n:
-            raise ValueError(f"sequence {b}: {n} nodes at row {q0} do not fit")
         par, dr, ta = (t[q0:q0 + n].tolist() for t in (parents, draft_ids, target_ids))
         at, j = 0, 0
         while at is not None:
@@ -819,11 +837,14 @@ def _tree_commit_ref(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, dra
             at = next((c for c in range(at + 1, n) if par[c] == at and dr[c] == ta[at]), None)
         accepted[b] = j
         for i, node in enumerate(path[b, :j].tolist()):
-            src, dst = lens[b] - n + node, lens[b] - n + i
-            sb, db = int(block_tables[b, src // bs]), int(block_tables[b, dst // bs])
-            for t in (kv_data, kv_scales, kv_side):
-                if t is not None and src != dst:
-                    t[db, :, :, :, dst % bs] = t[sb, :, :, :, src % bs]
+            if node != i:
+                src, dst = ((_check_tree_block(b, block_tables, x // bs, kv_data.shape[0]), x % bs)
+                            for x in (lens[b] - n + node, lens[b] - n + i))
+                moves.append((src, dst))
+    for (sb, sy), (db, dy) in moves:
+        for t in (kv_data, kv_scales, kv_side):
+            if t is not None:
+                t[db, :, :, :, dy] = t[sb, :, :, :, sy]
     return accepted, path, tokens
 
 

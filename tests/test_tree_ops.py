@@ -1092,3 +1092,32 @@ def test_tree_int8_stage_stays_within_its_limit(mode):
     out, used, launches = call(wide[:, :b.tables.shape[1]])
     assert torch.equal(out, want) and launches == 2
     assert used <= 64 * b.tables.shape[1] * 64 * 4 * (128 * 4 + 8) + rest
+
+
+@pytest.mark.parametrize("what", ["long", "descend", "outside", "prefix", "table", "block", "negative"])
+def test_tree_operators_on_the_cpu_refuse_what_does_not_fit(what):
+    """What the kernels leave out and report in the status word is a ValueError on the CPU."""
+    b = Batch("cpu", [4, 9, 3], [40, 20, 5], 8, 2, 64, 16, "star")
+    q, kv, cu, lens, tab, par, n, sc = b.args()
+    draft = torch.zeros_like(par)
+    target = torch.zeros_like(par)
+    draft[4 + 1:4 + 9] = 1                       # the second tree accepts its last node alone: a row moves
+    draft[4 + 8] = 0
+    if what == "long":
+        n = 8                                    # of 9 nodes
+    elif what == "descend":
+        cu[1], cu[2] = 13, 4
+    elif what == "outside":
+        cu[3] = 17
+    elif what == "prefix":
+        lens[1] = 8
+    elif what == "table":
+        tab = tab[:, :1].contiguous()            # the nodes lie in the second block
+    else:
+        tab[1, 1] = b.pool.num_blocks if what == "block" else -1
+    before = b.pool.data.clone()
+    with pytest.raises(ValueError):
+        ops.tree_attention(q, kv, cu, lens, tab, par, n, sc)
+    with pytest.raises(ValueError):
+        ops.tree_commit(b.pool.data, cu, lens, tab, par, draft, target, n)
+    assert torch.equal(before, b.pool.data)
