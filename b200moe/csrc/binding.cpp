@@ -818,6 +818,7 @@ std::tuple<Tensor, int> tree_attn(Tensor q, Tensor k_cache, Tensor v_cache,
                 t->stride(3) == 1, "cache planes must be contiguous [kv_heads, block_size, head_dim]");
   CHECK_VALUE(D == 64 || D == 128, "head_dim must be 64 or 128, got ", std::to_string(D));
   CHECK_VALUE(nkv >= 1 && nq >= 1 && nq % nkv == 0, "q heads must be a multiple of kv heads");
+  CHECK_VALUE(block_size >= 1, "cache blocks must hold rows");
   const bool int8 = k_cache.scalar_type() == torch::kInt8;
   CHECK_VALUE(int8 || k_cache.scalar_type() == torch::kBFloat16, "cache must be bf16 or int8");
   check_tree(cu, lens, tables, parents, q.device(), max_q_len);
@@ -888,6 +889,8 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
   check_contiguous(kv_data, "kv_data");
   CHECK_VALUE(kv_data.dim() == 6 && kv_data.size(2) == 2,
               "kv_data must be [blocks, layers, 2, kv_heads, block_size, head_dim]");
+  CHECK_VALUE(kv_data.size(1) >= 1 && kv_data.size(3) >= 1 && kv_data.size(4) >= 1,
+              "kv_data must have layers, heads and rows");
   check_tree(cu, lens, tables, parents, kv_data.device(), max_q_len);
   for (const Tensor* t : {&draft, &target})
     CHECK_VALUE(t->device() == kv_data.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous() &&

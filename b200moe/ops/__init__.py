@@ -752,6 +752,8 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
         raise ValueError("q and out must not overlap")
     if q.shape[1] % kv_layer.num_kv_heads:
         raise ValueError("q heads must be a multiple of kv heads")
+    if kv_layer.block_size < 1:
+        raise ValueError("cache blocks must hold rows")
     cu = cu_seqlens_q.tolist()
     for b, keys in enumerate(seq_lens.tolist()):
         _check_tree_row(b, cu[b], cu[b + 1], keys, q.shape[0], max_q_len)
@@ -809,6 +811,8 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
             raise ValueError(f"{name} must be int32 like parents")
     if kv_data.dim() != 6 or kv_data.shape[2] != 2 or not kv_data.is_contiguous():
         raise ValueError("kv_data must be contiguous [blocks, layers, 2, kv_heads, block_size, head_dim]")
+    if 0 in kv_data.shape[1:5]:
+        raise ValueError("kv_data must have layers, heads and rows")
     for name, t in (("kv_scales", kv_scales), ("kv_side", kv_side)):
         if t is not None and (t.shape[:5] != kv_data.shape[:5] or not t.is_contiguous() or t.device != kv_data.device):
             raise ValueError(f"{name} must be contiguous rows [blocks, layers, 2, kv_heads, block_size] like kv_data")

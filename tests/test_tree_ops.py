@@ -1121,3 +1121,17 @@ def test_tree_operators_on_the_cpu_refuse_what_does_not_fit(what):
     with pytest.raises(ValueError):
         ops.tree_commit(b.pool.data, cu, lens, tab, par, draft, target, n)
     assert torch.equal(before, b.pool.data)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_operators_refuse_a_pool_without_slots(dev):
+    b = Batch(dev, [4], [20], 8, 2, 128, 16)
+    d = torch.zeros_like(b.parents)
+    shape = list(b.pool.data.shape)
+    for dim in (1, 3, 4):                        # no layers, no heads, blocks of no rows
+        data = b.pool.data.new_zeros([0 if i == dim else n for i, n in enumerate(shape)])
+        with pytest.raises(ValueError):
+            ops.tree_commit(data, b.cu, b.lens, b.tables, b.parents, d, d, b.max_nodes)
+    empty = KVPool(3, 1, 2, 0, 128, torch.bfloat16, dev)
+    with pytest.raises(ValueError):
+        ops.tree_attention(b.q, empty.layer(0), b.cu, b.lens, b.tables, b.parents, b.max_nodes, b.scale)
