@@ -891,6 +891,8 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
               "kv_data must be [blocks, layers, 2, kv_heads, block_size, head_dim]");
   CHECK_VALUE(kv_data.size(1) >= 1 && kv_data.size(3) >= 1 && kv_data.size(4) >= 1,
               "kv_data must have layers, heads and rows");
+  CHECK_VALUE(kv_data.scalar_type() != torch::kInt8 || kv_scales.has_value() || kv_side.has_value(),
+              "int8 rows move with their kv_scales or kv_side");
   check_tree(cu, lens, tables, parents, kv_data.device(), max_q_len);
   for (const Tensor* t : {&draft, &target})
     CHECK_VALUE(t->device() == kv_data.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous() &&

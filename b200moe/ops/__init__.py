@@ -813,6 +813,8 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
         raise ValueError("kv_data must be contiguous [blocks, layers, 2, kv_heads, block_size, head_dim]")
     if 0 in kv_data.shape[1:5]:
         raise ValueError("kv_data must have layers, heads and rows")
+    if kv_data.dtype == torch.int8 and kv_scales is None and kv_side is None:
+        raise ValueError("int8 rows move with their kv_scales or kv_side")
     for name, t in (("kv_scales", kv_scales), ("kv_side", kv_side)):
         if t is not None and (t.shape[:5] != kv_data.shape[:5] or not t.is_contiguous() or t.device != kv_data.device):
             raise ValueError(f"{name} must be contiguous rows [blocks, layers, 2, kv_heads, block_size] like kv_data")

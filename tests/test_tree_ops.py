@@ -1135,3 +1135,14 @@ def test_tree_operators_refuse_a_pool_without_slots(dev):
     empty = KVPool(3, 1, 2, 0, 128, torch.bfloat16, dev)
     with pytest.raises(ValueError):
         ops.tree_attention(b.q, empty.layer(0), b.cu, b.lens, b.tables, b.parents, b.max_nodes, b.scale)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tree_commit_refuses_int8_rows_without_their_scales(dev):
+    """Moving the payload alone would leave every moved row with another row's scale."""
+    for mode in ("token", "channel"):
+        b, draft, target = _commit_case(dev, 1, [6, 3], [10, 4], True, mode)
+        before = b.pool.data.clone()
+        with pytest.raises(ValueError):
+            ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, draft, target, b.max_nodes)
+        assert torch.equal(before, b.pool.data)
