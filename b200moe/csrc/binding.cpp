@@ -881,11 +881,12 @@ std::tuple<Tensor, int> tree_attn(Tensor q, Tensor k_cache, Tensor v_cache,
   return {out, b200::tree_attn(a, stream())};
 }
 
-// Accepted paths of a batch of trees; the rows of kv_data (and scales / side) move in place.
-std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Tensor> kv_scales,
-                                               c10::optional<Tensor> kv_side, Tensor cu, Tensor lens, Tensor tables,
-                                               Tensor parents, Tensor draft, Tensor target, int64_t max_q_len,
-                                               Tensor status) {
+// Accepted paths of a batch of trees and the number of kernels launched; the rows of kv_data (and scales / side) move
+// in place.
+std::tuple<Tensor, Tensor, Tensor, int> tree_commit(Tensor kv_data, c10::optional<Tensor> kv_scales,
+                                                    c10::optional<Tensor> kv_side, Tensor cu, Tensor lens,
+                                                    Tensor tables, Tensor parents, Tensor draft, Tensor target,
+                                                    int64_t max_q_len, Tensor status) {
   check_contiguous(kv_data, "kv_data");
   CHECK_VALUE(kv_data.dim() == 6 && kv_data.size(2) == 2,
               "kv_data must be [blocks, layers, 2, kv_heads, block_size, head_dim]");
@@ -934,8 +935,8 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(Tensor kv_data, c10::optional<Ten
   a.tokens = tokens.data_ptr<int>();
   a.status = status.data_ptr<int>();
   c10::cuda::CUDAGuard guard(kv_data.device());
-  b200::tree_commit(a, stream());
-  return {accepted, path, tokens};
+  const int launches = b200::tree_commit(a, stream());
+  return {accepted, path, tokens, launches};
 }
 
 Tensor moe_few(Tensor x, Tensor router, Tensor w13, c10::optional<Tensor> s13, Tensor w2, c10::optional<Tensor> s2,

@@ -98,6 +98,7 @@ struct TreeCommitArgs {
   int* tokens;               // [batch, max_q_len], -1 behind the path
   int* status;
 };
-void tree_commit(const TreeCommitArgs& a, cudaStream_t s);
+// Returns the number of kernels that it launched.
+int tree_commit(const TreeCommitArgs& a, cudaStream_t s);
 
 }  // namespace b200

@@ -151,12 +151,24 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const TreeCommitA
 
 }  // namespace
 
-void tree_commit(const TreeCommitArgs& a, cudaStream_t s) {
-  if (a.batch == 0) return;
+int tree_commit(const TreeCommitArgs& a, cudaStream_t s) {
   const int per = 8;   // planes of a CTA
-  pdl_launch(tree_commit_kernel, dim3((a.planes + per - 1) / per, a.batch), kThreads, 0, s, a, per);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) throw std::runtime_error(std::string("tree_commit: ") + cudaGetErrorString(e));
+  constexpr int kMost = 65535;   // blocks of a grid in y
+  int launches = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kMost, ++launches) {
+    TreeCommitArgs x = a;
+    x.batch = std::min(kMost, a.batch - b0);
+    x.cu_seqlens_q += b0;
+    x.seq_lens += b0;
+    x.block_tables += b0 * a.table_stride;
+    x.accepted += b0;
+    x.path += (int64_t)b0 * a.max_q_len;
+    x.tokens += (int64_t)b0 * a.max_q_len;
+    pdl_launch(tree_commit_kernel, dim3((x.planes + per - 1) / per, x.batch), kThreads, 0, s, x, per);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) throw std::runtime_error(std::string("tree_commit: ") + cudaGetErrorString(e));
+  }
+  return launches;
 }
 
 }  // namespace b200

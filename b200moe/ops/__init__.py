@@ -801,10 +801,11 @@ def tree_commit(kv_data, cu_seqlens_q, seq_lens, block_tables, parents, draft_id
     P + accepted.  A malformed row accepts nothing, a move through a block id outside the pool is left
     out; both set the status word (the CPU path raises)."""
     if kv_data.is_cuda:
-        res = native().tree_commit(kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents,
-                                   draft_ids, target_ids, max_q_len, status_word(kv_data.device))
-        count_launches(1 if seq_lens.shape[0] else 0)
-        return res
+        accepted, path, tokens, launches = native().tree_commit(
+            kv_data, kv_scales, kv_side, cu_seqlens_q, seq_lens, block_tables, parents, draft_ids, target_ids, max_q_len,
+            status_word(kv_data.device))
+        count_launches(launches)
+        return accepted, path, tokens
     _check_tree(None, cu_seqlens_q, seq_lens, block_tables, parents, max_q_len, kv_data.device)
     for name, t in (("draft_ids", draft_ids), ("target_ids", target_ids)):
         if t.dtype != torch.int32 or t.shape != parents.shape or t.device != kv_data.device or not t.is_contiguous():

@@ -1146,3 +1146,25 @@ def test_tree_commit_refuses_int8_rows_without_their_scales(dev):
         with pytest.raises(ValueError):
             ops.tree_commit(b.pool.data, b.cu, b.lens, b.tables, b.parents, draft, target, b.max_nodes)
         assert torch.equal(before, b.pool.data)
+
+
+@pytest.mark.gpu
+def test_tree_commit_of_more_sequences_than_a_grid_is_high():
+    """65,540 trees of three nodes: a grid has 65,535 rows of blocks at most."""
+    B, n, bs = 65540, 3, 4
+    i32 = dict(dtype=torch.int32, device="cuda")
+    data = torch.randn(B, 1, 2, 1, bs, 8, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    cu, lens = torch.arange(0, B * n + 1, n, **i32), torch.full((B,), n + 1, **i32)
+    tables = torch.arange(B, **i32).flip(0).unsqueeze(1).contiguous()
+    parents = torch.tensor([-1, 0, 0], **i32).repeat(B)
+    draft = torch.tensor([9, 1, 2], **i32).repeat(B)
+    target = torch.tensor([2, 0, 0], **i32).repeat(B)        # node 2 is accepted: slot 3 moves to slot 2
+    want = data.clone()
+    want[:, :, :, :, 2] = data[:, :, :, :, 3]
+    before = ops.launch_count()
+    acc, path, tokens = ops.tree_commit(data, cu, lens, tables, parents, draft, target, n)
+    assert ops.launch_count() - before == 2
+    assert bool((acc == 2).all()) and torch.equal(data, want)
+    assert bool((path == torch.tensor([0, 2, -1], **i32)).all())
+    assert bool((tokens == torch.tensor([2, 0, -1], **i32)).all())
+    ops.check_status(data.device)
