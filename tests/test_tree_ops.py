@@ -1168,3 +1168,106 @@ def test_tree_commit_of_more_sequences_than_a_grid_is_high():
     assert bool((path == torch.tensor([0, 2, -1], **i32)).all())
     assert bool((tokens == torch.tensor([2, 0, -1], **i32)).all())
     ops.check_status(data.device)
+
+
+class Spy:
+    """The tree operators of a model's steps, each call checked against the exact values."""
+
+    def __init__(self, monkeypatch, pool):
+        self.attn, self.commit, self.pool = ops.tree_attention, ops.tree_commit, pool
+        self.calls = {"attn": 0, "commit": 0}
+        monkeypatch.setattr(ops, "tree_attention", self.check_attn)
+        monkeypatch.setattr(ops, "tree_commit", self.check_commit)
+
+    @staticmethod
+    def batch(cu, lens, tables, parents):
+        b = Batch.__new__(Batch)
+        b.cu_list, b.tables = cu.tolist(), tables
+        b.nodes = [y - x for x, y in zip(b.cu_list, b.cu_list[1:])]
+        b.ctx = [n - k for n, k in zip(lens.tolist(), b.nodes)]
+        b.trees = [parents.tolist()[x:y] for x, y in zip(b.cu_list, b.cu_list[1:])]
+        return b
+
+    def check_attn(self, q, layer, cu, lens, tables, parents, max_q, scale, out):
+        got = self.attn(q, layer, cu, lens, tables, parents, max_q, scale, out)
+        b = self.batch(cu, lens, tables, parents)
+        b.q, b.layer, b.scale, b.nq, b.nkv = q, layer, scale, q.shape[1], layer.num_kv_heads
+        b.check(got)
+        self.calls["attn"] += 1
+        return got
+
+    def check_commit(self, data, cu, lens, tables, parents, draft, target, max_q, kv_scales=None, kv_side=None):
+        b = self.batch(cu, lens, tables, parents)
+        b.pool = self.pool
+        paths, toks = _commit_expect(b, draft, target)
+        kept = [t for t in (data, kv_scales, kv_side) if t is not None]
+        want = [_commit_moved(b, paths, t) for t in kept]
+        res = self.commit(data, cu, lens, tables, parents, draft, target, max_q, kv_scales=kv_scales, kv_side=kv_side)
+        assert res[0].tolist() == [len(p) for p in paths]
+        assert [t[:len(p)] for t, p in zip(res[2].tolist(), paths)] == toks
+        assert all(torch.equal(t, w) for t, w in zip(kept, want))
+        self.calls["commit"] += 1
+        return res
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 48])
+@pytest.mark.parametrize("mode", [None, "token", "channel"])
+def test_verify_steps_on_every_pool_gpu(monkeypatch, bs, mode):
+    """Verification steps of a model on bf16 and both int8 pools, with and without the tensor-core form."""
+    d = Decoder("cuda", PROMPTS, "tiny-moe-fp8", int8=mode == "token", bs=bs)
+    if mode == "channel":
+        a = d.args
+        d.pool = KVPool(d.pool.num_blocks, a.num_hidden_layers, a.num_key_value_heads, bs, a.head_dim, d.model.dtype,
+                        "cuda", int8=True, int8_mode="channel")
+        d.pool.calibrate_begin()
+        d.prefill()
+        torch.cuda.synchronize()
+        d.pool.calibrate_freeze(sum(len(p) - 1 for p in PROMPTS))
+        # two dimensions of every head in the side values, whatever the calibration found
+        d.pool.n_out.fill_(2)
+        d.pool.out_idx[..., 0], d.pool.out_idx[..., 1] = 1, a.head_dim - 2
+        for x in (1, a.head_dim - 2):
+            d.pool.ch_dscale[..., x] = 0
+    d.prefill()
+    spy = Spy(monkeypatch, d.pool)
+    g = torch.Generator().manual_seed(6)
+    truth = [t + list(range(1, 99)) for t in d.seqs]
+    for _ in range(2):
+        d.verify(*d.drafts(truth, 4, g))
+    assert spy.calls == {"attn": 2 * d.args.num_hidden_layers, "commit": 2}
+    ops.check_status(d.pool.data.device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_decode_and_tree_rows_in_one_step_gpu(monkeypatch, int8):
+    """Decode rows in front of tree rows: the tree rows of q, the output and the tables start behind them."""
+    d = Decoder("cuda", PROMPTS, "tiny-moe-fp8", int8=int8)
+    d.prefill()
+    spy = Spy(monkeypatch, d.pool)
+    decode, decoded = ops.decode_attention, []
+
+    def check_decode(q, layer, tables, lens, scale, out, split_len, nsplit, ws):
+        got = decode(q, layer, tables, lens, scale, out, split_len, nsplit, ws)
+        b = Spy.batch(torch.arange(q.shape[0] + 1), lens, tables, torch.full((q.shape[0],), -1))
+        b.q, b.layer, b.scale, b.nq, b.nkv = q, layer, scale, q.shape[1], layer.num_kv_heads
+        decoded.append((b, got.clone(), b.exact()))
+        return got
+
+    monkeypatch.setattr(ops, "decode_attention", check_decode)
+    g = torch.Generator().manual_seed(3)
+    trees = [_tree(n, "random", g) for n in (5, 8)]
+    rows = [(s, len(d.seqs[s]) - 1, 1) for s in (0, 1)] + [(s + 2, len(d.seqs[s + 2]) - 1, len(p))
+                                                           for s, p in enumerate(trees)]
+    toks = [d.seqs[0][-1], d.seqs[1][-1]] + [d.seqs[2][-1], 5, 6, 7, 8] + [d.seqs[3][-1]] + list(range(11, 18))
+    inp = d.inputs(rows, toks, [[-1], [-1]] + trees, num_decode=2)
+    inp.tree_parents = inp.tree_parents[2:].contiguous()
+    inp.prefill_cu = (inp.cu_seqlens_q[2:] - 2).contiguous()
+    h = d.model(inp, d.pool)
+    assert bool(torch.isfinite(h.float()).all())
+    assert spy.calls["attn"] == len(decoded) == d.args.num_hidden_layers
+    for b, got, (o, mass) in decoded:            # one query: the output and P rounded to bf16, as in Batch.check
+        lim = HALF * o.abs() + (2 * HALF + 2 ** -13) * mass + 1e-30
+        assert bool(((got.double().cpu() - o).abs() <= lim).all())
+    ops.check_status(d.pool.data.device)
