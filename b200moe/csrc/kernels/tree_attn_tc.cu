@@ -229,6 +229,13 @@ struct Row {
   int unit, item;      // units (parts, see Plan) and items in front of it
 };
 
+// First sequence with work that holds a row, else the last.  Not inlined: that cost the ragged batch 0.15 us.
+__device__ __noinline__ int holder(const Row* rows, int batch, int row) {
+  int b = 0;
+  while (b < batch - 1 && !(rows[b + 1].unit != rows[b].unit && rows[b].q0 <= row && row < rows[b + 1].q0)) ++b;
+  return b;
+}
+
 // The grid's work, in one of three ways:
 //   whole items    nothing is cut, several items to a CTA;
 //   parts          every item in equal parts of at most `parts` tiles, one part to a CTA (fewer items than CTAs);
@@ -420,6 +427,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_max_nt = reinterpret_cast<int*>(tmem_slot + 2);
   int* s_parts = s_max_nt + 1;
+  int* s_bad = s_max_nt + 2;              // a tree does not fit
   Row* rows = reinterpret_cast<Row*>(smem + L::TAB);
   volatile Seg* segs = reinterpret_cast<volatile Seg*>(smem + L::SEG);
   uint32_t* anc = reinterpret_cast<uint32_t*>(smem + L::ANC);
@@ -437,9 +445,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     tma_prefetch_desc(&q_map);
   }
   // ---- the work of every sequence; a tree that does not fit has none
-  if (threadIdx.x == 0) *s_max_nt = 0;
+  if (threadIdx.x == 0) *s_max_nt = *s_bad = 0;
   __syncthreads();
-  bool any_bad = false;
   for (int b = threadIdx.x; b < a.batch; b += kThreads) {
     const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seq_lens[b];
     const bool bad = !tree_fits(q0, q1, a.rows, a.max_q_len, len) ||
@@ -452,8 +459,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       r.unit = r.item * nt;
       atomicMax(s_max_nt, nt);
     }
-    if (bad) r.item = -1;
-    any_bad |= bad;
+    if (bad) *s_bad = 1;
     rows[b] = r;
     if (b == a.batch - 1) rows[b + 1].q0 = q1;
   }
@@ -483,25 +489,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     fence_barrier_init();
     *abort_flag = 0;
   }
-  if (__syncthreads_or(any_bad)) {
-    // The join looks rows up by their sequence's first one.  A bad tree in front of which another is bad
-    // has no offset to go by: it takes the end of the last good one, so that the offsets still ascend.
-    if (threadIdx.x == 0) {
-      int end = 0;
-      bool after_bad = true;
-      for (int b = 0; b < a.batch; ++b) {
-        const bool bad = rows[b].item < 0;
-        if (bad) {
-          rows[b].item = 0;
-          if (after_bad) rows[b].q0 = end;
-        } else {
-          end = rows[b + 1].q0;
-        }
-        after_bad = bad;
-      }
-    }
-    __syncthreads();
-  }
+  __syncthreads();
   if (warp == 0) {
     int units = 0, items = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
@@ -1071,6 +1059,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
   // ---- join the parts of items that a share cut: a lane per row (node and query head) and 16 columns
   if (plan.whole) return;
+  const bool any_bad = *s_bad;
   cg::this_grid().sync();
   const int nq = a.num_kv_heads * G, qrows = a.rows * G, groups = (qrows + 31) / 32;
   const int tasks = groups * a.num_kv_heads * (D / 16);
@@ -1084,6 +1073,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const int mid = (lo + up) >> 1;
       if (rows[mid].q0 <= row) lo = mid; else up = mid;
     }
+    if (any_bad) lo = holder(rows, a.batch, row);   // (offsets of a bad tree may lead that search astray)
     const int b = lo, unit0 = rows[b].unit;
     const int node = row - rows[b].q0;
     // nothing to do for a tree that was left out and for rows behind the last sequence
