@@ -37,10 +37,11 @@
 //
 // Bound by the weight stream where it is long: 16 tokens of 128 experts (hidden 2048, inner 768, top-8)
 // read 390 MB in 92 us, 64 tokens 595 MB in 143 us, 4.2 TB/s with about 15 us of logits, routing and
-// barriers.  One token (38 MB, 26 us) and small layers (12 us) are bound by the chain of launch, logits,
-// barrier, routing, two dependent streams and the last sums.
+// barriers.  One token (38 MB, 27 us) and small layers (12.5 us) are bound by the chain of launch, logits,
+// barrier, routing, two dependent streams and the last sums.  (Kernel times, 18 calls in a graph; in a long
+// row of calls 95, 152, 28.8 and 14.3 us, the 64 tokens at the clock that the card sustains.)
 //
-// Rounding points: the logits and the routing weights are rounded to bf16 (those of the
+// Rounding points: the logits (fp64 sums) and the routing weights are rounded to bf16 (those of the
 // model's router), the output once.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

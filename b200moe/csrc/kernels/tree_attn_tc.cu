@@ -31,11 +31,13 @@
 // that divides O adds the rounded values, which cancels that rounding where few keys
 // carry the weight.
 //
-// What bounds it.  64 chains of 4 nodes at 4k context: the cache, 542 MB in 96.6 us (5.6 TB/s).
-// 4 trees of 64 nodes at 32k, 16 query heads on a KV head: 272 GFLOP in 287 us, 0.58 of the bf16 peak; a
-// tile's chain S, softmax, P V, next S is as long as the softmax of a tile (about 2,100 cycles), and TMEM
-// has no room for a third S.  Smaller calls: setup, first loads, epilogue, barrier and join, 10 to 12 us
-// (one request at 500 context 12.4 us, 32 at 1.1k 26.7 us).
+// What bounds it (kernel times, 18 calls in a graph on a card that was idle before; calls in a long row of
+// them in brackets).  64 chains of 4 nodes at 4k context: the cache, 542 MB in 96.7 us, 5.6 TB/s [110 to 113].
+// 4 trees of 64 nodes at 32k, 16 query heads on a KV head: 272 GFLOP in 300 us, 0.56 of the bf16 burst peak
+// [353: 1000 W hold the card at 1.52 GHz, 0.56 of the bf16 peak that it sustains]; a tile's chain S, softmax,
+// P V, next S is as long as the softmax of a tile (about 2,100 cycles), and TMEM has no room for a third S.
+// Smaller calls: setup, first loads, epilogue, barrier and join, 10 to 12 us (one request at 500 context
+// 12.4 us [14.3], 32 at 1.1k 26.8 [28.7]; 13 ragged ones 17.3 to 22.3 by card [18.5]).
 //
 // A masked place never reaches the result: scores are selected, not added to, and a V
 // row is cleaned by its producer in front of the MMA (0 * NaN is NaN) -- rows behind the sequence become

@@ -19,8 +19,9 @@
 // its place (j' = path[j] > j), and moving in place is safe without a copy.
 //
 // Bound by latency: table, tree, walk and rows are four dependent reads.  One request of 8 nodes over 48
-// layers takes 4.1 us, 32 requests of up to 32 nodes (22 MB read and written) 8.9 us, 24 requests on an int8
-// pool with its scales 7.0 us.  A CTA takes 8 planes: with 4 the walks of twice the CTAs cost more than the
+// layers takes 4.1 us (kernel in a graph, 5.1 on the slowest card), 32 requests of up to 32 nodes (22 MB read and
+// written) 8.5 to 10.6 us, 24 requests on an int8 pool with its scales 7.1 to 8.1 us.  Calls in a row take 8.1,
+// 10.2 and 8.3 us, because the host needs 8.7 us for one: its checks, three outputs, the launch.  A CTA takes 8 planes: with 4 the walks of twice the CTAs cost more than the
 // copies gain (10.9 us for the 32 requests), with 16 the one request takes 5.0 us.
 #include <cuda_runtime.h>
 

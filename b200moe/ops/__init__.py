@@ -725,7 +725,8 @@ def tree_attention(q, kv_layer, cu_seqlens_q, seq_lens, block_tables, parents, m
     its tree, below the node's own; -1 for a node that follows the prefix directly.  max_q_len: no tree
     has more nodes (at most ``TREE_MAX_NODES``).  Chains (parents i - 1) give causal attention.  Rows
     behind the last sequence are left as they are.  bf16 and int8 pools, head_dim 64 or 128; out must
-    not overlap q.  int8 pools go through a bf16 stage of as many sequences at a time as ``TREE_STAGE_MAX_BYTES`` and
+    not overlap q.  Block sizes other than 8, 16, 32 and multiples of 64, and more than 128 query heads on a KV head,
+    take a form without tensor cores that is some 200 times slower.  int8 pools go through a bf16 stage of as many sequences at a time as ``TREE_STAGE_MAX_BYTES`` and
     ``INT8_STAGE_MAX_BYTES`` hold, at least one, each as long as its table row; a graph keeps the stage of a captured
     call.  block_tables may be a view of the first columns of a wider table, which makes it shorter.  A tree
     that does not fit (offsets outside q, more nodes than keys or than max_q_len, more keys than its
