@@ -762,3 +762,23 @@ def test_int8_channel_attention_decode_and_prefill(D, nq, nkv, bs):
     torch.cuda.synchronize()
     ops.check_status(DEV)
     torch.testing.assert_close(out.float(), ref, atol=2e-2, rtol=2e-2)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("D,nq,nkv,bs", [(128, 64, 4, 256), (128, 32, 4, 16), (64, 4, 2, 16), (128, 8, 8, 64)])
+def test_decode_attention_repeats_itself(D, nq, nkv, bs, int8):
+    """The same call gives the same bits: the parts of a sum are added in one order."""
+    seq_lens = [1, 17, 255, 401, 551, 1300]
+    B = len(seq_lens)
+    pool = _pool(sum(math.ceil(L / bs) for L in seq_lens) + 2, bs, nkv, D, int8=int8)
+    tables = _fill_pool(pool, seq_lens, bs, nkv, D, int8)
+    q = torch.randn(B, nq, D, device=DEV).to(torch.bfloat16)
+    lens = torch.tensor(seq_lens, dtype=torch.int32, device=DEV)
+    for split_len, nsplit in [(2048, 1), (64, 21)]:
+        ws = (torch.empty(B * nq * nsplit, D, device=DEV), torch.empty(B * nq * nsplit, device=DEV),
+              torch.empty(B * nq * nsplit, device=DEV))
+        out = torch.empty(100, B, nq, D, dtype=torch.bfloat16, device=DEV)
+        for o in out:
+            ops.decode_attention(q, pool.layer(1), tables, lens, D ** -0.5, o, split_len, nsplit, ws)
+        assert bool((out == out[0]).all())
+    ops.check_status(torch.device(DEV, 0))
